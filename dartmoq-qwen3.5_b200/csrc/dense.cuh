@@ -1,0 +1,61 @@
+// Dense products y = A B^T of the operators beside the packed experts: what a launch is given, and its epilogues.
+//
+//   kind 16-bit (bf16 or fp16, fp32 sums) or 8-bit integers (int32 sums); an operand is K-major (its rows run along K) or
+//   MN-major (its rows run along the output axis), as the caller's tensors lie in memory: nothing is transposed or copied.
+#pragma once
+#include "dense_ptx.cuh"
+
+namespace dense {
+
+enum Kind { KIND_16 = 0, KIND_I8 = 1 };
+enum Epi {
+  EPI_OUT = 0,        // out0 = v                                       (16-bit products)
+  EPI_SCALE = 1,      // out0 = v * a_scale[row] * b_scale[col] + bias  (8-bit products)
+  EPI_SILU = 2,       // g, u from two weights: out0 = silu(g) u
+  EPI_SILU_SAVE = 3,  // the same, and out1 = silu(g), out2 = u silu'(g): what the gradients need
+  EPI_GRAD = 4        // v = dh: out0 = dh * in1 (= u silu'(g)), out1 = dh * in0 (= silu(g))
+};
+constexpr __host__ __device__ bool is_dual(int epi) { return epi == EPI_SILU || epi == EPI_SILU_SAVE; }
+
+struct Maps {
+  CUtensorMap a[2], b[2];
+};
+
+struct Args {
+  int M, N, K;              // output rows, output columns (of one of the two products when dual), length of a K segment
+  int segs;                 // K segments: segment s multiplies a[s] by b[s], all into one sum
+  int bf16;                 // 16-bit type of inputs and outputs: bf16, else fp16
+  int vec;                  // outputs (and in0 / in1) may be accessed four elements at a time
+  const float* a_scale;     // 8-bit: one per row
+  const float* b_scale[2];  // 8-bit: one per column (of each product when dual)
+  const uint16_t* bias;     // 8-bit, optional, type of the output
+  const uint16_t *in0, *in1;
+  uint16_t *out0, *out1, *out2;
+  long long ld_in, ld_out;  // row pitches in elements
+};
+
+// One output element's value: v0 (and v1 of the second product) are the sums.
+// The gradient of silu: silu'(g) = s (1 + g (1 - s)), s = sigmoid(g).
+template <int KIND, int EPI>
+__device__ __forceinline__ void finish(const Args& a, long long row, int col, uint32_t v0, uint32_t v1, float sa, float (&o)[3]) {
+  float x = (KIND == KIND_I8) ? (float)(int)v0 : __uint_as_float(v0);
+  float y = (KIND == KIND_I8) ? (float)(int)v1 : __uint_as_float(v1);
+  if (KIND == KIND_I8) {
+    x *= sa * a.b_scale[0][col];
+    if (is_dual(EPI)) y *= sa * a.b_scale[1][col];
+  }
+  if (EPI == EPI_OUT) {
+    o[0] = x;
+  } else if (EPI == EPI_SCALE) {
+    o[0] = a.bias ? x + unpack16(a.bias[col], a.bf16) : x;
+  } else if (EPI == EPI_SILU) {
+    o[0] = x * sigmoid(x) * y;
+  } else if (EPI == EPI_SILU_SAVE) {
+    const float s = sigmoid(x), si = x * s;
+    o[0] = si * y;
+    o[1] = si;
+    o[2] = y * (s + si * (1.f - s));
+  }
+}
+
+}  // namespace dense

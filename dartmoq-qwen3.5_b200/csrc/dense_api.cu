@@ -1,0 +1,275 @@
+// C entry points of the dense operators: argument checks, tensor maps, choice of the kernel.
+#include "dense.cuh"
+
+namespace dense {
+
+int tile_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, const Args& a, int splits, cudaStream_t s);
+
+namespace {
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_tiled_fn() {
+  static EncodeTiledFn fn = nullptr;
+  if (fn == nullptr) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+      return nullptr;
+    fn = reinterpret_cast<EncodeTiledFn>(p);
+  }
+  return fn;
+}
+
+// A matrix of `rows` rows of `cols` elements (1 or 2 bytes), `pitch` elements apart.
+struct Matrix {
+  const void* p;
+  long long rows, cols, pitch;
+};
+
+// Every check comes before the first launch of a call.
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool tma_ok(const Matrix& m, int es) { return aligned16(m.p) && (m.pitch * es) % 16 == 0 && m.pitch >= m.cols; }
+
+// Copied in boxes of 128 bytes x box_rows rows with the 128-byte swizzle; what lies past the matrix reads as zero.
+int make_map(CUtensorMap* map, const Matrix& m, int es, int box_rows) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (fn == nullptr) return DMOQ_EDEVICE;
+  const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)m.pitch * es};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / es), (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  auto encode = [&] {
+    return fn(map, es == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(m.p), dims,
+              strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult rc = encode();
+  if (rc == CUDA_ERROR_INVALID_CONTEXT || rc == CUDA_ERROR_NOT_INITIALIZED) {
+    // a thread that has made no runtime call yet (autograd runs backward passes on threads of its own) has no context bound
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return DMOQ_EDEVICE;
+    rc = encode();
+  }
+  return rc == CUDA_SUCCESS ? DMOQ_OK : DMOQ_EINVAL;
+}
+
+// A product of operands as they lie in memory: a_mn / b_mn say that a matrix runs along the output axis (its rows are K).
+struct Product {
+  int kind = KIND_16, epi = EPI_OUT;
+  bool a_mn = false, b_mn = false;
+  Matrix a[2] = {}, b[2] = {};
+  Args args = {};
+};
+
+int run(const Product& p, cudaStream_t s) {
+  const int es = p.kind == KIND_I8 ? 1 : 2, bk = 128 / es;
+  const int cols = is_dual(p.epi) ? 64 : 128;
+  const long long tiles = (long long)dmoq_ceil_div(p.args.M, 128) * dmoq_ceil_div(p.args.N, cols);
+  const int steps = dmoq_ceil_div(p.args.K, bk) * p.args.segs;
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= dmoq_sm_count() && steps >= splits * 8) splits *= 2;
+  Maps maps;
+  const int n_a = p.args.segs, n_b = is_dual(p.epi) ? 2 : p.args.segs;
+  for (int i = 0; i < 2; ++i) {
+    const Matrix& a = p.a[i < n_a ? i : 0];
+    const Matrix& b = p.b[i < n_b ? i : 0];
+    if (!tma_ok(a, es) || !tma_ok(b, es)) return DMOQ_EINVAL;
+    int rc = make_map(&maps.a[i], a, es, p.a_mn ? bk : 128);
+    if (rc == DMOQ_OK) rc = make_map(&maps.b[i], b, es, p.b_mn ? bk : cols);
+    if (rc != DMOQ_OK) return rc;
+  }
+  return tile_product(p.kind, p.a_mn, p.b_mn, p.epi, maps, p.args, splits, s);
+}
+
+// four-element accesses to a 16-bit matrix
+bool vec4(const void* p, long long n, long long pitch) { return reinterpret_cast<uintptr_t>(p) % 8 == 0 && n % 4 == 0 && pitch % 4 == 0; }
+
+constexpr int kMaxK8 = 131056;   // |sum of K products of codes| <= 128 * 128 K stays inside 32 bits
+
+bool usable(const void* p) { return p != nullptr && aligned16(p); }
+bool rows_usable(const void* p, long long pitch, int cols) { return usable(p) && pitch >= cols && pitch % 8 == 0; }   // 16-bit rows
+
+int check_sizes8(int T, int N, int K) {
+  if (T < 0 || N < 1 || K < 16 || K % 16 != 0) return DMOQ_EINVAL;
+  return K > kMaxK8 ? DMOQ_ESIZE : DMOQ_OK;
+}
+bool quant_ok(const void* x, long long pitch, int K, const void* codes, const void* scales) {
+  return rows_usable(x, pitch, K) && usable(codes) && scales;
+}
+bool weight8_ok(const void* w, const void* scale) { return usable(w) && scale; }
+bool ffn_sizes_ok(int T, int H, int I) { return T >= 0 && H >= 8 && I >= 8 && H % 8 == 0 && I % 8 == 0 && I <= (1 << 30); }
+
+int int8_product(const int8_t* codes, const float* scales, const int8_t* w0, const float* s0, const int8_t* w1, const float* s1,
+                 const void* bias, int bf16, int T, int N, int K, void* out, cudaStream_t s) {
+  Product p;
+  p.kind = KIND_I8;
+  p.epi = w1 ? EPI_SILU : EPI_SCALE;
+  p.a[0] = {codes, T, K, K};
+  p.b[0] = {w0, N, K, K};
+  if (w1) p.b[1] = {w1, N, K, K};
+  Args& a = p.args;
+  a.M = T, a.N = N, a.K = K, a.segs = 1, a.bf16 = bf16;
+  a.a_scale = scales, a.b_scale[0] = s0, a.b_scale[1] = s1;
+  a.bias = static_cast<const uint16_t*>(bias);
+  a.out0 = static_cast<uint16_t*>(out);
+  a.ld_out = N;
+  a.vec = vec4(out, N, N);
+  return run(p, s);
+}
+
+}  // namespace
+}  // namespace dense
+
+int dmoq_token_quant_launch(const void* x, int bf16, int T, int K, long long pitch, int8_t* codes, float* scales, cudaStream_t s);
+
+using namespace dense;
+
+extern "C" int dmoq_token_quant(const void* x, int32_t is_bf16, int32_t T, int32_t K, int64_t x_pitch, int8_t* codes, float* scales,
+                                void* stream) {
+  DMOQ_CHECK_ARG(T >= 0 && K >= 16 && K % 16 == 0);
+  if (T == 0) return DMOQ_OK;
+  DMOQ_CHECK_ARG(quant_ok(x, x_pitch, K, codes, scales));
+  return dmoq_token_quant_launch(x, is_bf16, T, K, x_pitch, codes, scales, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int dmoq_int8_gemm(const int8_t* codes, const float* scales, const int8_t* w, const float* w_scale, const void* bias,
+                              int32_t is_bf16, int32_t T, int32_t N, int32_t K, void* out, void* stream) {
+  const int rc = check_sizes8(T, N, K);
+  if (rc != DMOQ_OK || T == 0) return rc;
+  DMOQ_CHECK_ARG(usable(codes) && scales && weight8_ok(w, w_scale) && out);
+  return int8_product(codes, scales, w, w_scale, nullptr, nullptr, bias, is_bf16, T, N, K, out, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int dmoq_int8_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w, const float* w_scale, const void* bias,
+                                int32_t T, int32_t N, int32_t K, int8_t* codes, float* scales, void* out, void* stream) {
+  const int rc = check_sizes8(T, N, K);
+  if (rc != DMOQ_OK || T == 0) return rc;
+  DMOQ_CHECK_ARG(quant_ok(x, x_pitch, K, codes, scales) && weight8_ok(w, w_scale) && out);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int rq = dmoq_token_quant_launch(x, is_bf16, T, K, x_pitch, codes, scales, s);
+  if (rq != DMOQ_OK) return rq;
+  return int8_product(codes, scales, w, w_scale, nullptr, nullptr, bias, is_bf16, T, N, K, out, s);
+}
+
+extern "C" int dmoq_int8_gated_gemm(const int8_t* codes, const float* scales, const int8_t* w_gate, const float* gate_scale,
+                                    const int8_t* w_up, const float* up_scale, int32_t is_bf16, int32_t T, int32_t I, int32_t K,
+                                    void* out, void* stream) {
+  const int rc = check_sizes8(T, I, K);
+  if (rc != DMOQ_OK || T == 0) return rc;
+  DMOQ_CHECK_ARG(usable(codes) && scales && weight8_ok(w_gate, gate_scale) && weight8_ok(w_up, up_scale) && out);
+  return int8_product(codes, scales, w_gate, gate_scale, w_up, up_scale, nullptr, is_bf16, T, I, K, out, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int dmoq_int8_gated_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w_gate, const float* gate_scale,
+                                      const int8_t* w_up, const float* up_scale, int32_t T, int32_t I, int32_t K, int8_t* codes,
+                                      float* scales, void* out, void* stream) {
+  const int rc = check_sizes8(T, I, K);
+  if (rc != DMOQ_OK || T == 0) return rc;
+  DMOQ_CHECK_ARG(quant_ok(x, x_pitch, K, codes, scales) && weight8_ok(w_gate, gate_scale) && weight8_ok(w_up, up_scale) && out);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int rq = dmoq_token_quant_launch(x, is_bf16, T, K, x_pitch, codes, scales, s);
+  if (rq != DMOQ_OK) return rq;
+  return int8_product(codes, scales, w_gate, gate_scale, w_up, up_scale, nullptr, is_bf16, T, I, K, out, s);
+}
+
+extern "C" int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate, const void* w_up, const void* w_down,
+                              int32_t T, int32_t H, int32_t I, void* h, void* silu, void* slope, void* y, void* stream) {
+  DMOQ_CHECK_ARG(ffn_sizes_ok(T, H, I));
+  DMOQ_CHECK_ARG((silu == nullptr) == (slope == nullptr));
+  if (T == 0) return DMOQ_OK;
+  DMOQ_CHECK_ARG(rows_usable(x, x_pitch, H) && usable(w_gate) && usable(w_up) && usable(w_down) && usable(h) && usable(y));
+  DMOQ_CHECK_ARG(aligned16(silu) && aligned16(slope));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  Product up;
+  up.epi = silu ? EPI_SILU_SAVE : EPI_SILU;
+  up.a[0] = {x, T, H, x_pitch};
+  up.b[0] = {w_gate, I, H, H};
+  up.b[1] = {w_up, I, H, H};
+  up.args.M = T, up.args.N = I, up.args.K = H, up.args.segs = 1, up.args.bf16 = is_bf16, up.args.vec = 1;
+  up.args.out0 = static_cast<uint16_t*>(h);
+  up.args.out1 = static_cast<uint16_t*>(silu);
+  up.args.out2 = static_cast<uint16_t*>(slope);
+  up.args.ld_out = I;
+  int rc = run(up, s);
+  if (rc != DMOQ_OK) return rc;
+  Product down;
+  down.a[0] = {h, T, I, I};
+  down.b[0] = {w_down, H, I, I};
+  down.args.M = T, down.args.N = H, down.args.K = I, down.args.segs = 1, down.args.bf16 = is_bf16, down.args.vec = 1;
+  down.args.out0 = static_cast<uint16_t*>(y);
+  down.args.ld_out = H;
+  return run(down, s);
+}
+
+extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate,
+                                       const void* w_up, const void* w_down, int32_t T, int32_t H, int32_t I, const void* h,
+                                       const void* silu, const void* slope, void* d_gate_up, void* dx, void* dw_gate, void* dw_up,
+                                       void* dw_down, void* stream) {
+  DMOQ_CHECK_ARG(ffn_sizes_ok(T, H, I));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const size_t w_bytes = (size_t)H * I * 2;
+  if (T == 0) {   // no tokens: the weights' gradients are zero
+    void* dw[3] = {dw_gate, dw_up, dw_down};
+    for (void* p : dw)
+      if (p && cudaMemsetAsync(p, 0, w_bytes, s) != cudaSuccess) return DMOQ_ELAUNCH;
+    return DMOQ_OK;
+  }
+  const bool inner = dx || dw_gate || dw_up;    // anything behind the hidden values
+  DMOQ_CHECK_ARG(aligned16(dx) && aligned16(dw_gate) && aligned16(dw_up) && aligned16(dw_down));
+  DMOQ_CHECK_ARG(!(inner || dw_down) || rows_usable(dy, dy_pitch, H));
+  DMOQ_CHECK_ARG(!dw_down || usable(h));
+  DMOQ_CHECK_ARG(!inner || (usable(w_down) && usable(silu) && usable(slope) && usable(d_gate_up)));
+  DMOQ_CHECK_ARG(!dx || (usable(w_gate) && usable(w_up)));
+  DMOQ_CHECK_ARG(!(dw_gate || dw_up) || rows_usable(x, x_pitch, H));
+  uint16_t* dg = static_cast<uint16_t*>(d_gate_up);
+  int rc = DMOQ_OK;
+  if (inner) {   // dh = dy Wd; dg = dh u silu'(g), du = dh silu(g), side by side in rows of 2 I
+    Product p;
+    p.epi = EPI_GRAD;
+    p.b_mn = true;
+    p.a[0] = {dy, T, H, dy_pitch};
+    p.b[0] = {w_down, H, I, I};
+    p.args.M = T, p.args.N = I, p.args.K = H, p.args.segs = 1, p.args.bf16 = is_bf16, p.args.vec = 1;
+    p.args.in0 = static_cast<const uint16_t*>(silu);
+    p.args.in1 = static_cast<const uint16_t*>(slope);
+    p.args.ld_in = I;
+    p.args.out0 = dg;
+    p.args.out1 = dg + I;
+    p.args.ld_out = 2 * (long long)I;
+    if ((rc = run(p, s)) != DMOQ_OK) return rc;
+  }
+  if (dx) {      // dx = dg Wg + du Wu: one sum over two K segments
+    Product p;
+    p.b_mn = true;
+    p.a[0] = {dg, T, I, 2 * (long long)I};
+    p.a[1] = {dg + I, T, I, 2 * (long long)I};
+    p.b[0] = {w_gate, I, H, H};
+    p.b[1] = {w_up, I, H, H};
+    p.args.M = T, p.args.N = H, p.args.K = I, p.args.segs = 2, p.args.bf16 = is_bf16, p.args.vec = 1;
+    p.args.out0 = static_cast<uint16_t*>(dx);
+    p.args.ld_out = H;
+    if ((rc = run(p, s)) != DMOQ_OK) return rc;
+  }
+  auto weight_grad = [&](const Matrix& a, const Matrix& b, void* out) {   // a^T b, both along the tokens
+    Product p;
+    p.a_mn = p.b_mn = true;
+    p.a[0] = a;
+    p.b[0] = b;
+    p.args.M = (int)a.cols, p.args.N = (int)b.cols, p.args.K = T, p.args.segs = 1, p.args.bf16 = is_bf16, p.args.vec = 1;
+    p.args.out0 = static_cast<uint16_t*>(out);
+    p.args.ld_out = b.cols;
+    return run(p, s);
+  };
+  const Matrix xm = {x, T, H, x_pitch};
+  if (dw_gate && dw_up && static_cast<char*>(dw_up) == static_cast<char*>(dw_gate) + w_bytes) {   // one product for both halves
+    if ((rc = weight_grad({dg, T, 2 * (long long)I, 2 * (long long)I}, xm, dw_gate)) != DMOQ_OK) return rc;
+  } else {
+    if (dw_gate && (rc = weight_grad({dg, T, I, 2 * (long long)I}, xm, dw_gate)) != DMOQ_OK) return rc;
+    if (dw_up && (rc = weight_grad({dg + I, T, I, 2 * (long long)I}, xm, dw_up)) != DMOQ_OK) return rc;
+  }
+  if (dw_down) rc = weight_grad({dy, T, H, dy_pitch}, {h, T, I, I}, dw_down);
+  return rc;
+}

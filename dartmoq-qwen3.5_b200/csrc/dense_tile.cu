@@ -1,0 +1,266 @@
+// Dense products on the tensor cores, one 128-row output tile a cluster: the K axis is split over the cluster's blocks and
+// their partial sums are joined through distributed shared memory, in rank order, so that a result does not depend on
+// timing.
+//
+// A block multiplies its share of K steps (128 bytes of K each) into one TMEM accumulator: warp 0 brings the operand boxes in
+// by TMA, warp 1 issues tcgen05.mma, warps 4-7 take the accumulator to shared memory (over the operand stages, which are
+// idle by then); after a cluster barrier every block finishes 128 / splits rows of the tile.
+#include "dense.cuh"
+
+__device__ int g_dmoq_dense_status = 0;
+
+namespace dense {
+namespace {
+
+template <int BN>
+struct TileCfg {
+  static constexpr int kStageBytes = 128 * 128 + BN * 128;
+  static constexpr int kStages = BN == 256 ? 4 : 6;
+  static constexpr int kPitch = BN * 4 + 16;              // accumulator rows in shared memory: 16 bytes of padding against bank conflicts
+  static constexpr int kBar = kStages * kStageBytes;      // barriers after the stages
+  static constexpr int kSmem = kBar + 256 + 1024;
+  static_assert(128 * kPitch <= kBar, "the accumulator rows lie over the operand stages");
+};
+
+template <int KIND, bool AMN, bool BMN, int EPI, int BN>
+__global__ void __launch_bounds__(256, 1) dense_tile_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args a) {
+  using C = TileCfg<BN>;
+  constexpr bool kDual = is_dual(EPI);
+  constexpr int kCols = kDual ? BN / 2 : BN;              // output columns of the tile
+  constexpr int kBK = KIND == KIND_I8 ? 128 : 64;         // elements of K in a step
+  constexpr int kStages = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t sb = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  auto stage_a = [&](uint32_t s) { return sb + s * C::kStageBytes; };
+  auto stage_b = [&](uint32_t s) { return sb + s * C::kStageBytes + 128 * 128; };
+  auto bar_full = [&](uint32_t s) { return sb + C::kBar + 8 * s; };
+  auto bar_empty = [&](uint32_t s) { return sb + C::kBar + 64 + 8 * s; };
+  const uint32_t bar_acc = sb + C::kBar + 128, tmem_slot = sb + C::kBar + 136, abort_flag = sb + C::kBar + 140;
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const uint32_t rank = cluster_rank(), splits = cluster_size();
+  const int tiles_n = (a.N + kCols - 1) / kCols;
+  const int tile = blockIdx.x / splits;
+  const int m0 = tile / tiles_n * 128, n0 = tile % tiles_n * kCols;
+  const int seg_steps = (a.K + kBK - 1) / kBK;
+  const int steps = seg_steps * a.segs;
+  const int it0 = (int)((long long)steps * rank / splits), it1 = (int)((long long)steps * (rank + 1) / splits);
+
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar_full(s), 1);
+      mbar_init(bar_empty(s), 1);
+    }
+    mbar_init(bar_acc, 1);
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(abort_flag), "r"(0) : "memory");
+    mbar_init_fence();
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(BN));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int done = 0;
+      for (int it = it0; it < it1; ++it, ++done) {
+        const uint32_t s = done % kStages;
+        if (done >= kStages && !mbar_wait(bar_empty(s), (done / kStages - 1) & 1, abort_flag, &g_dmoq_dense_status)) break;
+        const int seg = it >= seg_steps ? 1 : 0, k = (it - seg * seg_steps) * kBK;
+        mbar_arrive_expect_tx(bar_full(s), C::kStageBytes);
+        if (AMN) {
+          tma_load(stage_a(s), &maps.a[seg], m0, k, bar_full(s));
+          tma_load(stage_a(s) + 8192, &maps.a[seg], m0 + 64, k, bar_full(s));
+        } else {
+          tma_load(stage_a(s), &maps.a[seg], k, m0, bar_full(s));
+        }
+        if (BMN) {
+#pragma unroll
+          for (int j = 0; j < BN / 64; ++j) tma_load(stage_b(s) + 8192 * j, &maps.b[seg], n0 + 64 * j, k, bar_full(s));
+        } else if (kDual) {
+          tma_load(stage_b(s), &maps.b[0], k, n0, bar_full(s));
+          tma_load(stage_b(s) + BN * 64, &maps.b[1], k, n0, bar_full(s));
+        } else {
+          tma_load(stage_b(s), &maps.b[seg], k, n0, bar_full(s));
+        }
+      }
+      // nothing may still be on its way into this block's shared memory when it is reused or the block ends (matters after an abort)
+      for (int j = done > kStages ? done - kStages : 0; j < done; ++j) mbar_wait_quiet(bar_full(j % kStages), (j / kStages) & 1);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t shape = ((uint32_t)(BN >> 3) << 17) | (8u << 24);
+      const uint32_t type = a.bf16 ? 1u : 0u;
+      const uint32_t idesc = KIND == KIND_I8 ? (2u << 4) | (1u << 7) | (1u << 10) | shape
+                                             : (1u << 4) | (type << 7) | (type << 10) | (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u) | shape;
+      // 32 bytes of K an instruction: 32 bytes along a K-major row, sixteen 128-byte rows of an MN-major tile
+      constexpr uint32_t step_a = AMN ? 128 : 2, step_b = BMN ? 128 : 2;
+      for (int done = 0; done < it1 - it0; ++done) {
+        const uint32_t s = done % kStages;
+        if (!mbar_wait(bar_full(s), (done / kStages) & 1, abort_flag, &g_dmoq_dense_status)) break;
+        tc_fence_after();
+        const uint64_t da = operand_desc(stage_a(s), AMN ? 8192 : 16), db = operand_desc(stage_b(s), BMN ? 8192 : 16);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t acc = (done > 0 || k > 0) ? 1u : 0u;
+          if (KIND == KIND_I8) {
+            asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
+                         "l"(da + step_a * k), "l"(db + step_b * k), "r"(idesc), "r"(acc)
+                         : "memory");
+          } else {
+            asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
+                         "l"(da + step_a * k), "l"(db + step_b * k), "r"(idesc), "r"(acc)
+                         : "memory");
+          }
+        }
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_empty(s)) : "memory");
+      }
+      asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_acc) : "memory");
+    }
+  } else if (warp >= 4) {
+    mbar_wait(bar_acc, 0, abort_flag, &g_dmoq_dense_status);
+    if (flag_get(abort_flag)) mbar_wait_quiet(bar_acc, 0);
+    tc_fence_after();
+    const int w = warp - 4;
+    const uint32_t row = sb + (uint32_t)(w * 32 + lane) * C::kPitch;
+#pragma unroll 1
+    for (int c = 0; c < BN; c += 32) {
+      uint32_t v[32];
+      tc_ld32(tmem + ((uint32_t)(w * 32) << 16) + c, v);
+      tc_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) st_shared_v4(row + (c + i) * 4, v[i], v[i + 1], v[i + 2], v[i + 3]);
+    }
+    tc_fence_before();
+  }
+  __syncwarp();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(BN));
+  }
+  if (splits > 1) cluster_sync();
+
+  // join and finish: this block's rows of the tile, four columns a thread
+  constexpr int kQuads = kCols / 4;
+  const int row_lo = 128 * rank / splits, row_hi = 128 * (rank + 1) / splits;
+  for (int i = row_lo * kQuads + tid; i < row_hi * kQuads; i += 256) {
+    const int r = i / kQuads, c = i % kQuads * 4;
+    const long long row = m0 + r;
+    const int col = n0 + c;
+    if (row >= a.M || col >= a.N) continue;
+    uint32_t v[4] = {0u, 0u, 0u, 0u}, u[4] = {0u, 0u, 0u, 0u};
+    for (uint32_t q = 0; q < splits; ++q) {
+      const uint32_t at = map_to_rank(sb, q) + r * C::kPitch + c * 4;
+      auto add = [&](uint32_t(&t)[4], const uint4 p) {
+        const uint32_t e[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          t[j] = KIND == KIND_I8 ? t[j] + e[j] : __float_as_uint(__uint_as_float(t[j]) + __uint_as_float(e[j]));
+      };
+      add(v, ld_cluster_v4(at));
+      if (kDual) add(u, ld_cluster_v4(at + kCols * 4));
+    }
+    const int n = min(4, a.N - col);
+    const float sa = KIND == KIND_I8 ? a.a_scale[row] : 1.f;
+    const long long at_out = row * a.ld_out + col;
+    float o[3][4];
+    if (EPI == EPI_GRAD) {
+      const long long at_in = row * a.ld_in + col;
+      uint32_t s[4], p[4];
+      if (a.vec) {
+        const uint2 s2 = *reinterpret_cast<const uint2*>(a.in0 + at_in), p2 = *reinterpret_cast<const uint2*>(a.in1 + at_in);
+        s[0] = s2.x & 0xffffu, s[1] = s2.x >> 16, s[2] = s2.y & 0xffffu, s[3] = s2.y >> 16;
+        p[0] = p2.x & 0xffffu, p[1] = p2.x >> 16, p[2] = p2.y & 0xffffu, p[3] = p2.y >> 16;
+      } else {
+        for (int j = 0; j < 4; ++j) s[j] = j < n ? a.in0[at_in + j] : 0u, p[j] = j < n ? a.in1[at_in + j] : 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        o[0][j] = __uint_as_float(v[j]) * unpack16(p[j], a.bf16);
+        o[1][j] = __uint_as_float(v[j]) * unpack16(s[j], a.bf16);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float e[3] = {0.f, 0.f, 0.f};
+        if (j < n) finish<KIND, EPI>(a, row, col + j, v[j], u[j], sa, e);
+        o[0][j] = e[0], o[1][j] = e[1], o[2][j] = e[2];
+      }
+    }
+    constexpr int kOuts = EPI == EPI_SILU_SAVE ? 3 : EPI == EPI_GRAD ? 2 : 1;
+    uint16_t* outs[3] = {a.out0, a.out1, a.out2};
+#pragma unroll
+    for (int e = 0; e < kOuts; ++e) {
+      const uint32_t lo = pack16(o[e][0], o[e][1], a.bf16), hi = pack16(o[e][2], o[e][3], a.bf16);
+      uint16_t* dst = outs[e] + at_out;
+      if (a.vec) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+      } else {
+        const uint32_t h[4] = {lo & 0xffffu, lo >> 16, hi & 0xffffu, hi >> 16};
+        for (int j = 0; j < n; ++j) dst[j] = (uint16_t)h[j];
+      }
+    }
+  }
+  if (splits > 1) cluster_sync();   // a block's shared memory lives until the others have read it
+}
+
+template <int KIND, bool AMN, bool BMN, int EPI, int BN>
+int launch(const Maps& maps, const Args& a, int splits, cudaStream_t s) {
+  using C = TileCfg<BN>;
+  static DmoqOncePerDevice once;
+  bool* configured = once.slot();
+  if (configured == nullptr) return DMOQ_EDEVICE;
+  auto* kernel = dense_tile_kernel<KIND, AMN, BMN, EPI, BN>;
+  if (!*configured) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess) return DMOQ_ELAUNCH;
+    *configured = true;
+  }
+  constexpr int kCols = is_dual(EPI) ? BN / 2 : BN;
+  const long long blocks = (long long)dmoq_ceil_div(a.M, 128) * dmoq_ceil_div(a.N, kCols) * splits;
+  if (blocks > 0x7fffffffLL) return DMOQ_ESIZE;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, maps, a) == cudaSuccess ? DMOQ_OK : DMOQ_ELAUNCH;
+}
+
+}  // namespace
+
+int tile_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, const Args& a, int splits, cudaStream_t s) {
+  const int key = kind * 1000 + a_mn * 200 + b_mn * 100 + epi;
+  switch (key) {
+    case EPI_OUT: return launch<KIND_16, false, false, EPI_OUT, 128>(maps, a, splits, s);
+    case EPI_SILU: return launch<KIND_16, false, false, EPI_SILU, 128>(maps, a, splits, s);
+    case EPI_SILU_SAVE: return launch<KIND_16, false, false, EPI_SILU_SAVE, 128>(maps, a, splits, s);
+    case 100 + EPI_OUT: return launch<KIND_16, false, true, EPI_OUT, 128>(maps, a, splits, s);
+    case 100 + EPI_GRAD: return launch<KIND_16, false, true, EPI_GRAD, 128>(maps, a, splits, s);
+    case 300 + EPI_OUT: return launch<KIND_16, true, true, EPI_OUT, 128>(maps, a, splits, s);
+    case 1000 + EPI_SCALE: return launch<KIND_I8, false, false, EPI_SCALE, 128>(maps, a, splits, s);
+    case 1000 + EPI_SILU: return launch<KIND_I8, false, false, EPI_SILU, 128>(maps, a, splits, s);
+    default: return DMOQ_EINVAL;
+  }
+}
+
+}  // namespace dense
+
+int dmoq_dense_status(int* out) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_dmoq_dense_status, sizeof(int)) != cudaSuccess) return DMOQ_EDEVICE;
+  *out = v;
+  return DMOQ_OK;
+}

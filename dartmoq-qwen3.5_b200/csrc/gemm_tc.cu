@@ -924,6 +924,7 @@ extern "C" int dmoq_tc_profile(unsigned long long* out32, int reset) {
 #endif
 
 int dmoq_img_status(int* out);
+int dmoq_dense_status(int* out);
 
 // Device status word of the tensor-core kernels (both kernel families): 0 = no bounded wait has ever timed out on
 // this device.
@@ -933,6 +934,9 @@ extern "C" int dmoq_tc_status(int32_t* status_host) {
   if (cudaMemcpyFromSymbol(&v, g_dmoq_tc_status, sizeof(int)) != cudaSuccess) return DMOQ_EDEVICE;
   const int rc = dmoq_img_status(&w);
   if (rc != DMOQ_OK) return rc;
-  *status_host = v | w;
+  int d = 0;
+  const int rd = dmoq_dense_status(&d);
+  if (rd != DMOQ_OK) return rd;
+  *status_host = v | w | d;
   return DMOQ_OK;
 }

@@ -7,6 +7,8 @@ Same storage and constructor as the reference classes
 state_dict keys: ``packed_indices`` (uint8), ``norms`` (fp16), ``codebook`` (fp16), optional ``bias``.
 ``forward`` = group rotation (+ activation quantisation) followed by the same
 grouped LUT-dequant GEMM the MoE uses, run as a single "expert" over all rows.
+
+``W8A8Linear`` beside them stores plain 8-bit weights: no rotation and no codebook, one scale a weight row and one a token.
 """
 from __future__ import annotations
 
@@ -18,6 +20,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
+from . import dense
 from . import format as fmt
 from . import kernels as K
 from ._lib import A16, A8, FP8, EPI_PLAIN
@@ -143,3 +146,56 @@ class WxA8Linear(WxA16Linear):
 class WxFP8Linear(WxA16Linear):
     """e4m3 activations and an e4m3 codebook LUT."""
     MODE = FP8
+
+
+class W8A8Linear(nn.Module):
+    """y = x @ W^T (+ bias) with W in 8-bit integers (one fp32 scale a row) and x quantised a token at a time.
+
+    state_dict keys: ``weight`` (int8 (out, in)), ``weight_scale`` (fp32 (out,)), optional ``bias`` (the activations' 16-bit type).
+    ``in_features`` is a multiple of 16."""
+
+    def __init__(self, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None):
+        super().__init__()
+        if weight.dtype != torch.int8 or weight_scale.dtype != torch.float32:
+            raise TypeError(f"weight must be int8 with an fp32 scale, got {weight.dtype} and {weight_scale.dtype}")
+        if weight.dim() != 2 or tuple(weight_scale.shape) != (weight.shape[0],):
+            raise ValueError(f"weight must be a matrix with one scale a row, got {tuple(weight.shape)} and "
+                             f"{tuple(weight_scale.shape)}")
+        self.out_features, self.in_features = weight.shape
+        if self.in_features % 16:
+            raise ValueError(f"in_features must be a multiple of 16, got {self.in_features}")
+        self.register_buffer("weight", weight)
+        self.register_buffer("weight_scale", weight_scale)
+        if bias is not None:
+            self.register_buffer("bias", bias)
+        else:
+            self.bias = None
+
+    @classmethod
+    @torch.no_grad()
+    def from_linear(cls, linear: nn.Linear) -> "W8A8Linear":
+        """Quantise a 16-bit ``nn.Linear`` on a CUDA device, row by row, with the tokens' own quantiser."""
+        codes, scale = dense.quantize_int8_tokens(linear.weight.data)
+        return cls(codes, scale, linear.bias.data.clone() if linear.bias is not None else None)
+
+    @classmethod
+    def from_metadata(cls, meta: dict) -> "W8A8Linear":
+        """Placeholder buffers of the saved shapes; the state dict fills them."""
+        n, k = meta["out_features"], meta["in_features"]
+        dtype = getattr(torch, str(meta.get("orig_dtype", "torch.bfloat16")).split(".")[-1])
+        return cls(torch.empty((n, k), dtype=torch.int8), torch.empty((n,), dtype=torch.float32),
+                   torch.empty((n,), dtype=dtype) if meta.get("bias_shape") else None)
+
+    def _apply(self, fn, *args, **kwargs):
+        # .to(dtype) / .half() move the 16-bit bias; the scales stay fp32
+        scale = self.weight_scale
+        ret = super()._apply(fn, *args, **kwargs)
+        if self.weight_scale.dtype != torch.float32:
+            self.weight_scale = scale.to(self.weight_scale.device)
+        return ret
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return dense.int8_linear(x, self.weight, self.weight_scale, self.bias)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"

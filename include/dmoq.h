@@ -356,6 +356,44 @@ int dmoq_expand_weights(const dmoq_pool_t* pool, int32_t is_down, int32_t hidden
 int dmoq_quantize_packed(const void* w, int32_t w_kind, int32_t N, int32_t K, int32_t bit, const float* rot,
                          const float* edges, uint8_t* indices_packed, uint16_t* norms, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Dense operators beside the packed experts (no counterpart in the reference, which runs them as torch modules).
+ * 16-bit tensors are bf16 when is_bf16, else fp16; matrices are row-major; weights, codes and outputs are contiguous and
+ * 16-byte aligned; a pitch is the distance between rows in elements (rows 16-byte aligned).  T may be 0.
+ *
+ * 8-bit products: K a multiple of 16, at most 131056 (the int32 sums are exact); any number of outputs.
+ *   token_quant: scales[t] = max|x[t]| / 127, codes[t][k] = rint(127 x[t][k] / max|x[t]|), ties to even, correctly rounded; a row
+ *                of zeros has scale 0, a row with an infinity or NaN has codes 0 and scale NaN
+ *   int8_gemm:   out[t][n] = scales[t] w_scale[n] sum_k codes[t][k] w[n][k] (+ bias[n]), rounded once to 16 bits
+ *   int8_gated_gemm: out = silu(g) u, g and u the products with w_gate and w_up, rounded once
+ *   int8_linear, int8_gated_linear: the same with token_quant in front; codes (T, K) and scales (T) are scratch
+ */
+int dmoq_token_quant(const void* x, int32_t is_bf16, int32_t T, int32_t K, int64_t x_pitch, int8_t* codes, float* scales,
+                     void* stream);
+int dmoq_int8_gemm(const int8_t* codes, const float* scales, const int8_t* w, const float* w_scale, const void* bias,
+                   int32_t is_bf16, int32_t T, int32_t N, int32_t K, void* out, void* stream);
+int dmoq_int8_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w, const float* w_scale, const void* bias,
+                     int32_t T, int32_t N, int32_t K, int8_t* codes, float* scales, void* out, void* stream);
+int dmoq_int8_gated_gemm(const int8_t* codes, const float* scales, const int8_t* w_gate, const float* gate_scale,
+                         const int8_t* w_up, const float* up_scale, int32_t is_bf16, int32_t T, int32_t I, int32_t K, void* out,
+                         void* stream);
+int dmoq_int8_gated_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w_gate, const float* gate_scale,
+                           const int8_t* w_up, const float* up_scale, int32_t T, int32_t I, int32_t K, int8_t* codes,
+                           float* scales, void* out, void* stream);
+
+/*
+ * Gated feed-forward block: h = silu(x w_gate^T) * (x w_up^T), y = h w_down^T; x, y (T, H), w_gate and w_up (I, H), w_down (H, I),
+ * h (T, I); H and I multiples of 8.  silu and slope (both or neither) receive silu(g) and u silu'(g), (T, I), for the gradients.
+ * backward: dh = dy w_down, dg = dh * slope, du = dh * silu; d_gate_up (T, 2 I) scratch = [dg | du];
+ *   dx = dg w_gate + du w_up, dw_gate = dg^T x, dw_up = du^T x, dw_down = dy^T h.  Outputs that are NULL are not computed, and
+ *   what only they need may be NULL too.  dw_up = dw_gate + H * I elements lets one product compute both.
+ */
+int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate, const void* w_up, const void* w_down,
+                   int32_t T, int32_t H, int32_t I, void* h, void* silu, void* slope, void* y, void* stream);
+int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate,
+                            const void* w_up, const void* w_down, int32_t T, int32_t H, int32_t I, const void* h, const void* silu,
+                            const void* slope, void* d_gate_up, void* dx, void* dw_gate, void* dw_up, void* dw_down, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

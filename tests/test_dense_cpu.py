@@ -1,0 +1,118 @@
+"""Dense operators, what needs no GPU: refusals of the C entry points and of the Python functions, module plumbing."""
+import ctypes as C
+
+import pytest
+import torch
+
+import dartmoq_b200 as D
+from dartmoq_b200 import _lib, dense
+
+EINVAL, ESIZE, OK = -1, -3, 0
+P = C.c_void_p(4096)          # an aligned address that no refused call touches
+ODD = C.c_void_p(4104)        # not 16-byte aligned
+
+
+def test_token_quant_refuses():
+    f = _lib.load().dmoq_token_quant
+    assert f(P, 1, 0, 128, 128, P, P, None) == OK                    # no tokens: nothing to do
+    for bad in ((None, 1, 4, 128, 128, P, P), (P, 1, 4, 128, 128, None, P), (P, 1, 4, 128, 128, P, None),
+                (ODD, 1, 4, 128, 128, P, P), (P, 1, 4, 128, 128, ODD, P),
+                (P, 1, 4, 120, 120, P, P), (P, 1, 4, 0, 0, P, P), (P, 1, -1, 128, 128, P, P),
+                (P, 1, 4, 128, 124, P, P), (P, 1, 4, 128, 132, P, P)):
+        assert f(*bad, None) == EINVAL, bad
+
+
+def test_int8_products_refuse():
+    lib = _lib.load()
+    good = [P, P, P, P, None, 1, 4, 33, 128, P]
+    assert lib.dmoq_int8_gemm(*(good[:6] + [0] + good[7:]), None) == OK
+    for i in (0, 1, 2, 3, 9):
+        assert lib.dmoq_int8_gemm(*(good[:i] + [None] + good[i + 1:]), None) == EINVAL
+    for i, v in ((0, ODD), (2, ODD), (6, -1), (7, 0), (8, 8), (8, 0), (8, 136)):
+        assert lib.dmoq_int8_gemm(*(good[:i] + [v] + good[i + 1:]), None) == EINVAL, (i, v)
+    assert lib.dmoq_int8_gemm(*(good[:8] + [131072] + good[9:]), None) == ESIZE
+    good = [P, P, P, P, P, P, 1, 4, 33, 128, P]
+    assert lib.dmoq_int8_gated_gemm(*(good[:7] + [0] + good[8:]), None) == OK
+    for i in (0, 1, 2, 3, 4, 5, 10):
+        assert lib.dmoq_int8_gated_gemm(*(good[:i] + [None] + good[i + 1:]), None) == EINVAL
+    assert lib.dmoq_int8_gated_gemm(*(good[:9] + [1 << 20] + good[10:]), None) == ESIZE
+    # with the quantiser in front nothing is launched before everything is known to be right
+    good = [P, 1, 128, P, P, None, 4, 33, 128, P, P, P]
+    for i, v in ((0, None), (2, 127), (3, None), (4, None), (7, 0), (8, 100), (9, None), (10, None), (11, None), (3, ODD)):
+        assert lib.dmoq_int8_linear(*(good[:i] + [v] + good[i + 1:]), None) == EINVAL, (i, v)
+    assert lib.dmoq_int8_linear(*(good[:2] + [131072, P, P, None, 4, 33, 131072] + good[9:]), None) == ESIZE
+    good = [P, 1, 128, P, P, P, P, 4, 33, 128, P, P, P]
+    for i in (0, 3, 4, 5, 6, 10, 11, 12):
+        assert lib.dmoq_int8_gated_linear(*(good[:i] + [None] + good[i + 1:]), None) == EINVAL, i
+
+
+def test_gated_ffn_refuses():
+    lib = _lib.load()
+    good = [P, 1, 64, P, P, P, 4, 64, 32, P, None, None, P]
+    assert lib.dmoq_gated_ffn(*(good[:6] + [0] + good[7:]), None) == OK
+    for i in (0, 3, 4, 5, 9, 12):
+        assert lib.dmoq_gated_ffn(*(good[:i] + [None] + good[i + 1:]), None) == EINVAL, i
+    for i, v in ((2, 60), (2, 68), (7, 60), (7, 0), (8, 12), (8, 0), (6, -4), (10, P), (11, P), (0, ODD), (3, ODD), (4, ODD), (5, ODD),
+                 (9, ODD), (12, ODD)):
+        assert lib.dmoq_gated_ffn(*(good[:i] + [v] + good[i + 1:]), None) == EINVAL, (i, v)
+    #       dy pitch x bf pitch wg wu wd  T   H   I  h silu slope dgu dx dwg dwu dwd
+    good = [P, 64, P, 1, 64, P, P, P, 4, 64, 32, P, P, P, P, P, P, P, P]
+    for i in (0, 2, 5, 6, 7, 11, 12, 13, 14):
+        assert lib.dmoq_gated_ffn_backward(*(good[:i] + [None] + good[i + 1:]), None) == EINVAL, i
+    for i, v in ((1, 60), (4, 60), (9, 4), (10, 12), (0, ODD), (2, ODD), (11, ODD), (12, ODD), (14, ODD), (15, ODD), (16, ODD), (18, ODD)):
+        assert lib.dmoq_gated_ffn_backward(*(good[:i] + [v] + good[i + 1:]), None) == EINVAL, (i, v)
+
+
+def test_functions_refuse_cpu_tensors():
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    w8, s8 = torch.zeros(32, 64, dtype=torch.int8), torch.zeros(32)
+    w = torch.zeros(32, 64, dtype=torch.bfloat16)
+    for call in (lambda: dense.quantize_int8_tokens(x), lambda: dense.int8_linear(x, w8, s8),
+                 lambda: dense.int8_gated_linear(x, w8, s8, w8, s8), lambda: dense.gated_feed_forward(x, w, w, w.t()),
+                 lambda: dense.int8_matmul(w8, s8, w8, s8), lambda: D.GatedFeedForward(64, 32)(x)):
+        with pytest.raises(_lib.DmoqError):
+            call()
+
+
+def test_w8a8_linear_plumbing():
+    lin = D.W8A8Linear.from_metadata({"out_features": 33, "in_features": 64, "bias_shape": [33], "orig_dtype": "torch.float16"})
+    assert set(lin.state_dict()) == {"weight", "weight_scale", "bias"}
+    src = {"weight": torch.randint(-127, 128, (33, 64), dtype=torch.int8), "weight_scale": torch.rand(33),
+           "bias": torch.rand(33).half()}
+    lin.load_state_dict(src, strict=True, assign=True)
+    assert torch.equal(lin.weight, src["weight"]) and lin.bias.dtype == torch.float16
+    lin.to(torch.bfloat16)                                           # the bias follows, the scales stay 32-bit
+    assert lin.bias.dtype == torch.bfloat16 and torch.equal(lin.weight_scale, src["weight_scale"])
+    assert set(D.W8A8Linear.from_metadata({"out_features": 3, "in_features": 16}).state_dict()) == {"weight", "weight_scale"}
+    with pytest.raises(ValueError):
+        D.W8A8Linear(torch.zeros(4, 24, dtype=torch.int8), torch.zeros(4))
+    with pytest.raises(ValueError):
+        D.W8A8Linear(torch.zeros(4, 32, dtype=torch.int8), torch.zeros(5))
+    with pytest.raises(TypeError):
+        D.W8A8Linear(torch.zeros(4, 32), torch.zeros(4))
+
+
+def test_feed_forward_plumbing():
+    class Mlp(torch.nn.Module):
+        def __init__(self, bias=False):
+            super().__init__()
+            self.gate_proj, self.up_proj = torch.nn.Linear(64, 32, bias=bias), torch.nn.Linear(64, 32, bias=bias)
+            self.down_proj = torch.nn.Linear(32, 64, bias=bias)
+
+    mlp = Mlp()
+    block = D.GatedFeedForward.from_mlp(mlp)
+    assert block.gate_proj is mlp.gate_proj and set(block.state_dict()) == set(mlp.state_dict())
+    assert (block.hidden_size, block.intermediate_size) == (64, 32)
+    assert {k: tuple(v.shape) for k, v in D.GatedFeedForward(64, 32).state_dict().items()} == \
+        {"gate_proj.weight": (32, 64), "up_proj.weight": (32, 64), "down_proj.weight": (64, 32)}
+    with pytest.raises(ValueError):
+        D.GatedFeedForward.from_mlp(Mlp(bias=True))
+    with pytest.raises(TypeError):
+        D.GatedFeedForward.from_mlp(torch.nn.Linear(2, 2))
+    lin = lambda n, k: D.W8A8Linear(torch.zeros(n, k, dtype=torch.int8), torch.zeros(n))   # noqa: E731
+    assert set(D.W8A8GatedFeedForward(lin(32, 64), lin(32, 64), lin(64, 32)).state_dict()) == \
+        {f"{p}_proj.{t}" for p in ("gate", "up", "down") for t in ("weight", "weight_scale")}
+    with pytest.raises(ValueError):
+        D.W8A8GatedFeedForward(lin(32, 64), lin(48, 64), lin(64, 32))
+    with pytest.raises(ValueError):
+        D.W8A8GatedFeedForward(lin(32, 64), lin(32, 64), lin(64, 48))

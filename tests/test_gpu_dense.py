@@ -1,0 +1,460 @@
+"""Dense operators on the GPU against their 64-bit values (tests/dense_oracle.py has the tolerances)."""
+import ctypes as C
+
+import pytest
+import torch
+
+import dartmoq_b200 as D
+import dense_oracle as R
+from dartmoq_b200 import _lib, dense, synth
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+DTYPES = (torch.bfloat16, torch.float16)
+
+
+def rng(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def randn(g, *shape, scale=1.0, dtype=torch.float32):
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).to(DEV)
+
+
+def acts(g, t, k, dtype):
+    x = torch.randn(t, k, generator=g)
+    x[:, torch.rand(k, generator=g) < 0.01] *= 20
+    return x.to(dtype).to(DEV)
+
+
+def weight8(g, n, k):
+    codes = (torch.randn(n, k, generator=g) * 32).round().clamp(-127, 127).to(torch.int8)
+    return codes.to(DEV), (0.02 / 32 * torch.exp(0.3 * torch.randn(n, generator=g))).to(DEV)
+
+
+def healthy():
+    D.WxA16BitPartitionedGroupMoE.check_device_status()
+
+
+# --------------------------------------------------------------------------------------------- quantiser
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,k", [(1, 16), (3, 128), (77, 2064), (5, 8192), (2, 40000)])
+def test_quantize_codes_equal_the_definition(t, k, dtype):
+    x = acts(rng(t * k), t, k, dtype)
+    codes, scale = dense.quantize_int8_tokens(x)
+    want, s = R.quantize(x)
+    assert codes.dtype == torch.int8 and scale.dtype == torch.float32 and scale.shape == (t,)
+    assert torch.equal(codes.double().cpu(), want)
+    assert torch.equal(scale.cpu(), s.float())                     # max / 127, correctly rounded
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_special_rows(dtype):
+    fi = torch.finfo(dtype)
+    k = 256
+    x = torch.zeros(9, k)
+    x[1] = torch.arange(k) * 0.5 - 64.0                            # with max 127 every odd entry is a tie
+    x[1, 0] = 127.0
+    x[2], x[2, 3] = fi.max / 3, -fi.max
+    x[3], x[3, 5] = fi.smallest_normal, fi.smallest_normal * fi.eps * 3   # subnormals
+    x[4] = fi.smallest_normal * fi.eps                             # the smallest number everywhere
+    x[5, 7] = float("nan")
+    x[6, k - 1] = float("-inf")
+    x[7, 100] = 1.0
+    x[8] = torch.randn(k, generator=rng(1)) * 1e-3
+    x = x.to(dtype).to(DEV)
+    codes, scale = dense.quantize_int8_tokens(x)
+    fine = [0, 1, 2, 3, 4, 7, 8]
+    want, s = R.quantize(x[fine])
+    assert torch.equal(codes[fine].double().cpu(), want) and torch.equal(scale[fine].cpu(), s.float())
+    assert int(codes[[0, 5, 6]].abs().max()) == 0 and torch.isnan(scale[[5, 6]]).all() and float(scale[0]) == 0.0
+    w, ws = weight8(rng(2), 24, k)
+    y = dense.int8_linear(x, w, ws)
+    assert torch.isnan(y[[5, 6]]).all() and torch.isfinite(y[[0, 1, 4, 7, 8]]).all() and float(y[0].abs().max()) == 0.0
+
+
+def test_quantize_shapes_and_strides():
+    g = rng(3)
+    big = randn(g, 6, 5, 320, dtype=torch.bfloat16)
+    codes, scale = dense.quantize_int8_tokens(big[:, 1:4, :128])    # rows that do not follow one another
+    want, s = R.quantize(big[:, 1:4, :128])
+    assert codes.shape == (6, 3, 128) and scale.shape == (6, 3)
+    assert torch.equal(codes.double().cpu(), want) and torch.equal(scale.cpu(), s.float())
+    for view in (big[:, 0, 8:136], big[:, 0, 3:131], big[0, :, :64].t()[:, :1].expand(64, 16), big[:, :, 5:21].transpose(0, 1)):
+        codes, scale = dense.quantize_int8_tokens(view)
+        assert torch.equal(codes.double().cpu(), R.quantize(view)[0])
+    vec, s = dense.quantize_int8_tokens(big[0, 0])
+    assert vec.shape == (320,) and s.shape == ()
+    none, s = dense.quantize_int8_tokens(big[:0])
+    assert none.shape == (0, 5, 320) and s.shape == (0, 5)
+
+
+# --------------------------------------------------------------------------------------------- 8-bit products
+
+SIZES8 = [(1, 1, 16), (1, 33, 128), (2, 512, 2048), (7, 1001, 144), (16, 256, 2064), (17, 96, 4096), (64, 640, 512), (127, 130, 272),
+          (129, 257, 1024), (300, 1001, 2064), (700, 4096, 256), (1300, 2200, 640)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bias", (False, True))
+@pytest.mark.parametrize("t,n,k", SIZES8)
+def test_int8_linear(t, n, k, bias, dtype):
+    g = rng(t + n + k)
+    x, (w, ws) = acts(g, t, k, dtype), weight8(g, n, k)
+    b = randn(g, n, dtype=dtype) if bias else None
+    y = dense.int8_linear(x, w, ws, b)
+    codes, s = R.quantize(x)
+    prod = (codes @ w.double().cpu().t()) * s[:, None] * ws.double().cpu()
+    want = prod + (b.double().cpu() if bias else 0)
+    # one rounding to 16 bits of a value that carries five 32-bit roundings (sum to float, two scales, scale / 127, bias);
+    # smallest_normal * eps is a step below the normal numbers
+    fi = torch.finfo(dtype)
+    e32 = 5 * 2.0 ** -24 * (prod.abs() + want.abs())
+    tol = fi.eps / 2 * (want.abs() + e32) + e32 + fi.smallest_normal * fi.eps
+    assert y.shape == (t, n) and y.dtype == dtype
+    assert ((y.double().cpu() - want).abs() <= tol).all()
+    q, sc = dense.quantize_int8_tokens(x)
+    assert torch.equal(dense.int8_matmul(q, sc, w, ws, b, out_dtype=dtype), y)
+    healthy()
+
+
+def test_int8_sums_are_exact_at_the_largest_inner_size():
+    k = 131056
+    codes = torch.full((3, k), -128, dtype=torch.int8, device=DEV)
+    w = torch.full((20, k), -128, dtype=torch.int8, device=DEV)
+    w[1] = 127
+    w[2, ::2] = 127
+    one = torch.ones(20, device=DEV)
+    y = dense.int8_matmul(codes, torch.full((3,), 2.0 ** -20, device=DEV), w, one, out_dtype=torch.bfloat16)
+    want = (codes.double() @ w.double().t()).cpu() * 2.0 ** -20
+    assert ((y.double().cpu() - want).abs() <= 2.0 ** -8 * want.abs() * (1 + 2.0 ** -22)).all()
+    with pytest.raises(_lib.DmoqError):
+        wide = torch.zeros((1, k + 16), dtype=torch.int8, device=DEV)
+        dense.int8_matmul(wide, torch.ones(1, device=DEV), wide, one[:1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,n,k", SIZES8)
+def test_int8_gated_linear(t, n, k, dtype):
+    g = rng(t * n + k)
+    x, (wg, sg), (wu, su) = acts(g, t, k, dtype), weight8(g, n, k), weight8(g, n, k)
+    sg, su = sg * (64 / k) ** 0.5 * 4, su * (64 / k) ** 0.5         # gates of a few units at every inner size
+    h = dense.int8_gated_linear(x, wg, sg, wu, su)
+    codes, s = R.quantize(x)
+    gate = (codes @ wg.double().cpu().t()) * s[:, None] * sg.double().cpu()
+    up = (codes @ wu.double().cpu().t()) * s[:, None] * su.double().cpu()
+    want = R.silu(gate) * up
+    # silu's relative condition is at most 1 + |g|; g carries four 32-bit roundings, u four, the exponential 2 + |g| and the
+    # quotient and products five
+    fi = torch.finfo(dtype)
+    e32 = 2.0 ** -24 * (4 * (1 + gate.abs()) + 4 + 2 * (2 + gate.abs()) + 5)
+    tol = want.abs() * (fi.eps / 2 * (1 + e32) + e32) + fi.smallest_normal * fi.eps
+    assert h.shape == (t, n) and ((h.double().cpu() - want).abs() <= tol).all()
+    healthy()
+
+
+def test_int8_shapes_strides_and_refusals():
+    g = rng(11)
+    x = randn(g, 4, 6, 512, dtype=torch.bfloat16)
+    w, ws = weight8(g, 48, 256)
+    y = dense.int8_linear(x[:, ::2, 128:384], w, ws)
+    assert y.shape == (4, 3, 48) and torch.equal(y, dense.int8_linear(x[:, ::2, 128:384].contiguous(), w, ws))
+    wide, wide_scale = weight8(g, 48, 512)
+    assert torch.equal(dense.int8_linear(x[0, :, :256], wide[:, :256], ws), dense.int8_linear(x[0, :, :256], wide[:, :256].contiguous(), ws))
+    assert dense.int8_linear(x[:0, 0, :256], w, ws).shape == (0, 48)
+    assert dense.int8_linear(x[0, 0, :256], w, ws).shape == (48,)
+    codes, s = dense.quantize_int8_tokens(x)
+    part = dense.int8_matmul(codes[:, :, 16:272], s, w, ws)
+    assert torch.equal(part, dense.int8_matmul(codes[:, :, 16:272].contiguous(), s, w, ws))
+    with pytest.raises(TypeError):
+        dense.int8_linear(x.float(), w, ws)
+    with pytest.raises(TypeError):
+        dense.int8_linear(x[..., :256], w, ws.half())
+    with pytest.raises(TypeError):
+        dense.int8_linear(x[..., :256], w, ws, torch.zeros(48, device=DEV))
+    with pytest.raises(ValueError):
+        dense.int8_linear(x, w, ws)                                  # inner sizes differ
+    with pytest.raises(ValueError):
+        dense.int8_linear(x[..., :256], w, ws[:-1])
+    with pytest.raises(ValueError):
+        dense.int8_linear(x[..., :256], w.cpu(), ws)
+    with pytest.raises(ValueError):
+        dense.quantize_int8_tokens(x[..., :100])
+    with pytest.raises(ValueError):
+        dense.int8_gated_linear(x[..., :256], w, ws, w[:-1], ws[:-1])
+    with pytest.raises(TypeError):
+        dense.int8_matmul(codes, s, wide, wide_scale, out_dtype=torch.float32)
+
+
+# --------------------------------------------------------------------------------------------- gated feed-forward
+
+FFN_SIZES = [(1, 8, 8), (1, 256, 136), (3, 72, 200), (16, 512, 256), (33, 128, 1032), (64, 256, 72), (128, 320, 128), (129, 264, 136),
+             (257, 1032, 520), (1000, 256, 128), (640, 520, 1040)]
+
+
+def ffn_inputs(t, h, i, dtype, seed=0):
+    g = rng(seed + 7 * t + h + i)
+    x = randn(g, t, h, dtype=dtype)
+    wg, wu = (randn(g, i, h, scale=1.5 * h ** -0.5, dtype=dtype) for _ in range(2))
+    wd = randn(g, h, i, scale=i ** -0.5, dtype=dtype)
+    return x, wg, wu, wd, randn(g, t, h, dtype=dtype)
+
+
+# y: hidden values and y rounded.  dw_down: hidden values and the gradient.  The others: what is kept of the hidden values, dg
+# or du, the gradient.
+ROUNDINGS = {"y": 2, "dx": 3, "dw_gate": 3, "dw_up": 3, "dw_down": 2}
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,h,i", FFN_SIZES)
+def test_ffn_forward(t, h, i, dtype):
+    x, wg, wu, wd, _ = ffn_inputs(t, h, i, dtype)
+    y = dense.gated_feed_forward(x, wg, wu, wd)
+    assert not y.requires_grad
+    R.close(y, R.ffn(x, wg, wu, wd)[3], ROUNDINGS["y"], "y")
+    assert torch.equal(y, dense.gated_feed_forward(x, wg, wu, wd))
+    healthy()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,h,i", FFN_SIZES)
+def test_ffn_gradients(t, h, i, dtype):
+    x, wg, wu, wd, dy = ffn_inputs(t, h, i, dtype, seed=1)
+    leaves = [v.requires_grad_(True) for v in (x, wg, wu, wd)]
+    y = dense.gated_feed_forward(*leaves)
+    grads = dict(zip(("dx", "dw_gate", "dw_up", "dw_down"), torch.autograd.grad(y, leaves, dy, retain_graph=True)))
+    want = R.ffn_grads(x, wg, wu, wd, dy)
+    R.close(y, R.ffn(x, wg, wu, wd)[3], ROUNDINGS["y"], "y")
+    for name, v in grads.items():
+        R.close(v, want[name], ROUNDINGS[name], name)
+    again = torch.autograd.grad(y, leaves, dy)
+    assert all(torch.equal(a, b) for a, b in zip(grads.values(), again))
+    healthy()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_ffn_gradients_against_differences(dtype):
+    x, wg, wu, wd, dy = ffn_inputs(40, 136, 264, dtype, seed=2)
+    leaves = [v.requires_grad_(True) for v in (x, wg, wu, wd)]
+    grads = torch.autograd.grad(dense.gated_feed_forward(*leaves), leaves, dy)
+    base = [v.detach().double().cpu() for v in leaves]
+    g = rng(5)
+    for i, grad in enumerate(grads):
+        # along the gradient itself, so that the slope is its squared norm and nothing cancels
+        way = grad.double().cpu() + 0.3 * grad.double().cpu().std() * torch.randn(grad.shape, generator=g).double()
+        eps = 1e-5 / float(way.abs().max())
+        loss = lambda e: float((R.ffn(*[b + (e * way if j == i else 0) for j, b in enumerate(base)])[3] * dy.double().cpu()).sum())  # noqa: E731
+        slope = (loss(eps) - loss(-eps)) / (2 * eps)
+        mine = float((grad.double().cpu() * way).sum())
+        assert abs(mine - slope) <= 3 * R.half(dtype) * abs(slope) + 1e-6 * abs(slope), (i, mine, slope)
+
+
+def test_ffn_computes_only_the_gradients_that_are_needed():
+    x, wg, wu, wd, dy = ffn_inputs(70, 264, 136, torch.bfloat16, seed=3)
+    want = R.ffn_grads(x, wg, wu, wd, dy)
+    names = ("dx", "dw_gate", "dw_up", "dw_down")
+    for mask in range(1, 16):
+        leaves = [v.detach().clone().requires_grad_(bool(mask >> i & 1)) for i, v in enumerate((x, wg, wu, wd))]
+        y = dense.gated_feed_forward(*leaves)
+        y.backward(dy)
+        for i, v in enumerate(leaves):
+            assert (v.grad is None) == (not mask >> i & 1)
+            if v.grad is not None:
+                R.close(v.grad, want[names[i]], ROUNDINGS[names[i]], f"{names[i]} (mask {mask})")
+
+
+def test_ffn_empty_shapes_strides_and_refusals():
+    x, wg, wu, wd, dy = ffn_inputs(24, 264, 136, torch.float16, seed=4)
+    leaves = [v.requires_grad_(True) for v in (x[:0].detach(), wg, wu, wd)]
+    y = dense.gated_feed_forward(*leaves)
+    assert y.shape == (0, 264)
+    gx, *gw = torch.autograd.grad(y.sum(), leaves)
+    assert gx.shape == (0, 264) and all(float(v.abs().max()) == 0 for v in gw)
+    # a view of a wider tensor, three dimensions, an upstream gradient without memory of its own
+    wide = randn(rng(5), 4, 6, 400, dtype=torch.float16).requires_grad_(True)
+    view = wide[:, 1:5, 64:328]
+    gy = torch.autograd.grad(dense.gated_feed_forward(view, wg, wu, wd).sum(), (wide, wg))
+    flat = view.detach().reshape(-1, 264).contiguous().requires_grad_(True)
+    out = dense.gated_feed_forward(flat, wg, wu, wd)
+    gf = torch.autograd.grad(out, (flat, wg), torch.ones_like(out))
+    assert torch.equal(gy[0][:, 1:5, 64:328].reshape(-1, 264), gf[0]) and torch.equal(gy[1], gf[1])
+    assert float(gy[0][:, 0].abs().max()) == 0
+    # weights that are views
+    assert torch.equal(dense.gated_feed_forward(x.detach(), wg.t().contiguous().t(), wu, wd), dense.gated_feed_forward(x.detach(), wg, wu, wd))
+    with pytest.raises(TypeError):
+        dense.gated_feed_forward(x, wg.bfloat16(), wu, wd)
+    with pytest.raises(ValueError):
+        dense.gated_feed_forward(x, wg, wu[:-8], wd)
+    with pytest.raises(ValueError):
+        dense.gated_feed_forward(x, wg, wu, wd.t())
+    with pytest.raises(ValueError):
+        dense.gated_feed_forward(x[:, :260], wg[:, :260], wu[:, :260], wd[:260])
+    with pytest.raises(ValueError):
+        dense.gated_feed_forward(x, wg, wu, wd.cpu())
+    double = torch.autograd.grad(dense.gated_feed_forward(x, wg, wu, wd).square().sum(), wg, create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        double.sum().backward()                                      # once differentiable
+
+
+def test_ffn_infinities_and_nan_stay_in_their_rows():
+    x, wg, wu, wd, _ = ffn_inputs(140, 264, 136, torch.bfloat16, seed=6)
+    clean = dense.gated_feed_forward(x, wg, wu, wd)
+    x2 = x.clone()
+    x2[3, 5], x2[131, 0] = float("nan"), float("inf")
+    y = dense.gated_feed_forward(x2, wg, wu, wd)
+    rest = [r for r in range(140) if r not in (3, 131)]
+    assert torch.equal(y[rest], clean[rest]) and torch.isnan(y[3]).all() and not torch.isfinite(y[131]).any()
+
+
+# --------------------------------------------------------------------------------------------- how they are used
+
+def test_outputs_stay_inside_their_memory():
+    """Through the C entries, with rows of sentinels in front of and behind every output."""
+    lib = _lib.load()
+    for t, n, k in ((5, 37, 128), (130, 129, 256), (200, 1001, 128)):
+        g = rng(n)
+        x, (w, ws) = acts(g, t, k, torch.bfloat16), weight8(g, n, k)
+        out = torch.full((t + 2, n), 7.0, dtype=torch.bfloat16, device=DEV)
+        codes = torch.full((t + 2, k), 99, dtype=torch.int8, device=DEV)
+        scale = torch.full((t + 2,), 7.0, device=DEV)
+        p = lambda v: C.c_void_p(v.data_ptr())  # noqa: E731
+        for name, extra in (("dmoq_int8_linear", (p(w), p(ws), None)), ("dmoq_int8_gated_linear", (p(w), p(ws), p(w), p(ws)))):
+            _lib.check(getattr(lib, name)(p(x), 1, k, *extra, t, n, k, p(codes[1]), p(scale[1:]), p(out[1]), None), name)
+            torch.cuda.synchronize()
+            for v, s in ((out, 7.0), (codes, 99), (scale, 7.0)):
+                assert (v[0] == s).all() and (v[-1] == s).all()
+    t, h, i = 130, 136, 72
+    x, wg, wu, wd, dy = ffn_inputs(t, h, i, torch.bfloat16)
+    pad = lambda r, c: torch.full((r + 2, c), 7.0, dtype=torch.bfloat16, device=DEV)  # noqa: E731
+    hid, si, sl, y = pad(t, i), pad(t, i), pad(t, i), pad(t, h)
+    dgu, dx, dw, dwd = pad(t, 2 * i), pad(t, h), pad(2 * i, h), pad(h, i)
+    q = lambda v: C.c_void_p(v[1].data_ptr())  # noqa: E731
+    _lib.check(lib.dmoq_gated_ffn(p(x), 1, h, p(wg), p(wu), p(wd), t, h, i, q(hid), q(si), q(sl), q(y), None), "ffn")
+    _lib.check(lib.dmoq_gated_ffn_backward(p(dy), h, p(x), 1, h, p(wg), p(wu), p(wd), t, h, i, q(hid), q(si), q(sl), q(dgu), q(dx), q(dw),
+                                           C.c_void_p(dw[1 + i].data_ptr()), q(dwd), None), "ffn backward")
+    torch.cuda.synchronize()
+    for v in (hid, si, sl, y, dgu, dx, dw, dwd):
+        assert (v[0] == 7.0).all() and (v[-1] == 7.0).all()
+    R.close(dw[1:1 + 2 * i], torch.cat([R.ffn_grads(x, wg, wu, wd, dy)[k] for k in ("dw_gate", "dw_up")]), 3, "dw")
+    # the gradients of the two projections in memory that is not adjacent: two products
+    a, b = pad(i, h), pad(i, h)
+    _lib.check(lib.dmoq_gated_ffn_backward(p(dy), h, p(x), 1, h, None, None, p(wd), t, h, i, None, q(si), q(sl), q(dgu), None, q(a), q(b),
+                                           None, None), "ffn backward")
+    torch.cuda.synchronize()
+    assert torch.equal(a[1:-1], dw[1:1 + i]) and torch.equal(b[1:-1], dw[1 + i:1 + 2 * i])
+    assert (a[-1] == 7.0).all() and (b[0] == 7.0).all()
+
+
+def test_streams_and_captured_graphs():
+    """Work goes to the current stream; two captured graphs replayed at once do not share scratch."""
+    g = rng(21)
+    k, n = 512, 640
+    w, ws = weight8(g, n, k)
+    xs = [acts(g, t, k, torch.bfloat16) for t in (40, 300)]
+    fx, wg, wu, wd, _ = ffn_inputs(300, 264, 136, torch.bfloat16, seed=9)
+
+    def work(x):
+        return dense.int8_linear(x, w, ws), dense.int8_gated_linear(x, w, ws, w, ws), dense.gated_feed_forward(fx, wg, wu, wd)
+
+    want = [[v.clone() for v in work(x)] for x in xs]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(2_000_000)                                # whatever ran on another stream would be too early
+        late = [x.clone() for x in xs]
+        got = [work(x) for x in late]
+    side.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+    graphs, static, outs = [], [torch.zeros_like(x) for x in xs], []
+    for s in static:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(work(s))
+        graphs.append(graph)
+    for s, x in zip(static, xs):
+        s.copy_(x)
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            graphs[0].replay()
+        with torch.cuda.stream(other):
+            graphs[1].replay()
+    torch.cuda.synchronize()
+    for a, b in zip(want, outs):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+    healthy()
+
+
+def test_training_step_in_a_captured_graph():
+    x, wg, wu, wd, dy = ffn_inputs(96, 264, 136, torch.bfloat16, seed=12)
+    leaves = [v.requires_grad_(True) for v in (x, wg, wu, wd)]
+
+    def step():
+        return torch.autograd.grad(dense.gated_feed_forward(*leaves), leaves, dy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = [v.clone() for v in step()]
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for v in got:
+        v.fill_(0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("tokens", (1, 40, 700))
+@pytest.mark.parametrize("eight_bit", (False, True))
+def test_as_shared_expert_of_a_packed_layer(tokens, eight_bit):
+    """The MoE module with an unpacked shared expert: routed experts packed, the shared one a dense block of this file."""
+    moe = synth.build_layer(hidden=256, n_experts=8, top_k=2, inter=128, bit_mix={2: 0.5, 4: 0.5}, seed=5).to(DEV)
+    x = synth.make_activations(tokens, 256, seed=3).to(DEV).unsqueeze(0)
+    routed = moe(x).clone()
+    g = rng(tokens)
+    block = D.GatedFeedForward(256, 384, device=DEV)
+    with torch.no_grad():
+        for p in block.parameters():
+            p.copy_(randn(g, *p.shape, scale=0.05, dtype=torch.bfloat16))
+    expert = D.W8A8GatedFeedForward.from_mlp(block) if eight_bit else block
+    moe.shared_expert = expert
+    moe.shared_expert_gate = torch.nn.Linear(256, 1, bias=False, dtype=torch.bfloat16, device=DEV)
+    moe._engine = moe._graphs = None
+    for _ in range(3):                                              # eager, captured, replayed
+        y = moe(x)
+        want = routed[0] + expert(x[0]) * torch.sigmoid(moe.shared_expert_gate(x[0]))
+        assert torch.equal(y[0], want)
+    ref = R.ffn(x[0], block.gate_proj.weight, block.up_proj.weight, block.down_proj.weight)[3]
+    if eight_bit:
+        # two quantisations of tokens and one of every weight: each is off by at most half a step, max / 254, of a row whose
+        # root mean square is at least max / 127 * 10 here, and rounding errors of a row add up in squares (x 1 / sqrt(3))
+        assert float((expert(x[0]).double().cpu() - ref).norm() / ref.norm()) <= 4 * 0.5 / 10 / 3 ** 0.5
+    else:
+        R.close(expert(x[0]), ref, 2, "shared expert")
+    healthy()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_modules(dtype):
+    g = rng(31)
+    lin = torch.nn.Linear(144, 57, bias=True, dtype=dtype, device=DEV)
+    q = D.W8A8Linear.from_linear(lin)
+    codes, s = R.quantize(lin.weight)
+    assert torch.equal(q.weight.double().cpu(), codes) and torch.equal(q.weight_scale.cpu(), s.float())
+    x = acts(g, 9, 144, dtype)
+    assert torch.equal(q(x), dense.int8_linear(x, q.weight, q.weight_scale, q.bias))
+    again = D.W8A8Linear.from_metadata({"out_features": 57, "in_features": 144, "bias_shape": [57], "orig_dtype": str(dtype)})
+    again.load_state_dict(q.state_dict(), strict=True, assign=True)
+    assert torch.equal(again(x), q(x))
+    block = D.GatedFeedForward(144, 72, dtype=dtype, device=DEV)
+    y = block(x)
+    y.float().square().sum().backward()
+    grads = R.ffn_grads(x, *(p.weight for p in (block.gate_proj, block.up_proj, block.down_proj)), 2 * y)
+    for p, name in ((block.gate_proj, "dw_gate"), (block.up_proj, "dw_up"), (block.down_proj, "dw_down")):
+        R.close(p.weight.grad, grads[name], ROUNDINGS[name], name)
