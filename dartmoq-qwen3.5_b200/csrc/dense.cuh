@@ -9,28 +9,41 @@ namespace dense {
 
 enum Kind { KIND_16 = 0, KIND_I8 = 1 };
 enum Epi {
-  EPI_OUT = 0,        // out0 = v                                       (16-bit products)
-  EPI_SCALE = 1,      // out0 = v * a_scale[row] * b_scale[col] + bias  (8-bit products)
-  EPI_SILU = 2,       // g, u from two weights: out0 = silu(g) u
-  EPI_SILU_SAVE = 3,  // the same, and out1 = silu(g), out2 = u silu'(g): what the gradients need
-  EPI_GRAD = 4        // v = dh: out0 = dh * in1 (= u silu'(g)), out1 = dh * in0 (= silu(g))
+  EPI_OUT = 0,        // out[0] = v                                       (16-bit products)
+  EPI_SCALE = 1,      // out[0] = v * a_scale[row] * b_scale[col] + bias  (8-bit products)
+  EPI_SILU = 2,       // g, u from two weights: out[0] = silu(g) u
+  EPI_SILU_SAVE = 3,  // the same, and silu(g), u silu'(g) for the gradients in three planes (see Saved)
+  EPI_GRAD = 4        // v = dh: out[0] = dg = dh * u silu'(g), out[1] = du = dh * silu(g), from those planes
 };
 constexpr __host__ __device__ bool is_dual(int epi) { return epi == EPI_SILU || epi == EPI_SILU_SAVE; }
 
+constexpr __host__ __device__ int outputs_of(int epi) { return epi == EPI_SILU_SAVE ? 4 : epi == EPI_GRAD ? 2 : 1; }
+
 struct Maps {
   CUtensorMap a[2], b[2];
+  CUtensorMap out[4];       // only where stores go through TMA
 };
+
+// silu(g) and u silu'(g) are kept to the upper 24 bits of their 32-bit floats, whatever the tensors' 16-bit type: planes 1 and 2
+// hold the upper 16 bits of either, plane 3 the next eight of both.  Rounded to 16 bits they would add a third rounding of the
+// type to dg and du, which are themselves rounded as operands of the next products; this costs half as much traffic
+// again and leaves 2^-16.  The lower bits are cut off, not rounded, so that a NaN stays one.
+__device__ __forceinline__ uint32_t saved_low(float silu, float slope) {
+  return ((__float_as_uint(silu) >> 8) & 0xffu) | (__float_as_uint(slope) & 0xff00u);
+}
+__device__ __forceinline__ float saved_silu(uint32_t hi, uint32_t low) { return __uint_as_float((hi << 16) | ((low & 0xffu) << 8)); }
+__device__ __forceinline__ float saved_slope(uint32_t hi, uint32_t low) { return __uint_as_float((hi << 16) | (low & 0xff00u)); }
 
 struct Args {
   int M, N, K;              // output rows, output columns (of one of the two products when dual), length of a K segment
   int segs;                 // K segments: segment s multiplies a[s] by b[s], all into one sum
   int bf16;                 // 16-bit type of inputs and outputs: bf16, else fp16
-  int vec;                  // outputs (and in0 / in1) may be accessed four elements at a time
+  int vec;                  // output rows may be written four elements at a time
   const float* a_scale;     // 8-bit: one per row
   const float* b_scale[2];  // 8-bit: one per column (of each product when dual)
   const uint16_t* bias;     // 8-bit, optional, type of the output
-  const uint16_t *in0, *in1;
-  uint16_t *out0, *out1, *out2;
+  const uint16_t* in[3];    // the saved planes
+  uint16_t* out[4];
   long long ld_in, ld_out;  // row pitches in elements
 };
 
@@ -44,7 +57,7 @@ __device__ __forceinline__ void finish(const Args& a, long long row, int col, ui
     x *= sa * a.b_scale[0][col];
     if (is_dual(EPI)) y *= sa * a.b_scale[1][col];
   }
-  if (EPI == EPI_OUT) {
+  if (EPI == EPI_OUT || EPI == EPI_GRAD) {
     o[0] = x;
   } else if (EPI == EPI_SCALE) {
     o[0] = a.bias ? x + unpack16(a.bias[col], a.bf16) : x;

@@ -4,6 +4,7 @@
 namespace dense {
 
 int tile_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, const Args& a, int splits, cudaStream_t s);
+int pair_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, const Args& a, cudaStream_t s);
 
 namespace {
 
@@ -33,17 +34,19 @@ struct Matrix {
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 bool tma_ok(const Matrix& m, int es) { return aligned16(m.p) && (m.pitch * es) % 16 == 0 && m.pitch >= m.cols; }
 
-// Copied in boxes of 128 bytes x box_rows rows with the 128-byte swizzle; what lies past the matrix reads as zero.
-int make_map(CUtensorMap* map, const Matrix& m, int es, int box_rows) {
+// Copied in boxes of box_bytes (128 or 64) x box_rows rows with the swizzle of that width; what lies past the matrix reads as
+// zero and is not written.
+int make_map(CUtensorMap* map, const Matrix& m, int es, int box_rows, int box_bytes = 128) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (fn == nullptr) return DMOQ_EDEVICE;
   const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows};
   const cuuint64_t strides[1] = {(cuuint64_t)m.pitch * es};
-  const cuuint32_t box[2] = {(cuuint32_t)(128 / es), (cuuint32_t)box_rows};
+  const cuuint32_t box[2] = {(cuuint32_t)(box_bytes / es), (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
   auto encode = [&] {
     return fn(map, es == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(m.p), dims,
-              strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
   CUresult rc = encode();
@@ -66,7 +69,10 @@ struct Product {
 
 int run(const Product& p, cudaStream_t s) {
   const int es = p.kind == KIND_I8 ? 1 : 2, bk = 128 / es;
-  const int cols = is_dual(p.epi) ? 64 : 128;
+  const bool dual = is_dual(p.epi);
+  const long long pair_tiles = (long long)dmoq_ceil_div(p.args.M, 256) * dmoq_ceil_div(p.args.N, dual ? 128 : 256);
+  const bool pair = pair_tiles * 4 >= dmoq_sm_count();
+  const int cols = dual ? 64 : 128;
   const long long tiles = (long long)dmoq_ceil_div(p.args.M, 128) * dmoq_ceil_div(p.args.N, cols);
   const int steps = dmoq_ceil_div(p.args.K, bk) * p.args.segs;
   int splits = 1;
@@ -78,8 +84,21 @@ int run(const Product& p, cudaStream_t s) {
     const Matrix& b = p.b[i < n_b ? i : 0];
     if (!tma_ok(a, es) || !tma_ok(b, es)) return DMOQ_EINVAL;
     int rc = make_map(&maps.a[i], a, es, p.a_mn ? bk : 128);
-    if (rc == DMOQ_OK) rc = make_map(&maps.b[i], b, es, p.b_mn ? bk : cols);
+    if (rc == DMOQ_OK) rc = make_map(&maps.b[i], b, es, p.b_mn ? bk : pair ? 128 : cols);
     if (rc != DMOQ_OK) return rc;
+  }
+  if (pair) {
+    Args args = p.args;
+    args.vec = 1;
+    for (int e = 0; e < outputs_of(p.epi); ++e) {
+      const Matrix o = {args.out[e], args.M, args.N, args.ld_out};
+      args.vec = args.vec && tma_ok(o, 2);
+    }
+    for (int e = 0; args.vec && e < outputs_of(p.epi); ++e) {
+      const int rc = make_map(&maps.out[e], {args.out[e], args.M, args.N, args.ld_out}, 2, 32, 64);
+      if (rc != DMOQ_OK) return rc;
+    }
+    return pair_product(p.kind, p.a_mn, p.b_mn, p.epi, maps, args, s);
   }
   return tile_product(p.kind, p.a_mn, p.b_mn, p.epi, maps, p.args, splits, s);
 }
@@ -92,15 +111,20 @@ constexpr int kMaxK8 = 131056;   // |sum of K products of codes| <= 128 * 128 K 
 bool usable(const void* p) { return p != nullptr && aligned16(p); }
 bool rows_usable(const void* p, long long pitch, int cols) { return usable(p) && pitch >= cols && pitch % 8 == 0; }   // 16-bit rows
 
+constexpr int kMaxDim = 1 << 30;   // rows and columns: tile coordinates stay inside 32 bits
+
 int check_sizes8(int T, int N, int K) {
   if (T < 0 || N < 1 || K < 16 || K % 16 != 0) return DMOQ_EINVAL;
-  return K > kMaxK8 ? DMOQ_ESIZE : DMOQ_OK;
+  return K > kMaxK8 || T > kMaxDim || N > kMaxDim ? DMOQ_ESIZE : DMOQ_OK;
 }
 bool quant_ok(const void* x, long long pitch, int K, const void* codes, const void* scales) {
   return rows_usable(x, pitch, K) && usable(codes) && scales;
 }
 bool weight8_ok(const void* w, const void* scale) { return usable(w) && scale; }
-bool ffn_sizes_ok(int T, int H, int I) { return T >= 0 && H >= 8 && I >= 8 && H % 8 == 0 && I % 8 == 0 && I <= (1 << 30); }
+int check_ffn(int T, int H, int I) {
+  if (T < 0 || H < 8 || I < 8 || H % 8 != 0 || I % 8 != 0) return DMOQ_EINVAL;
+  return T > kMaxDim || H > kMaxDim || I > kMaxDim / 2 ? DMOQ_ESIZE : DMOQ_OK;   // the gradients of both projections are one product of 2 I rows
+}
 
 int int8_product(const int8_t* codes, const float* scales, const int8_t* w0, const float* s0, const int8_t* w1, const float* s1,
                  const void* bias, int bf16, int T, int N, int K, void* out, cudaStream_t s) {
@@ -114,7 +138,7 @@ int int8_product(const int8_t* codes, const float* scales, const int8_t* w0, con
   a.M = T, a.N = N, a.K = K, a.segs = 1, a.bf16 = bf16;
   a.a_scale = scales, a.b_scale[0] = s0, a.b_scale[1] = s1;
   a.bias = static_cast<const uint16_t*>(bias);
-  a.out0 = static_cast<uint16_t*>(out);
+  a.out[0] = static_cast<uint16_t*>(out);
   a.ld_out = N;
   a.vec = vec4(out, N, N);
   return run(p, s);
@@ -130,6 +154,7 @@ using namespace dense;
 extern "C" int dmoq_token_quant(const void* x, int32_t is_bf16, int32_t T, int32_t K, int64_t x_pitch, int8_t* codes, float* scales,
                                 void* stream) {
   DMOQ_CHECK_ARG(T >= 0 && K >= 16 && K % 16 == 0);
+  if (T > kMaxDim) return DMOQ_ESIZE;
   if (T == 0) return DMOQ_OK;
   DMOQ_CHECK_ARG(quant_ok(x, x_pitch, K, codes, scales));
   return dmoq_token_quant_launch(x, is_bf16, T, K, x_pitch, codes, scales, static_cast<cudaStream_t>(stream));
@@ -176,22 +201,20 @@ extern "C" int dmoq_int8_gated_linear(const void* x, int32_t is_bf16, int64_t x_
 }
 
 extern "C" int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate, const void* w_up, const void* w_down,
-                              int32_t T, int32_t H, int32_t I, void* h, void* silu, void* slope, void* y, void* stream) {
-  DMOQ_CHECK_ARG(ffn_sizes_ok(T, H, I));
-  DMOQ_CHECK_ARG((silu == nullptr) == (slope == nullptr));
-  if (T == 0) return DMOQ_OK;
+                              int32_t T, int32_t H, int32_t I, void* h, void* saved, void* y, void* stream) {
+  const int size = check_ffn(T, H, I);
+  if (size != DMOQ_OK || T == 0) return size;
   DMOQ_CHECK_ARG(rows_usable(x, x_pitch, H) && usable(w_gate) && usable(w_up) && usable(w_down) && usable(h) && usable(y));
-  DMOQ_CHECK_ARG(aligned16(silu) && aligned16(slope));
+  DMOQ_CHECK_ARG(aligned16(saved));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   Product up;
-  up.epi = silu ? EPI_SILU_SAVE : EPI_SILU;
+  up.epi = saved ? EPI_SILU_SAVE : EPI_SILU;
   up.a[0] = {x, T, H, x_pitch};
   up.b[0] = {w_gate, I, H, H};
   up.b[1] = {w_up, I, H, H};
   up.args.M = T, up.args.N = I, up.args.K = H, up.args.segs = 1, up.args.bf16 = is_bf16, up.args.vec = 1;
-  up.args.out0 = static_cast<uint16_t*>(h);
-  up.args.out1 = static_cast<uint16_t*>(silu);
-  up.args.out2 = static_cast<uint16_t*>(slope);
+  up.args.out[0] = static_cast<uint16_t*>(h);
+  for (int e = 0; saved && e < 3; ++e) up.args.out[1 + e] = static_cast<uint16_t*>(saved) + e * (size_t)T * I;
   up.args.ld_out = I;
   int rc = run(up, s);
   if (rc != DMOQ_OK) return rc;
@@ -199,16 +222,17 @@ extern "C" int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, c
   down.a[0] = {h, T, I, I};
   down.b[0] = {w_down, H, I, I};
   down.args.M = T, down.args.N = H, down.args.K = I, down.args.segs = 1, down.args.bf16 = is_bf16, down.args.vec = 1;
-  down.args.out0 = static_cast<uint16_t*>(y);
+  down.args.out[0] = static_cast<uint16_t*>(y);
   down.args.ld_out = H;
   return run(down, s);
 }
 
 extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate,
                                        const void* w_up, const void* w_down, int32_t T, int32_t H, int32_t I, const void* h,
-                                       const void* silu, const void* slope, void* d_gate_up, void* dx, void* dw_gate, void* dw_up,
+                                       const void* saved, void* d_gate_up, void* dx, void* dw_gate, void* dw_up,
                                        void* dw_down, void* stream) {
-  DMOQ_CHECK_ARG(ffn_sizes_ok(T, H, I));
+  const int size = check_ffn(T, H, I);
+  if (size != DMOQ_OK) return size;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const size_t w_bytes = (size_t)H * I * 2;
   if (T == 0) {   // no tokens: the weights' gradients are zero
@@ -221,7 +245,7 @@ extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const v
   DMOQ_CHECK_ARG(aligned16(dx) && aligned16(dw_gate) && aligned16(dw_up) && aligned16(dw_down));
   DMOQ_CHECK_ARG(!(inner || dw_down) || rows_usable(dy, dy_pitch, H));
   DMOQ_CHECK_ARG(!dw_down || usable(h));
-  DMOQ_CHECK_ARG(!inner || (usable(w_down) && usable(silu) && usable(slope) && usable(d_gate_up)));
+  DMOQ_CHECK_ARG(!inner || (usable(w_down) && usable(saved) && usable(d_gate_up)));
   DMOQ_CHECK_ARG(!dx || (usable(w_gate) && usable(w_up)));
   DMOQ_CHECK_ARG(!(dw_gate || dw_up) || rows_usable(x, x_pitch, H));
   uint16_t* dg = static_cast<uint16_t*>(d_gate_up);
@@ -233,11 +257,10 @@ extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const v
     p.a[0] = {dy, T, H, dy_pitch};
     p.b[0] = {w_down, H, I, I};
     p.args.M = T, p.args.N = I, p.args.K = H, p.args.segs = 1, p.args.bf16 = is_bf16, p.args.vec = 1;
-    p.args.in0 = static_cast<const uint16_t*>(silu);
-    p.args.in1 = static_cast<const uint16_t*>(slope);
+    for (int e = 0; e < 3; ++e) p.args.in[e] = static_cast<const uint16_t*>(saved) + e * (size_t)T * I;
     p.args.ld_in = I;
-    p.args.out0 = dg;
-    p.args.out1 = dg + I;
+    p.args.out[0] = dg;
+    p.args.out[1] = dg + I;
     p.args.ld_out = 2 * (long long)I;
     if ((rc = run(p, s)) != DMOQ_OK) return rc;
   }
@@ -249,7 +272,7 @@ extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const v
     p.b[0] = {w_gate, I, H, H};
     p.b[1] = {w_up, I, H, H};
     p.args.M = T, p.args.N = H, p.args.K = I, p.args.segs = 2, p.args.bf16 = is_bf16, p.args.vec = 1;
-    p.args.out0 = static_cast<uint16_t*>(dx);
+    p.args.out[0] = static_cast<uint16_t*>(dx);
     p.args.ld_out = H;
     if ((rc = run(p, s)) != DMOQ_OK) return rc;
   }
@@ -259,7 +282,7 @@ extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const v
     p.a[0] = a;
     p.b[0] = b;
     p.args.M = (int)a.cols, p.args.N = (int)b.cols, p.args.K = T, p.args.segs = 1, p.args.bf16 = is_bf16, p.args.vec = 1;
-    p.args.out0 = static_cast<uint16_t*>(out);
+    p.args.out[0] = static_cast<uint16_t*>(out);
     p.args.ld_out = b.cols;
     return run(p, s);
   };

@@ -1,0 +1,356 @@
+// Dense products on the tensor cores, large outputs: a persistent pair of blocks (two SMs, tcgen05 cta_group::2) walks 256 x 256
+// output tiles.
+//
+// Each block of a pair holds 128 of the tile's rows: it loads its own 128 rows of A and one half of the tile's 256 columns of B
+// (when dual: the first block the gate's 128 columns, the second the up projection's), the leader's MMA thread multiplies both
+// halves, and each block finds its 128 rows x 256 columns of sums in its own TMEM.  Two such accumulators fill TMEM, so the
+// epilogue of a tile runs beside the products of the next one.
+//   warp 0      loads the operands by TMA (five steps of 128 bytes of K ahead)
+//   warp 1      issues tcgen05.mma (leader only)
+//   warps 4-11  take the sums out of TMEM, finish them, and write 32 x 32 blocks out through shared memory and TMA stores
+#include "dense.cuh"
+
+#include <algorithm>
+
+__device__ int g_dmoq_dense_pair_status = 0;
+
+namespace dense {
+namespace {
+
+constexpr int kStages = 5;
+constexpr int kStageBytes = 2 * 128 * 128;
+constexpr int kEpiWarps = 8;
+constexpr int kUnitBytes = 32 * 64;                       // 32 rows of 32 16-bit outputs on their way out
+constexpr int kUnits = 4;                                 // per epilogue warp
+constexpr int kUnitBase = kStages * kStageBytes;
+constexpr int kBarBase = kUnitBase + kEpiWarps * kUnits * kUnitBytes;
+constexpr int kSmem = kBarBase + 256 + 1024;
+constexpr int kThreads = 32 * (4 + kEpiWarps);
+constexpr int kGroupM = 8;                                // tile rows that are walked together, so that both operands are shared in L2
+
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t leader_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(leader_bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x),
+               "r"(y), "r"(src)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void tma_store_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+// completes on the barrier at this address in both blocks of the pair
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+               "h"((uint16_t)3)
+               : "memory");
+}
+
+template <int KIND, bool AMN, bool BMN, int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    dense_pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args a) {
+  constexpr bool kDual = is_dual(EPI);
+  constexpr int kCols = kDual ? 128 : 256;                 // output columns of a tile
+  constexpr int kBK = KIND == KIND_I8 ? 128 : 64;
+  extern __shared__ uint8_t smem_raw[];
+  uint32_t sb = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  asm volatile("" : "+r"(sb));
+  auto stage_a = [&](uint32_t s) { return sb + s * kStageBytes; };
+  auto stage_b = [&](uint32_t s) { return sb + s * kStageBytes + 128 * 128; };
+  auto bar_full = [&](uint32_t s) { return sb + kBarBase + 8 * s; };
+  auto bar_empty = [&](uint32_t s) { return sb + kBarBase + 64 + 8 * s; };
+  auto bar_acc_full = [&](uint32_t b) { return sb + kBarBase + 128 + 8 * b; };
+  auto bar_acc_empty = [&](uint32_t b) { return sb + kBarBase + 144 + 8 * b; };
+  const uint32_t bar_drain = sb + kBarBase + 160, tmem_slot = sb + kBarBase + 168, abort_flag = sb + kBarBase + 172;
+  int* status = &g_dmoq_dense_pair_status;
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int tiles_m = (a.M + 255) / 256, tiles_n = (a.N + kCols - 1) / kCols;
+  const int tiles = tiles_m * tiles_n;
+  const int seg_steps = (a.K + kBK - 1) / kBK, steps = seg_steps * a.segs;
+  auto tile_at = [&](int t, int& m0, int& n0) {            // columns of up to kGroupM tile rows, one tile column after the other
+    const int group = t / (kGroupM * tiles_n), first = group * kGroupM;
+    const int height = min(kGroupM, tiles_m - first), local = t - group * kGroupM * tiles_n;
+    m0 = (first + local % height) * 256 + (int)rank * 128;
+    n0 = local / height * kCols;
+  };
+
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar_full(s), 1);
+      mbar_init(bar_empty(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar_acc_full(b), 1);
+      mbar_init(bar_acc_empty(b), 2 * kEpiWarps);
+    }
+    mbar_init(bar_drain, 1);
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(abort_flag), "r"(0) : "memory");
+    mbar_init_fence();
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t done = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        int m0, n0;
+        tile_at(t, m0, n0);
+        for (int it = 0; it < steps; ++it, ++done) {
+          const uint32_t s = done % kStages;
+          if (done >= kStages && !mbar_wait(bar_empty(s), (done / kStages - 1) & 1, abort_flag, status)) {
+            ok = false;
+            break;
+          }
+          const uint32_t full = map_to_rank(bar_full(s), 0);
+          if (rank == 0) mbar_arrive_expect_tx(bar_full(s), 2 * kStageBytes);
+          const int seg = it >= seg_steps ? 1 : 0, k = (it - seg * seg_steps) * kBK;
+          if (AMN) {
+            tma_load_pair(stage_a(s), &maps.a[seg], m0, k, full);
+            tma_load_pair(stage_a(s) + 8192, &maps.a[seg], m0 + 64, k, full);
+          } else {
+            tma_load_pair(stage_a(s), &maps.a[seg], k, m0, full);
+          }
+          const int nb = kDual ? n0 : n0 + (int)rank * 128;
+          const CUtensorMap* mb = &maps.b[kDual ? (int)rank : seg];
+          if (BMN) {
+            tma_load_pair(stage_b(s), mb, nb, k, full);
+            tma_load_pair(stage_b(s) + 8192, mb, nb + 64, k, full);
+          } else {
+            tma_load_pair(stage_b(s), mb, k, nb, full);
+          }
+        }
+      }
+      // after an abort copies may still be on their way into either block; the leader's barriers count both blocks' bytes
+      if (!ok && rank == 0)
+        for (uint32_t j = done > kStages ? done - kStages : 0u; j < done; ++j) mbar_wait_quiet(bar_full(j % kStages), (j / kStages) & 1);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t shape = (32u << 17) | (16u << 24);
+      const uint32_t type = a.bf16 ? 1u : 0u;
+      const uint32_t idesc = KIND == KIND_I8 ? (2u << 4) | (1u << 7) | (1u << 10) | shape
+                                             : (1u << 4) | (type << 7) | (type << 10) | (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u) | shape;
+      constexpr uint32_t step_a = AMN ? 128 : 2, step_b = BMN ? 128 : 2;
+      uint32_t done = 0, i = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs, ++i) {
+        const uint32_t b = i & 1, d = tmem + b * 256;
+        if (i >= 2 && !mbar_wait(bar_acc_empty(b), (i / 2 - 1) & 1, abort_flag, status)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        for (int it = 0; it < steps; ++it, ++done) {
+          const uint32_t s = done % kStages;
+          if (!mbar_wait(bar_full(s), (done / kStages) & 1, abort_flag, status)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t da = operand_desc(stage_a(s), AMN ? 8192 : 16), db = operand_desc(stage_b(s), BMN ? 8192 : 16);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t acc = (it > 0 || k > 0) ? 1u : 0u;
+            if (KIND == KIND_I8) {
+              asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                           "l"(da + step_a * k), "l"(db + step_b * k), "r"(idesc), "r"(acc)
+                           : "memory");
+            } else {
+              asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                           "l"(da + step_a * k), "l"(db + step_b * k), "r"(idesc), "r"(acc)
+                           : "memory");
+            }
+          }
+          commit_pair(bar_empty(s));
+        }
+        if (ok) commit_pair(bar_acc_full(b));
+      }
+      if (!ok) {   // no product may still read shared memory when the blocks end
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_drain) : "memory");
+        mbar_wait_quiet(bar_drain, 0);
+      }
+    }
+  } else if (warp >= 4) {
+    const int e = warp - 4, quarter = e & 3, side = e >> 2;
+    const uint32_t units = sb + kUnitBase + e * (kUnits * kUnitBytes);
+    uint32_t i = 0, n_out = 0;
+    for (int t = pair; t < tiles; t += pairs, ++i) {
+      int m0, n0;
+      tile_at(t, m0, n0);
+      const uint32_t b = i & 1;
+      const int row0 = m0 + quarter * 32;
+      const long long row = row0 + lane;
+      const float sa = KIND == KIND_I8 && row < a.M ? a.a_scale[row] : 0.f;
+      if (!mbar_wait(bar_acc_full(b), (i / 2) & 1, abort_flag, status)) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + b * 256;
+      constexpr int kBlocks = kDual ? 2 : 4;               // 32-column blocks of this warp
+#pragma unroll 1
+      for (int u = 0; u < kBlocks; ++u) {
+        const int c = side * (kBlocks * 32) + u * 32, col0 = n0 + c;
+        uint32_t v[32], w[32];
+        tc_ld32(acc + c, v);
+        if (kDual) tc_ld32(acc + 128 + c, w);
+        uint4 in[3][4];
+        if (EPI == EPI_GRAD && row < a.M) {                // rows of the planes are whole groups of eight elements
+#pragma unroll
+          for (int p = 0; p < 3; ++p)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (col0 + 8 * j < a.N) in[p][j] = *reinterpret_cast<const uint4*>(a.in[p] + row * a.ld_in + col0 + 8 * j);
+        }
+        float sc0 = 1.f, sc1 = 1.f, bias = 0.f;            // of column col0 + lane
+        if (KIND == KIND_I8 && col0 + lane < a.N) {
+          sc0 = a.b_scale[0][col0 + lane];
+          if (kDual) sc1 = a.b_scale[1][col0 + lane];
+          if (EPI == EPI_SCALE && a.bias) bias = unpack16(a.bias[col0 + lane], a.bf16);
+        }
+        tc_wait_ld();
+        if (u == kBlocks - 1) {                            // the sums are in registers: the accumulator goes back to the leader
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            const uint32_t remote = map_to_rank(bar_acc_empty(b), 0);
+            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
+          }
+        }
+        uint32_t o[outputs_of(EPI)][16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          float x[2], y[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int q = 2 * j + h;
+            if (KIND == KIND_I8) {
+              x[h] = (float)(int)v[q] * (sa * __shfl_sync(0xffffffffu, sc0, q));
+              if (kDual) y[h] = (float)(int)w[q] * (sa * __shfl_sync(0xffffffffu, sc1, q));
+              if (EPI == EPI_SCALE) x[h] += __shfl_sync(0xffffffffu, bias, q);
+            } else {
+              x[h] = __uint_as_float(v[q]);
+              if (kDual) y[h] = __uint_as_float(w[q]);
+            }
+          }
+          if (EPI == EPI_OUT || EPI == EPI_SCALE) {
+            o[0][j] = pack16(x[0], x[1], a.bf16);
+          } else if (EPI == EPI_SILU) {
+            o[0][j] = pack16(x[0] * sigmoid(x[0]) * y[0], x[1] * sigmoid(x[1]) * y[1], a.bf16);
+          } else if (EPI == EPI_SILU_SAVE) {
+            float si[2], sl[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float s = sigmoid(x[h]);
+              si[h] = x[h] * s;
+              sl[h] = y[h] * (s + si[h] * (1.f - s));
+            }
+            o[0][j] = pack16(si[0] * y[0], si[1] * y[1], a.bf16);
+            o[1 % outputs_of(EPI)][j] = (__float_as_uint(si[0]) >> 16) | (__float_as_uint(si[1]) & 0xffff0000u);
+            o[2 % outputs_of(EPI)][j] = (__float_as_uint(sl[0]) >> 16) | (__float_as_uint(sl[1]) & 0xffff0000u);
+            o[3 % outputs_of(EPI)][j] = saved_low(si[0], sl[0]) | (saved_low(si[1], sl[1]) << 16);
+          } else {
+            auto word = [&](int p) {
+              const uint4 q = in[p][j / 4];
+              return (j & 3) == 0 ? q.x : (j & 3) == 1 ? q.y : (j & 3) == 2 ? q.z : q.w;
+            };
+            const uint32_t s2 = word(0), p2 = word(1), l2 = word(2);
+            o[0][j] = pack16(x[0] * saved_slope(p2 & 0xffffu, l2 & 0xffffu), x[1] * saved_slope(p2 >> 16, l2 >> 16), a.bf16);
+            o[1 % outputs_of(EPI)][j] = pack16(x[0] * saved_silu(s2 & 0xffffu, l2 & 0xffffu), x[1] * saved_silu(s2 >> 16, l2 >> 16), a.bf16);
+          }
+        }
+        if (row0 >= a.M || col0 >= a.N) continue;
+#pragma unroll
+        for (int p = 0; p < outputs_of(EPI); ++p, ++n_out) {
+          const uint32_t unit = units + (n_out % kUnits) * kUnitBytes;
+          if (lane == 0) tma_store_wait_read<kUnits - 1>();   // the store that used this unit four stores ago has read it
+          __syncwarp();
+          const uint32_t line = unit + lane * 64, swz = (lane >> 1) & 3;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) st_shared_v4(line + ((j ^ swz) << 4), o[p][4 * j], o[p][4 * j + 1], o[p][4 * j + 2], o[p][4 * j + 3]);
+          if (a.vec) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tma_store(&maps.out[p], unit, col0, row0);
+          } else {                                         // rows that are not 16-byte aligned: 64-byte runs of a row at a time
+            __syncwarp();
+            for (int r = 0; r < 32 && row0 + r < a.M; ++r) {
+              const uint32_t at = unit + r * 64 + ((((uint32_t)lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2;
+              uint16_t val;
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(val) : "r"(at) : "memory");
+              if (col0 + lane < a.N) a.out[p][(row0 + r) * a.ld_out + col0 + lane] = val;
+            }
+            __syncwarp();
+          }
+        }
+      }
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  if (warp == 2) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
+template <int KIND, bool AMN, bool BMN, int EPI>
+int launch(const Maps& maps, const Args& a, cudaStream_t s) {
+  static DmoqOncePerDevice once;
+  bool* configured = once.slot();
+  if (configured == nullptr) return DMOQ_EDEVICE;
+  auto* kernel = dense_pair_kernel<KIND, AMN, BMN, EPI>;
+  if (!*configured) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return DMOQ_ELAUNCH;
+    *configured = true;
+  }
+  constexpr int kCols = is_dual(EPI) ? 128 : 256;
+  const long long tiles = (long long)dmoq_ceil_div(a.M, 256) * dmoq_ceil_div(a.N, kCols);
+  if (tiles > 0x3fffffffLL) return DMOQ_ESIZE;
+  const int pairs = (int)std::min<long long>(tiles, dmoq_sm_count() / 2);
+  kernel<<<2 * pairs, kThreads, kSmem, s>>>(maps, a);
+  return dmoq_launch_status();
+}
+
+}  // namespace
+
+int pair_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, const Args& a, cudaStream_t s) {
+  const int key = kind * 1000 + a_mn * 200 + b_mn * 100 + epi;
+  switch (key) {
+    case EPI_OUT: return launch<KIND_16, false, false, EPI_OUT>(maps, a, s);
+    case EPI_SILU: return launch<KIND_16, false, false, EPI_SILU>(maps, a, s);
+    case EPI_SILU_SAVE: return launch<KIND_16, false, false, EPI_SILU_SAVE>(maps, a, s);
+    case 100 + EPI_OUT: return launch<KIND_16, false, true, EPI_OUT>(maps, a, s);
+    case 100 + EPI_GRAD: return launch<KIND_16, false, true, EPI_GRAD>(maps, a, s);
+    case 300 + EPI_OUT: return launch<KIND_16, true, true, EPI_OUT>(maps, a, s);
+    case 1000 + EPI_SCALE: return launch<KIND_I8, false, false, EPI_SCALE>(maps, a, s);
+    case 1000 + EPI_SILU: return launch<KIND_I8, false, false, EPI_SILU>(maps, a, s);
+    default: return DMOQ_EINVAL;
+  }
+}
+
+}  // namespace dense
+
+int dmoq_dense_pair_status(int* out) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_dmoq_dense_pair_status, sizeof(int)) != cudaSuccess) return DMOQ_EDEVICE;
+  *out = v;
+  return DMOQ_OK;
+}

@@ -5,8 +5,9 @@
 
 #include "common.cuh"
 
-// Status word of the dense kernels on the current device (defined in dense_tile.cu): bit 0 = a bounded wait ran out.
+// Status word of the dense kernels on the current device: bit 0 = a bounded wait ran out.
 int dmoq_dense_status(int* out);
+int dmoq_dense_pair_status(int* out);
 
 namespace dense {
 

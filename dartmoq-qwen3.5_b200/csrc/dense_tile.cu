@@ -171,19 +171,16 @@ __global__ void __launch_bounds__(256, 1) dense_tile_kernel(const __grid_constan
     const long long at_out = row * a.ld_out + col;
     float o[3][4];
     if (EPI == EPI_GRAD) {
-      const long long at_in = row * a.ld_in + col;
-      uint32_t s[4], p[4];
-      if (a.vec) {
-        const uint2 s2 = *reinterpret_cast<const uint2*>(a.in0 + at_in), p2 = *reinterpret_cast<const uint2*>(a.in1 + at_in);
-        s[0] = s2.x & 0xffffu, s[1] = s2.x >> 16, s[2] = s2.y & 0xffffu, s[3] = s2.y >> 16;
-        p[0] = p2.x & 0xffffu, p[1] = p2.x >> 16, p[2] = p2.y & 0xffffu, p[3] = p2.y >> 16;
-      } else {
-        for (int j = 0; j < 4; ++j) s[j] = j < n ? a.in0[at_in + j] : 0u, p[j] = j < n ? a.in1[at_in + j] : 0u;
-      }
+      const long long at_in = row * a.ld_in + col;   // the planes' rows are whole groups of four (sizes are multiples of 8)
+      uint2 pl[3];
+#pragma unroll
+      for (int e = 0; e < 3; ++e) pl[e] = *reinterpret_cast<const uint2*>(a.in[e] + at_in);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        o[0][j] = __uint_as_float(v[j]) * unpack16(p[j], a.bf16);
-        o[1][j] = __uint_as_float(v[j]) * unpack16(s[j], a.bf16);
+        auto half = [&](const uint2 w) { return ((j < 2 ? w.x : w.y) >> (16 * (j & 1))) & 0xffffu; };
+        const float dh = __uint_as_float(v[j]);
+        o[0][j] = dh * saved_slope(half(pl[1]), half(pl[2]));
+        o[1][j] = dh * saved_silu(half(pl[0]), half(pl[2]));
       }
     } else {
 #pragma unroll
@@ -193,12 +190,18 @@ __global__ void __launch_bounds__(256, 1) dense_tile_kernel(const __grid_constan
         o[0][j] = e[0], o[1][j] = e[1], o[2][j] = e[2];
       }
     }
-    constexpr int kOuts = EPI == EPI_SILU_SAVE ? 3 : EPI == EPI_GRAD ? 2 : 1;
-    uint16_t* outs[3] = {a.out0, a.out1, a.out2};
 #pragma unroll
-    for (int e = 0; e < kOuts; ++e) {
-      const uint32_t lo = pack16(o[e][0], o[e][1], a.bf16), hi = pack16(o[e][2], o[e][3], a.bf16);
-      uint16_t* dst = outs[e] + at_out;
+    for (int e = 0; e < outputs_of(EPI); ++e) {
+      uint32_t lo, hi;
+      if (EPI == EPI_SILU_SAVE && e > 0) {
+        auto word = [&](int j) {
+          return e == 3 ? saved_low(o[1][j], o[2][j]) : __float_as_uint(o[e < 3 ? e : 0][j]) >> 16;
+        };
+        lo = word(0) | (word(1) << 16), hi = word(2) | (word(3) << 16);
+      } else {
+        lo = pack16(o[e < 3 ? e : 0][0], o[e < 3 ? e : 0][1], a.bf16), hi = pack16(o[e < 3 ? e : 0][2], o[e < 3 ? e : 0][3], a.bf16);
+      }
+      uint16_t* dst = a.out[e] + at_out;
       if (a.vec) {
         *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
       } else {
@@ -261,6 +264,9 @@ int tile_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, cons
 int dmoq_dense_status(int* out) {
   int v = 0;
   if (cudaMemcpyFromSymbol(&v, g_dmoq_dense_status, sizeof(int)) != cudaSuccess) return DMOQ_EDEVICE;
-  *out = v;
+  int w = 0;
+  const int rc = dmoq_dense_pair_status(&w);
+  if (rc != DMOQ_OK) return rc;
+  *out = v | w;
   return DMOQ_OK;
 }

@@ -44,8 +44,8 @@ def _rows(t: torch.Tensor, cols: int) -> Tuple[torch.Tensor, int]:
     if t.dim() != 2:
         t = t.reshape(-1, cols)
     n = t.shape[0]
-    if n >= 1 << 31:
-        raise ValueError(f"at most 2^31 - 1 rows, got {n}")
+    if n > 1 << 30:
+        raise ValueError(f"at most 2^30 rows, got {n}")
     pitch = t.stride(0) if n > 1 else cols
     per16 = 16 // t.element_size()
     if t.stride(1) != 1 or pitch < cols or pitch % per16 or t.data_ptr() % 16:
@@ -183,33 +183,34 @@ def int8_gated_linear(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.T
 
 
 def _ffn_forward(x: torch.Tensor, pitch: int, wg: torch.Tensor, wu: torch.Tensor, wd: torch.Tensor, save: bool):
-    """y, and the hidden values h; with ``save`` also silu(g) and u silu'(g)."""
+    """y, and the hidden values h; with ``save`` also what the gradients need of them."""
     (t, hidden), inter, dev = x.shape, wg.shape[0], x.device
-    bufs = torch.empty((3 if save else 1, t, inter), dtype=x.dtype, device=dev)
+    h = torch.empty((t, inter), dtype=x.dtype, device=dev)
+    saved = torch.empty((3, t, inter), dtype=torch.int16, device=dev) if save else None
     y = torch.empty((t, hidden), dtype=x.dtype, device=dev)
-    h, silu, slope = bufs.unbind(0) if save else (bufs[0], None, None)
     _call("dmoq_gated_ffn", dev, x.data_ptr(), x.dtype == torch.bfloat16, pitch, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), t,
-          hidden, inter, h.data_ptr(), _ptr(silu), _ptr(slope), y.data_ptr())
-    return y, h, silu, slope
+          hidden, inter, h.data_ptr(), _ptr(saved), y.data_ptr())
+    return y, h, saved
 
 
 class _GatedFeedForward(torch.autograd.Function):
-    """What the gradients need of the hidden values is kept as silu(g) and u silu'(g), each rounded once to 16 bits like h, not
-    as g and u: dg = dh * (u silu'(g)) and du = dh * silu(g) then carry one stored rounding each, and backward computes no
-    exponentials.  dg and du are rounded to 16 bits because they are operands of the next products."""
+    """What the gradients need of the hidden values is kept as silu(g) and u silu'(g) to 24 bits each, not as g and u in 16: dg =
+    dh * (u silu'(g)) and du = dh * silu(g) are then rounded to 16 bits (they are operands of the next products) from values
+    that carry no other rounding of that type, and backward computes no exponentials.  With h that is 8 bytes a hidden
+    value, as much as g, u, silu(g) and h in 16 bits."""
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down):
         rows, pitch = _rows(x, x.shape[-1])
         inner = any(ctx.needs_input_grad[:3])
-        y, h, silu, slope = _ffn_forward(rows, pitch, w_gate, w_up, w_down, inner)
-        ctx.save_for_backward(rows, w_gate, w_up, w_down, h if ctx.needs_input_grad[3] else None, silu, slope)
+        y, h, saved = _ffn_forward(rows, pitch, w_gate, w_up, w_down, inner)
+        ctx.save_for_backward(rows, w_gate, w_up, w_down, h if ctx.needs_input_grad[3] else None, saved)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, wg, wu, wd, h, silu, slope = ctx.saved_tensors
+        x, wg, wu, wd, h, saved = ctx.saved_tensors
         need_x, need_g, need_u, need_d = ctx.needs_input_grad
         (t, hidden), inter, dev, dt = x.shape, wg.shape[0], x.device, x.dtype
         dy, dy_pitch = _rows(dy, hidden)
@@ -223,7 +224,7 @@ class _GatedFeedForward(torch.autograd.Function):
         dwu = dw[-1] if need_u else None
         dwd = torch.empty((hidden, inter), dtype=dt, device=dev) if need_d else None
         _call("dmoq_gated_ffn_backward", dev, dy.data_ptr(), dy_pitch, x.data_ptr(), dt == torch.bfloat16, x_pitch, wg.data_ptr(),
-              wu.data_ptr(), wd.data_ptr(), t, hidden, inter, _ptr(h), _ptr(silu), _ptr(slope), _ptr(dgu), _ptr(dx), _ptr(dwg),
+              wu.data_ptr(), wd.data_ptr(), t, hidden, inter, _ptr(h), _ptr(saved), _ptr(dgu), _ptr(dx), _ptr(dwg),
               _ptr(dwu), _ptr(dwd))
         return dx, dwg, dwu, dwd
 

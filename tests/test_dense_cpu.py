@@ -48,18 +48,18 @@ def test_int8_products_refuse():
 
 def test_gated_ffn_refuses():
     lib = _lib.load()
-    good = [P, 1, 64, P, P, P, 4, 64, 32, P, None, None, P]
+    good = [P, 1, 64, P, P, P, 4, 64, 32, P, None, P]
     assert lib.dmoq_gated_ffn(*(good[:6] + [0] + good[7:]), None) == OK
-    for i in (0, 3, 4, 5, 9, 12):
+    for i in (0, 3, 4, 5, 9, 11):
         assert lib.dmoq_gated_ffn(*(good[:i] + [None] + good[i + 1:]), None) == EINVAL, i
-    for i, v in ((2, 60), (2, 68), (7, 60), (7, 0), (8, 12), (8, 0), (6, -4), (10, P), (11, P), (0, ODD), (3, ODD), (4, ODD), (5, ODD),
-                 (9, ODD), (12, ODD)):
+    for i, v in ((2, 60), (2, 68), (7, 60), (7, 0), (8, 12), (8, 0), (6, -4), (10, ODD), (0, ODD), (3, ODD), (4, ODD), (5, ODD),
+                 (9, ODD), (11, ODD)):
         assert lib.dmoq_gated_ffn(*(good[:i] + [v] + good[i + 1:]), None) == EINVAL, (i, v)
-    #       dy pitch x bf pitch wg wu wd  T   H   I  h silu slope dgu dx dwg dwu dwd
-    good = [P, 64, P, 1, 64, P, P, P, 4, 64, 32, P, P, P, P, P, P, P, P]
-    for i in (0, 2, 5, 6, 7, 11, 12, 13, 14):
+    #       dy pitch x bf pitch wg wu wd  T   H   I  h saved dgu dx dwg dwu dwd
+    good = [P, 64, P, 1, 64, P, P, P, 4, 64, 32, P, P, P, P, P, P, P]
+    for i in (0, 2, 5, 6, 7, 11, 12, 13):
         assert lib.dmoq_gated_ffn_backward(*(good[:i] + [None] + good[i + 1:]), None) == EINVAL, i
-    for i, v in ((1, 60), (4, 60), (9, 4), (10, 12), (0, ODD), (2, ODD), (11, ODD), (12, ODD), (14, ODD), (15, ODD), (16, ODD), (18, ODD)):
+    for i, v in ((1, 60), (4, 60), (9, 4), (10, 12), (0, ODD), (2, ODD), (11, ODD), (12, ODD), (13, ODD), (14, ODD), (15, ODD), (17, ODD)):
         assert lib.dmoq_gated_ffn_backward(*(good[:i] + [v] + good[i + 1:]), None) == EINVAL, (i, v)
 
 

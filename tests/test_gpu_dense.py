@@ -93,7 +93,7 @@ def test_quantize_shapes_and_strides():
 # --------------------------------------------------------------------------------------------- 8-bit products
 
 SIZES8 = [(1, 1, 16), (1, 33, 128), (2, 512, 2048), (7, 1001, 144), (16, 256, 2064), (17, 96, 4096), (64, 640, 512), (127, 130, 272),
-          (129, 257, 1024), (300, 1001, 2064), (700, 4096, 256), (1300, 2200, 640)]
+          (129, 257, 1024), (300, 1001, 2064), (700, 4096, 256), (1300, 2200, 640), (1545, 2201, 144)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -190,7 +190,7 @@ def test_int8_shapes_strides_and_refusals():
 # --------------------------------------------------------------------------------------------- gated feed-forward
 
 FFN_SIZES = [(1, 8, 8), (1, 256, 136), (3, 72, 200), (16, 512, 256), (33, 128, 1032), (64, 256, 72), (128, 320, 128), (129, 264, 136),
-             (257, 1032, 520), (1000, 256, 128), (640, 520, 1040)]
+             (257, 1032, 520), (1000, 256, 128), (640, 520, 1040), (1500, 1032, 1544)]
 
 
 def ffn_inputs(t, h, i, dtype, seed=0):
@@ -201,9 +201,8 @@ def ffn_inputs(t, h, i, dtype, seed=0):
     return x, wg, wu, wd, randn(g, t, h, dtype=dtype)
 
 
-# y: hidden values and y rounded.  dw_down: hidden values and the gradient.  The others: what is kept of the hidden values, dg
-# or du, the gradient.
-ROUNDINGS = {"y": 2, "dx": 3, "dw_gate": 3, "dw_up": 3, "dw_down": 2}
+# y: hidden values and y rounded.  dw_down: hidden values and the gradient.  The others: dg or du, and the gradient.
+ROUNDINGS = {"y": 2, "dx": 2, "dw_gate": 2, "dw_up": 2, "dw_down": 2}
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -247,7 +246,7 @@ def test_ffn_gradients_against_differences(dtype):
         loss = lambda e: float((R.ffn(*[b + (e * way if j == i else 0) for j, b in enumerate(base)])[3] * dy.double().cpu()).sum())  # noqa: E731
         slope = (loss(eps) - loss(-eps)) / (2 * eps)
         mine = float((grad.double().cpu() * way).sum())
-        assert abs(mine - slope) <= 3 * R.half(dtype) * abs(slope) + 1e-6 * abs(slope), (i, mine, slope)
+        assert abs(mine - slope) <= 2 * R.half(dtype) * abs(slope) + 1e-6 * abs(slope), (i, mine, slope)
 
 
 def test_ffn_computes_only_the_gradients_that_are_needed():
@@ -327,19 +326,19 @@ def test_outputs_stay_inside_their_memory():
     t, h, i = 130, 136, 72
     x, wg, wu, wd, dy = ffn_inputs(t, h, i, torch.bfloat16)
     pad = lambda r, c: torch.full((r + 2, c), 7.0, dtype=torch.bfloat16, device=DEV)  # noqa: E731
-    hid, si, sl, y = pad(t, i), pad(t, i), pad(t, i), pad(t, h)
+    hid, saved, y = pad(t, i), pad(3 * t, i), pad(t, h)
     dgu, dx, dw, dwd = pad(t, 2 * i), pad(t, h), pad(2 * i, h), pad(h, i)
     q = lambda v: C.c_void_p(v[1].data_ptr())  # noqa: E731
-    _lib.check(lib.dmoq_gated_ffn(p(x), 1, h, p(wg), p(wu), p(wd), t, h, i, q(hid), q(si), q(sl), q(y), None), "ffn")
-    _lib.check(lib.dmoq_gated_ffn_backward(p(dy), h, p(x), 1, h, p(wg), p(wu), p(wd), t, h, i, q(hid), q(si), q(sl), q(dgu), q(dx), q(dw),
+    _lib.check(lib.dmoq_gated_ffn(p(x), 1, h, p(wg), p(wu), p(wd), t, h, i, q(hid), q(saved), q(y), None), "ffn")
+    _lib.check(lib.dmoq_gated_ffn_backward(p(dy), h, p(x), 1, h, p(wg), p(wu), p(wd), t, h, i, q(hid), q(saved), q(dgu), q(dx), q(dw),
                                            C.c_void_p(dw[1 + i].data_ptr()), q(dwd), None), "ffn backward")
     torch.cuda.synchronize()
-    for v in (hid, si, sl, y, dgu, dx, dw, dwd):
+    for v in (hid, saved, y, dgu, dx, dw, dwd):
         assert (v[0] == 7.0).all() and (v[-1] == 7.0).all()
-    R.close(dw[1:1 + 2 * i], torch.cat([R.ffn_grads(x, wg, wu, wd, dy)[k] for k in ("dw_gate", "dw_up")]), 3, "dw")
+    R.close(dw[1:1 + 2 * i], torch.cat([R.ffn_grads(x, wg, wu, wd, dy)[k] for k in ("dw_gate", "dw_up")]), 2, "dw")
     # the gradients of the two projections in memory that is not adjacent: two products
     a, b = pad(i, h), pad(i, h)
-    _lib.check(lib.dmoq_gated_ffn_backward(p(dy), h, p(x), 1, h, None, None, p(wd), t, h, i, None, q(si), q(sl), q(dgu), None, q(a), q(b),
+    _lib.check(lib.dmoq_gated_ffn_backward(p(dy), h, p(x), 1, h, None, None, p(wd), t, h, i, None, q(saved), q(dgu), None, q(a), q(b),
                                            None, None), "ffn backward")
     torch.cuda.synchronize()
     assert torch.equal(a[1:-1], dw[1:1 + i]) and torch.equal(b[1:-1], dw[1 + i:1 + 2 * i])
