@@ -1,12 +1,19 @@
 // C entry points of the dense operators: argument checks, tensor maps, choice of the kernel.
 #include "dense.cuh"
 
+int dmoq_token_quant_launch(const void* x, int bf16, int T, int K, long long pitch, int8_t* codes, float* scales, cudaStream_t s);
+
 namespace dense {
 
 int tile_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, const Args& a, int splits, cudaStream_t s);
 int pair_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, const Args& a, cudaStream_t s);
 
+int few_product(int kind, int epi, const void* x, long long x_pitch, const void* w0, const void* w1, const Args& a, cudaStream_t s);
+bool few_can_fuse(int T, int K);
+
 namespace {
+
+constexpr int kFewTokens = 16;   // up to here the kernel that streams the weights through registers
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -126,28 +133,34 @@ int check_ffn(int T, int H, int I) {
   return T > kMaxDim || H > kMaxDim || I > kMaxDim / 2 ? DMOQ_ESIZE : DMOQ_OK;   // the gradients of both projections are one product of 2 I rows
 }
 
-int int8_product(const int8_t* codes, const float* scales, const int8_t* w0, const float* s0, const int8_t* w1, const float* s1,
-                 const void* bias, int bf16, int T, int N, int K, void* out, cudaStream_t s) {
+// The products of `codes`, or of the 16-bit rows x (pitch in elements), whose codes then go into `codes` / `scales` first unless
+// the kernel makes them itself.
+int int8_product(const void* x, long long x_pitch, int8_t* codes, float* scales, const int8_t* w0, const float* s0, const int8_t* w1,
+                 const float* s1, const void* bias, int bf16, int T, int N, int K, void* out, cudaStream_t s) {
+  const bool few = T <= kFewTokens, fuse = x != nullptr && few && few_can_fuse(T, K);
+  if (x != nullptr && !fuse) {
+    const int rc = dmoq_token_quant_launch(x, bf16, T, K, x_pitch, codes, scales, s);
+    if (rc != DMOQ_OK) return rc;
+  }
   Product p;
   p.kind = KIND_I8;
   p.epi = w1 ? EPI_SILU : EPI_SCALE;
-  p.a[0] = {codes, T, K, K};
-  p.b[0] = {w0, N, K, K};
-  if (w1) p.b[1] = {w1, N, K, K};
   Args& a = p.args;
   a.M = T, a.N = N, a.K = K, a.segs = 1, a.bf16 = bf16;
-  a.a_scale = scales, a.b_scale[0] = s0, a.b_scale[1] = s1;
+  a.a_scale = fuse ? nullptr : scales, a.b_scale[0] = s0, a.b_scale[1] = s1;
   a.bias = static_cast<const uint16_t*>(bias);
   a.out[0] = static_cast<uint16_t*>(out);
   a.ld_out = N;
   a.vec = vec4(out, N, N);
+  if (few) return few_product(KIND_I8, p.epi, fuse ? x : codes, fuse ? 2 * x_pitch : K, w0, w1, a, s);
+  p.a[0] = {codes, T, K, K};
+  p.b[0] = {w0, N, K, K};
+  if (w1) p.b[1] = {w1, N, K, K};
   return run(p, s);
 }
 
 }  // namespace
 }  // namespace dense
-
-int dmoq_token_quant_launch(const void* x, int bf16, int T, int K, long long pitch, int8_t* codes, float* scales, cudaStream_t s);
 
 using namespace dense;
 
@@ -165,18 +178,8 @@ extern "C" int dmoq_int8_gemm(const int8_t* codes, const float* scales, const in
   const int rc = check_sizes8(T, N, K);
   if (rc != DMOQ_OK || T == 0) return rc;
   DMOQ_CHECK_ARG(usable(codes) && scales && weight8_ok(w, w_scale) && out);
-  return int8_product(codes, scales, w, w_scale, nullptr, nullptr, bias, is_bf16, T, N, K, out, static_cast<cudaStream_t>(stream));
-}
-
-extern "C" int dmoq_int8_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w, const float* w_scale, const void* bias,
-                                int32_t T, int32_t N, int32_t K, int8_t* codes, float* scales, void* out, void* stream) {
-  const int rc = check_sizes8(T, N, K);
-  if (rc != DMOQ_OK || T == 0) return rc;
-  DMOQ_CHECK_ARG(quant_ok(x, x_pitch, K, codes, scales) && weight8_ok(w, w_scale) && out);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int rq = dmoq_token_quant_launch(x, is_bf16, T, K, x_pitch, codes, scales, s);
-  if (rq != DMOQ_OK) return rq;
-  return int8_product(codes, scales, w, w_scale, nullptr, nullptr, bias, is_bf16, T, N, K, out, s);
+  return int8_product(nullptr, 0, const_cast<int8_t*>(codes), const_cast<float*>(scales), w, w_scale, nullptr, nullptr, bias, is_bf16, T, N, K,
+                      out, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int dmoq_int8_gated_gemm(const int8_t* codes, const float* scales, const int8_t* w_gate, const float* gate_scale,
@@ -185,19 +188,36 @@ extern "C" int dmoq_int8_gated_gemm(const int8_t* codes, const float* scales, co
   const int rc = check_sizes8(T, I, K);
   if (rc != DMOQ_OK || T == 0) return rc;
   DMOQ_CHECK_ARG(usable(codes) && scales && weight8_ok(w_gate, gate_scale) && weight8_ok(w_up, up_scale) && out);
-  return int8_product(codes, scales, w_gate, gate_scale, w_up, up_scale, nullptr, is_bf16, T, I, K, out, static_cast<cudaStream_t>(stream));
+  return int8_product(nullptr, 0, const_cast<int8_t*>(codes), const_cast<float*>(scales), w_gate, gate_scale, w_up, up_scale, nullptr, is_bf16,
+                      T, I, K, out, static_cast<cudaStream_t>(stream));
+}
+
+// scratch of the two calls below: the codes, then the scales (T K is a multiple of 16)
+extern "C" size_t dmoq_int8_scratch_bytes(int32_t T, int32_t K) {
+  if (check_sizes8(T, 1, K) != DMOQ_OK || few_can_fuse(T, K)) return 0;
+  return (size_t)T * K + (size_t)T * sizeof(float);
+}
+
+extern "C" int dmoq_int8_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w, const float* w_scale, const void* bias,
+                                int32_t T, int32_t N, int32_t K, void* scratch, void* out, void* stream) {
+  const int rc = check_sizes8(T, N, K);
+  if (rc != DMOQ_OK || T == 0) return rc;
+  DMOQ_CHECK_ARG(rows_usable(x, x_pitch, K) && weight8_ok(w, w_scale) && out && (few_can_fuse(T, K) || usable(scratch)));
+  int8_t* codes = static_cast<int8_t*>(scratch);
+  return int8_product(x, x_pitch, codes, reinterpret_cast<float*>(codes + (size_t)T * K), w, w_scale, nullptr, nullptr, bias, is_bf16, T, N, K,
+                      out, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int dmoq_int8_gated_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w_gate, const float* gate_scale,
-                                      const int8_t* w_up, const float* up_scale, int32_t T, int32_t I, int32_t K, int8_t* codes,
-                                      float* scales, void* out, void* stream) {
+                                      const int8_t* w_up, const float* up_scale, int32_t T, int32_t I, int32_t K, void* scratch, void* out,
+                                      void* stream) {
   const int rc = check_sizes8(T, I, K);
   if (rc != DMOQ_OK || T == 0) return rc;
-  DMOQ_CHECK_ARG(quant_ok(x, x_pitch, K, codes, scales) && weight8_ok(w_gate, gate_scale) && weight8_ok(w_up, up_scale) && out);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int rq = dmoq_token_quant_launch(x, is_bf16, T, K, x_pitch, codes, scales, s);
-  if (rq != DMOQ_OK) return rq;
-  return int8_product(codes, scales, w_gate, gate_scale, w_up, up_scale, nullptr, is_bf16, T, I, K, out, s);
+  DMOQ_CHECK_ARG(rows_usable(x, x_pitch, K) && weight8_ok(w_gate, gate_scale) && weight8_ok(w_up, up_scale) && out &&
+                 (few_can_fuse(T, K) || usable(scratch)));
+  int8_t* codes = static_cast<int8_t*>(scratch);
+  return int8_product(x, x_pitch, codes, reinterpret_cast<float*>(codes + (size_t)T * K), w_gate, gate_scale, w_up, up_scale, nullptr, is_bf16, T,
+                      I, K, out, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate, const void* w_up, const void* w_down,
@@ -216,7 +236,8 @@ extern "C" int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, c
   up.args.out[0] = static_cast<uint16_t*>(h);
   for (int e = 0; saved && e < 3; ++e) up.args.out[1 + e] = static_cast<uint16_t*>(saved) + e * (size_t)T * I;
   up.args.ld_out = I;
-  int rc = run(up, s);
+  const bool few = T <= kFewTokens;
+  int rc = few && !saved ? few_product(KIND_16, EPI_SILU, x, 2 * x_pitch, w_gate, w_up, up.args, s) : run(up, s);
   if (rc != DMOQ_OK) return rc;
   Product down;
   down.a[0] = {h, T, I, I};
@@ -224,7 +245,7 @@ extern "C" int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, c
   down.args.M = T, down.args.N = H, down.args.K = I, down.args.segs = 1, down.args.bf16 = is_bf16, down.args.vec = 1;
   down.args.out[0] = static_cast<uint16_t*>(y);
   down.args.ld_out = H;
-  return run(down, s);
+  return few ? few_product(KIND_16, EPI_OUT, h, 2 * (long long)I, w_down, nullptr, down.args, s) : run(down, s);
 }
 
 extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate,

@@ -10,8 +10,8 @@ The modules over them are ``linear.W8A8Linear`` and ``ffn.GatedFeedForward`` / `
 serve as ``shared_expert`` of the MoE modules.
 
 All work goes to the current stream of the tensors' device, whichever device is current; nothing synchronises and every
-buffer comes from torch's allocator.  Errors follow ``kernels``: ``DmoqError`` for tensors that are not on a CUDA device,
-``TypeError`` for a wrong dtype, ``ValueError`` for shapes.
+buffer comes from torch's allocator.  The 8-bit operators have no gradients: their results never require one.  Errors follow
+``kernels``: ``DmoqError`` for tensors that are not on a CUDA device, ``TypeError`` for a wrong dtype, ``ValueError`` for shapes.
 """
 from __future__ import annotations
 
@@ -22,36 +22,42 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 
-_HALF = (torch.bfloat16, torch.float16)
+_BF16, _FP16 = torch.bfloat16, torch.float16
+_MAX_ROWS = 1 << 30
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _call(name: str, device: torch.device, *args) -> None:
-    """One entry point on the current stream of ``device``; that device is current during the call."""
-    index = device.index
+def _call(name: str, index: int, *args) -> None:
+    """One entry point on the current stream of device ``index``, which is current during the call."""
     fn = getattr(_lib.load(), name)
     if index == torch.cuda.current_device():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+            rc = fn(*args, _raw_stream(index))
     if rc:
         _lib.check(rc, name)
 
 
-def _rows(t: torch.Tensor, cols: int) -> Tuple[torch.Tensor, int]:
+def _packed(t: torch.Tensor) -> torch.Tensor:
+    """``t``, copied only if it is not contiguous or not 16-byte aligned."""
+    return t if t.is_contiguous() and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _rows(t: torch.Tensor, cols: int) -> Tuple[torch.Tensor, int, int]:
     """``t`` as rows of ``cols`` elements that the kernels can read where they lie (unit inner stride, 16-byte aligned rows),
-    copied only if they cannot; and the pitch between rows in elements."""
+    copied only if they cannot; their number, and the pitch between them in elements."""
     if t.dim() != 2:
         t = t.reshape(-1, cols)
     n = t.shape[0]
-    if n > 1 << 30:
+    if n > _MAX_ROWS:
         raise ValueError(f"at most 2^30 rows, got {n}")
-    pitch = t.stride(0) if n > 1 else cols
-    per16 = 16 // t.element_size()
-    if t.stride(1) != 1 or pitch < cols or pitch % per16 or t.data_ptr() % 16:
+    if not t.is_contiguous() or t.data_ptr() & 15:
+        pitch = t.stride(0) if n > 1 else cols
+        if t.stride(1) == 1 and pitch >= cols and not (pitch * t.element_size() | t.data_ptr()) & 15:
+            return t, n, pitch
         t = t.clone(memory_format=torch.contiguous_format)
-        pitch = cols
-    return t, pitch
+    return t, n, cols
 
 
 def _need(cond: bool, message: str) -> None:
@@ -59,41 +65,49 @@ def _need(cond: bool, message: str) -> None:
         raise ValueError(message)
 
 
-def _check_input(x: torch.Tensor, what: str = "x") -> None:
+def _check_input(x: torch.Tensor) -> None:
     if not x.is_cuda:
         raise _lib.DmoqError("libdmoq operators take CUDA tensors only (no CPU path)")
-    if x.dtype not in _HALF:
-        raise TypeError(f"{what} must be fp16 or bf16, got {x.dtype}")
-    _need(x.dim() >= 1, f"{what} needs at least one dimension")
-
-
-def _check_weight8(w: torch.Tensor, scale: torch.Tensor, k: int, device, what: str) -> torch.Tensor:
-    if w.dtype != torch.int8 or scale.dtype != torch.float32:
-        raise TypeError(f"{what} must be int8 with an fp32 scale, got {w.dtype} and {scale.dtype}")
-    _need(w.dim() == 2 and w.shape[1] == k and w.shape[0] >= 1, f"{what} must have shape (outputs, {k}), got {tuple(w.shape)}")
-    _need(scale.numel() == w.shape[0], f"{what} needs one scale a row: {w.shape[0]} rows, {scale.numel()} scales")
-    _need(w.device == device and scale.device == device, f"{what} and its scale must be on {device}")
-    return w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
+    if x.dtype is not _BF16 and x.dtype is not _FP16:
+        raise TypeError(f"x must be fp16 or bf16, got {x.dtype}")
+    if x.dim() < 1:
+        raise ValueError("x needs at least one dimension")
 
 
 def _check_k8(k: int) -> None:
-    _need(k >= 16 and k % 16 == 0, f"8-bit products need an inner size that is a multiple of 16, got {k}")
+    if k < 16 or k & 15:
+        raise ValueError(f"8-bit products need an inner size that is a multiple of 16, got {k}")
 
 
-def _check_bias(bias: Optional[torch.Tensor], n: int, dtype, device) -> Optional[torch.Tensor]:
+def _weight8(w: torch.Tensor, scale: torch.Tensor, k: int, index: int, what: str) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The weight and its scales as the kernels take them."""
+    if w.dtype is not torch.int8 or scale.dtype is not torch.float32:
+        raise TypeError(f"{what} must be int8 with an fp32 scale, got {w.dtype} and {scale.dtype}")
+    shape = w.shape
+    if len(shape) != 2 or shape[1] != k or shape[0] < 1:
+        raise ValueError(f"{what} must have shape (outputs, {k}), got {tuple(shape)}")
+    if scale.shape != shape[:1]:
+        raise ValueError(f"{what} needs one scale a row: {shape[0]} rows, scales of shape {tuple(scale.shape)}")
+    if not (w.is_cuda and scale.is_cuda and w.get_device() == index and scale.get_device() == index):
+        raise ValueError(f"{what} and its scale must be on cuda:{index}")
+    return _packed(w), scale.contiguous()
+
+
+def _bias_ptr(bias: Optional[torch.Tensor], n: int, dtype: torch.dtype, index: int):
+    """(the bias as the kernels take it, its address); the caller holds the former until its call has been made."""
     if bias is None:
-        return None
-    if bias.dtype != dtype:
+        return None, None
+    if bias.dtype is not dtype:
         raise TypeError(f"bias must have the output's type {dtype}, got {bias.dtype}")
-    _need(tuple(bias.shape) == (n,) and bias.device == device, f"bias must have shape ({n},) on {device}")
-    return bias.contiguous()
+    _need(tuple(bias.shape) == (n,) and bias.is_cuda and bias.get_device() == index, f"bias must have shape ({n},) on cuda:{index}")
+    bias = bias.contiguous()
+    return bias, bias.data_ptr()
 
 
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-@torch.no_grad()
 def quantize_int8_tokens(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """Symmetric 8-bit codes of each row of ``x`` (..., K): scale = max|x| / 127 in fp32, code = rint(127 x / max|x|) with ties
     to even, correctly rounded.  A row of zeros has scale 0; a row with an infinity or a NaN has codes 0 and scale NaN, so
@@ -101,15 +115,13 @@ def quantize_int8_tokens(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     _check_input(x)
     k = x.shape[-1]
     _check_k8(k)
-    rows, pitch = _rows(x, k)
+    rows, t, pitch = _rows(x, k)
     codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    _call("dmoq_token_quant", x.device, rows.data_ptr(), x.dtype == torch.bfloat16, rows.shape[0], k, pitch, codes.data_ptr(),
-          scale.data_ptr())
+    _call("dmoq_token_quant", x.get_device(), rows.data_ptr(), x.dtype is _BF16, t, k, pitch, codes.data_ptr(), scale.data_ptr())
     return codes, scale
 
 
-@torch.no_grad()
 def int8_matmul(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
                 bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """out[t, n] = scale[t] * weight_scale[n] * sum_k codes[t, k] * weight[n, k] (+ bias[n]); exact int32 sums, scales and bias
@@ -117,79 +129,80 @@ def int8_matmul(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, 
     131056; any N."""
     if not codes.is_cuda:
         raise _lib.DmoqError("libdmoq operators take CUDA tensors only (no CPU path)")
-    if codes.dtype != torch.int8 or scale.dtype != torch.float32:
+    if codes.dtype is not torch.int8 or scale.dtype is not torch.float32:
         raise TypeError(f"codes must be int8 with an fp32 scale, got {codes.dtype} and {scale.dtype}")
-    if out_dtype not in _HALF:
+    if out_dtype is not _BF16 and out_dtype is not _FP16:
         raise TypeError(f"out_dtype must be fp16 or bf16, got {out_dtype}")
     _need(codes.dim() >= 1, "codes need at least one dimension")
-    k, dev = codes.shape[-1], codes.device
+    k, index = codes.shape[-1], codes.get_device()
     _check_k8(k)
-    _need(scale.shape == codes.shape[:-1] and scale.device == dev, f"one scale a token on {dev}: got {tuple(scale.shape)}")
-    w = _check_weight8(weight, weight_scale, k, dev, "weight")
+    _need(scale.shape == codes.shape[:-1] and scale.is_cuda and scale.get_device() == index,
+          f"one scale a token on cuda:{index}: got {tuple(scale.shape)}")
+    w, ws = _weight8(weight, weight_scale, k, index, "weight")
     n = w.shape[0]
-    bias = _check_bias(bias, n, out_dtype, dev)
-    a, pitch = _rows(codes, k)
+    bias, bias_ptr = _bias_ptr(bias, n, out_dtype, index)
+    a, t, pitch = _rows(codes, k)
     if pitch != k:
         a = a.contiguous()
-    scale, weight_scale = scale.contiguous(), weight_scale.contiguous()
-    out = torch.empty(codes.shape[:-1] + (n,), dtype=out_dtype, device=dev)
-    _call("dmoq_int8_gemm", dev, a.data_ptr(), scale.data_ptr(), w.data_ptr(), weight_scale.data_ptr(), _ptr(bias),
-          out_dtype == torch.bfloat16, a.shape[0], n, k, out.data_ptr())
+    scale = scale.contiguous()
+    out = torch.empty(codes.shape[:-1] + (n,), dtype=out_dtype, device=codes.device)
+    _call("dmoq_int8_gemm", index, a.data_ptr(), scale.data_ptr(), w.data_ptr(), ws.data_ptr(), bias_ptr, out_dtype is _BF16, t, n, k,
+          out.data_ptr())
     return out
 
 
-@torch.no_grad()
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
                 bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``int8_matmul(*quantize_int8_tokens(x), weight, weight_scale, bias, x.dtype)`` in one call: x (..., K) -> (..., N)."""
     _check_input(x)
-    k, dev = x.shape[-1], x.device
+    shape, index = x.shape, x.get_device()
+    k = shape[-1]
     _check_k8(k)
-    w = _check_weight8(weight, weight_scale, k, dev, "weight")
+    w, ws = _weight8(weight, weight_scale, k, index, "weight")
     n = w.shape[0]
-    bias = _check_bias(bias, n, x.dtype, dev)
-    rows, pitch = _rows(x, k)
-    t = rows.shape[0]
-    codes = torch.empty((t, k), dtype=torch.int8, device=dev)
-    scale = torch.empty((t,), dtype=torch.float32, device=dev)
-    weight_scale = weight_scale.contiguous()
-    out = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=dev)
-    _call("dmoq_int8_linear", dev, rows.data_ptr(), x.dtype == torch.bfloat16, pitch, w.data_ptr(), weight_scale.data_ptr(),
-          _ptr(bias), t, n, k, codes.data_ptr(), scale.data_ptr(), out.data_ptr())
+    bias, bias_ptr = _bias_ptr(bias, n, x.dtype, index)
+    rows, t, pitch = _rows(x, k)
+    scratch = _int8_scratch(x, t, k)
+    out = x.new_empty(shape[:-1] + (n,))
+    _call("dmoq_int8_linear", index, rows.data_ptr(), x.dtype is _BF16, pitch, w.data_ptr(), ws.data_ptr(), bias_ptr, t, n, k,
+          _ptr(scratch), out.data_ptr())
     return out
 
 
-@torch.no_grad()
+def _int8_scratch(x: torch.Tensor, t: int, k: int) -> Optional[torch.Tensor]:
+    need = _lib.load().dmoq_int8_scratch_bytes(t, k)
+    return x.new_empty((need,), dtype=torch.uint8) if need else None
+
+
 def int8_gated_linear(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tensor, w_up: torch.Tensor,
                       up_scale: torch.Tensor) -> torch.Tensor:
     """silu(g) * u with g, u the 8-bit products of x's codes with ``w_gate`` and ``w_up`` (each int8 (I, K), one scale a row):
     both products, the activation and the multiplication in one kernel, in fp32 up to one rounding.  x (..., K) -> (..., I)."""
     _check_input(x)
-    k, dev = x.shape[-1], x.device
+    shape, index = x.shape, x.get_device()
+    k = shape[-1]
     _check_k8(k)
-    wg = _check_weight8(w_gate, gate_scale, k, dev, "w_gate")
-    wu = _check_weight8(w_up, up_scale, k, dev, "w_up")
-    _need(wg.shape == wu.shape, f"w_gate and w_up must have one shape, got {tuple(wg.shape)} and {tuple(wu.shape)}")
+    wg, sg = _weight8(w_gate, gate_scale, k, index, "w_gate")
+    wu, su = _weight8(w_up, up_scale, k, index, "w_up")
     n = wg.shape[0]
-    rows, pitch = _rows(x, k)
-    t = rows.shape[0]
-    codes = torch.empty((t, k), dtype=torch.int8, device=dev)
-    scale = torch.empty((t,), dtype=torch.float32, device=dev)
-    gate_scale, up_scale = gate_scale.contiguous(), up_scale.contiguous()
-    out = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=dev)
-    _call("dmoq_int8_gated_linear", dev, rows.data_ptr(), x.dtype == torch.bfloat16, pitch, wg.data_ptr(), gate_scale.data_ptr(),
-          wu.data_ptr(), up_scale.data_ptr(), t, n, k, codes.data_ptr(), scale.data_ptr(), out.data_ptr())
+    if wu.shape[0] != n:
+        raise ValueError(f"w_gate and w_up must have one shape, got {tuple(wg.shape)} and {tuple(wu.shape)}")
+    rows, t, pitch = _rows(x, k)
+    scratch = _int8_scratch(x, t, k)
+    out = x.new_empty(shape[:-1] + (n,))
+    _call("dmoq_int8_gated_linear", index, rows.data_ptr(), x.dtype is _BF16, pitch, wg.data_ptr(), sg.data_ptr(), wu.data_ptr(),
+          su.data_ptr(), t, n, k, _ptr(scratch), out.data_ptr())
     return out
 
 
-def _ffn_forward(x: torch.Tensor, pitch: int, wg: torch.Tensor, wu: torch.Tensor, wd: torch.Tensor, save: bool):
+def _ffn_forward(x: torch.Tensor, t: int, pitch: int, wg: torch.Tensor, wu: torch.Tensor, wd: torch.Tensor, save: bool):
     """y, and the hidden values h; with ``save`` also what the gradients need of them."""
-    (t, hidden), inter, dev = x.shape, wg.shape[0], x.device
-    h = torch.empty((t, inter), dtype=x.dtype, device=dev)
-    saved = torch.empty((3, t, inter), dtype=torch.int16, device=dev) if save else None
-    y = torch.empty((t, hidden), dtype=x.dtype, device=dev)
-    _call("dmoq_gated_ffn", dev, x.data_ptr(), x.dtype == torch.bfloat16, pitch, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), t,
-          hidden, inter, h.data_ptr(), _ptr(saved), y.data_ptr())
+    hidden, inter = wd.shape
+    h = x.new_empty((t, inter))
+    saved = x.new_empty((3, t, inter), dtype=torch.int16) if save else None
+    y = x.new_empty((t, hidden))
+    _call("dmoq_gated_ffn", x.get_device(), x.data_ptr(), x.dtype is _BF16, pitch, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), t, hidden,
+          inter, h.data_ptr(), _ptr(saved), y.data_ptr())
     return y, h, saved
 
 
@@ -201,10 +214,11 @@ class _GatedFeedForward(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down):
-        rows, pitch = _rows(x, x.shape[-1])
-        inner = any(ctx.needs_input_grad[:3])
-        y, h, saved = _ffn_forward(rows, pitch, w_gate, w_up, w_down, inner)
-        ctx.save_for_backward(rows, w_gate, w_up, w_down, h if ctx.needs_input_grad[3] else None, saved)
+        rows, t, pitch = _rows(x, x.shape[-1])
+        need_x, need_g, need_u, need_d = ctx.needs_input_grad
+        y, h, saved = _ffn_forward(rows, t, pitch, w_gate, w_up, w_down, need_x or need_g or need_u)
+        ctx.save_for_backward(rows, w_gate, w_up, w_down, h if need_d else None, saved)
+        ctx.pitch = pitch
         return y
 
     @staticmethod
@@ -212,20 +226,17 @@ class _GatedFeedForward(torch.autograd.Function):
     def backward(ctx, dy):
         x, wg, wu, wd, h, saved = ctx.saved_tensors
         need_x, need_g, need_u, need_d = ctx.needs_input_grad
-        (t, hidden), inter, dev, dt = x.shape, wg.shape[0], x.device, x.dtype
-        dy, dy_pitch = _rows(dy, hidden)
-        x_pitch = x.stride(0) if t > 1 else hidden
-        inner = need_x or need_g or need_u
-        dgu = torch.empty((t, 2 * inter), dtype=dt, device=dev) if inner else None
-        dx = torch.empty((t, hidden), dtype=dt, device=dev) if need_x else None
+        hidden, inter = wd.shape
+        dy, t, dy_pitch = _rows(dy, hidden)
+        dgu = x.new_empty((t, 2 * inter)) if need_x or need_g or need_u else None
+        dx = x.new_empty((t, hidden)) if need_x else None
         # the two halves of one buffer: one product computes both
-        dw = torch.empty((int(need_g) + int(need_u), inter, hidden), dtype=dt, device=dev) if need_g or need_u else None
+        dw = x.new_empty((int(need_g) + int(need_u), inter, hidden)) if need_g or need_u else None
         dwg = dw[0] if need_g else None
         dwu = dw[-1] if need_u else None
-        dwd = torch.empty((hidden, inter), dtype=dt, device=dev) if need_d else None
-        _call("dmoq_gated_ffn_backward", dev, dy.data_ptr(), dy_pitch, x.data_ptr(), dt == torch.bfloat16, x_pitch, wg.data_ptr(),
-              wu.data_ptr(), wd.data_ptr(), t, hidden, inter, _ptr(h), _ptr(saved), _ptr(dgu), _ptr(dx), _ptr(dwg),
-              _ptr(dwu), _ptr(dwd))
+        dwd = x.new_empty((hidden, inter)) if need_d else None
+        _call("dmoq_gated_ffn_backward", x.get_device(), dy.data_ptr(), dy_pitch, x.data_ptr(), x.dtype is _BF16, ctx.pitch, wg.data_ptr(),
+              wu.data_ptr(), wd.data_ptr(), t, hidden, inter, _ptr(h), _ptr(saved), _ptr(dgu), _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd))
         return dx, dwg, dwu, dwd
 
 
@@ -235,23 +246,24 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     product's operand), so fp16 hidden values beyond 65504 become infinite.  Differentiable once in every argument; each gradient
     that is not needed is not computed."""
     _check_input(x)
-    hidden, dev, dt = x.shape[-1], x.device, x.dtype
-    for name, w in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
-        if w.dtype != dt:
-            raise TypeError(f"{name} must have x's type {dt}, got {w.dtype}")
-        _need(w.dim() == 2 and w.device == dev, f"{name} must be a matrix on {dev}")
-    inter = w_gate.shape[0]
-    _need(tuple(w_gate.shape) == (inter, hidden) and tuple(w_up.shape) == (inter, hidden) and tuple(w_down.shape) == (hidden, inter),
-          f"weights must be ({inter}, {hidden}) twice and ({hidden}, {inter}), got {tuple(w_gate.shape)}, {tuple(w_up.shape)}, "
-          f"{tuple(w_down.shape)}")
-    _need(hidden >= 8 and hidden % 8 == 0 and inter >= 8 and inter % 8 == 0,
-          f"hidden and intermediate sizes must be multiples of 8, got {hidden} and {inter}")
-    weights = [w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
-               for w in (w_gate, w_up, w_down)]
+    dt, index = x.dtype, x.get_device()
+    hidden = x.shape[-1]
+    if w_gate.dtype is not dt or w_up.dtype is not dt or w_down.dtype is not dt:
+        raise TypeError(f"the weights must have x's type {dt}, got {w_gate.dtype}, {w_up.dtype}, {w_down.dtype}")
+    inter = w_gate.shape[0] if w_gate.dim() else 0
+    if w_gate.shape != (inter, hidden) or w_up.shape != (inter, hidden) or w_down.shape != (hidden, inter):
+        raise ValueError(f"for x of {hidden} columns the weights must be (I, {hidden}) twice and ({hidden}, I), got {tuple(w_gate.shape)}, "
+                         f"{tuple(w_up.shape)}, {tuple(w_down.shape)}")
+    if hidden < 8 or inter < 8 or (hidden | inter) & 7:
+        raise ValueError(f"hidden and intermediate sizes must be multiples of 8, got {hidden} and {inter}")
+    for w in (w_gate, w_up, w_down):
+        if not w.is_cuda or w.get_device() != index:
+            raise ValueError(f"all weights must be on cuda:{index}")
+    w_gate, w_up, w_down = _packed(w_gate), _packed(w_up), _packed(w_down)
     rows = x if x.dim() == 2 else x.reshape(-1, hidden)
-    if torch.is_grad_enabled() and (x.requires_grad or any(w.requires_grad for w in weights)):
-        y = _GatedFeedForward.apply(rows, *weights)
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
+        y = _GatedFeedForward.apply(rows, w_gate, w_up, w_down)
     else:
-        rows, pitch = _rows(rows, hidden)
-        y = _ffn_forward(rows, pitch, *weights, save=False)[0]
+        rows, t, pitch = _rows(rows, hidden)
+        y = _ffn_forward(rows, t, pitch, w_gate, w_up, w_down, False)[0]
     return y if x.dim() == 2 else y.reshape(x.shape)

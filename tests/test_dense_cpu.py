@@ -37,13 +37,21 @@ def test_int8_products_refuse():
         assert lib.dmoq_int8_gated_gemm(*(good[:i] + [None] + good[i + 1:]), None) == EINVAL
     assert lib.dmoq_int8_gated_gemm(*(good[:9] + [1 << 20] + good[10:]), None) == ESIZE
     # with the quantiser in front nothing is launched before everything is known to be right
-    good = [P, 1, 128, P, P, None, 4, 33, 128, P, P, P]
-    for i, v in ((0, None), (2, 127), (3, None), (4, None), (7, 0), (8, 100), (9, None), (10, None), (11, None), (3, ODD)):
+    good = [P, 1, 128, P, P, None, 40, 33, 128, P, P]
+    for i, v in ((0, None), (2, 127), (3, None), (4, None), (7, 0), (8, 100), (9, None), (10, None), (3, ODD), (9, ODD)):
         assert lib.dmoq_int8_linear(*(good[:i] + [v] + good[i + 1:]), None) == EINVAL, (i, v)
-    assert lib.dmoq_int8_linear(*(good[:2] + [131072, P, P, None, 4, 33, 131072] + good[9:]), None) == ESIZE
-    good = [P, 1, 128, P, P, P, P, 4, 33, 128, P, P, P]
-    for i in (0, 3, 4, 5, 6, 10, 11, 12):
+    assert lib.dmoq_int8_linear(*(good[:2] + [131072, P, P, None, 40, 33, 131072] + good[9:]), None) == ESIZE
+    good = [P, 1, 128, P, P, P, P, 40, 33, 128, P, P]
+    for i in (0, 3, 4, 5, 6, 10, 11):
         assert lib.dmoq_int8_gated_linear(*(good[:i] + [None] + good[i + 1:]), None) == EINVAL, i
+
+
+def test_int8_scratch_size():
+    f = _lib.load().dmoq_int8_scratch_bytes
+    assert f(40, 128) == 40 * 128 + 40 * 4 and f(1000, 131056) == 1000 * 131056 + 4000
+    assert f(0, 128) == 0 and f(1, 128) == 0 and f(16, 512) == 0        # no tokens; few: the product makes the codes itself
+    assert f(16, 8192) == 16 * 8192 + 64 and f(1, 65536) == 65536 + 4   # few, but too long for that
+    assert f(4, 100) == 0 and f(-1, 128) == 0                           # refused by the calls themselves
 
 
 def test_gated_ffn_refuses():
