@@ -21,7 +21,6 @@ constexpr __host__ __device__ int outputs_of(int epi) { return epi == EPI_SILU_S
 
 struct Maps {
   CUtensorMap a[2], b[2];
-  CUtensorMap out[4];       // only where stores go through TMA
 };
 
 // silu(g) and u silu'(g) are kept to the upper 24 bits of their 32-bit floats, whatever the tensors' 16-bit type: planes 1 and 2

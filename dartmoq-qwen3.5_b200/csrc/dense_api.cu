@@ -1,4 +1,6 @@
 // C entry points of the dense operators: argument checks, tensor maps, choice of the kernel.
+#include <algorithm>
+
 #include "dense.cuh"
 
 int dmoq_token_quant_launch(const void* x, int bf16, int T, int K, long long pitch, int8_t* codes, float* scales, cudaStream_t s);
@@ -7,6 +9,7 @@ namespace dense {
 
 int tile_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, const Args& a, int splits, cudaStream_t s);
 int pair_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, const Args& a, cudaStream_t s);
+int pair_group(const Maps* maps, const Args* p, const bool* a_mn, int n_long, cudaStream_t s);
 
 int few_product(int kind, int epi, const void* x, long long x_pitch, const void* w0, const void* w1, const Args& a, cudaStream_t s);
 bool few_can_fuse(int T, int K);
@@ -41,19 +44,17 @@ struct Matrix {
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 bool tma_ok(const Matrix& m, int es) { return aligned16(m.p) && (m.pitch * es) % 16 == 0 && m.pitch >= m.cols; }
 
-// Copied in boxes of box_bytes (128 or 64) x box_rows rows with the swizzle of that width; what lies past the matrix reads as
-// zero and is not written.
-int make_map(CUtensorMap* map, const Matrix& m, int es, int box_rows, int box_bytes = 128) {
+// Copied in boxes of 128 bytes x box_rows rows with the 128-byte swizzle; what lies past the matrix reads as zero.
+int make_map(CUtensorMap* map, const Matrix& m, int es, int box_rows) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (fn == nullptr) return DMOQ_EDEVICE;
   const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows};
   const cuuint64_t strides[1] = {(cuuint64_t)m.pitch * es};
-  const cuuint32_t box[2] = {(cuuint32_t)(box_bytes / es), (cuuint32_t)box_rows};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / es), (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
   auto encode = [&] {
     return fn(map, es == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(m.p), dims,
-              strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-              CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
   CUresult rc = encode();
@@ -74,40 +75,77 @@ struct Product {
   Args args = {};
 };
 
-int run(const Product& p, cudaStream_t s) {
+// The tensor maps of a product: boxes of 128 rows of A and `b_box` rows of B (K-major), or of a step of K (MN-major).
+int make_maps(Maps& maps, const Product& p, int b_box) {
   const int es = p.kind == KIND_I8 ? 1 : 2, bk = 128 / es;
-  const bool dual = is_dual(p.epi);
-  const long long pair_tiles = (long long)dmoq_ceil_div(p.args.M, 256) * dmoq_ceil_div(p.args.N, dual ? 128 : 256);
-  const bool pair = pair_tiles * 4 >= dmoq_sm_count();
-  const int cols = dual ? 64 : 128;
-  const long long tiles = (long long)dmoq_ceil_div(p.args.M, 128) * dmoq_ceil_div(p.args.N, cols);
-  const int steps = dmoq_ceil_div(p.args.K, bk) * p.args.segs;
-  int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= dmoq_sm_count() && steps >= splits * 8) splits *= 2;
-  Maps maps;
   const int n_a = p.args.segs, n_b = is_dual(p.epi) ? 2 : p.args.segs;
-  for (int i = 0; i < 2; ++i) {
-    const Matrix& a = p.a[i < n_a ? i : 0];
-    const Matrix& b = p.b[i < n_b ? i : 0];
-    if (!tma_ok(a, es) || !tma_ok(b, es)) return DMOQ_EINVAL;
-    int rc = make_map(&maps.a[i], a, es, p.a_mn ? bk : 128);
-    if (rc == DMOQ_OK) rc = make_map(&maps.b[i], b, es, p.b_mn ? bk : pair ? 128 : cols);
+  for (int i = 0; i < n_a + n_b; ++i) {
+    const bool is_a = i < n_a;
+    const Matrix& m = is_a ? p.a[i] : p.b[i - n_a];
+    if (!tma_ok(m, es)) return DMOQ_EINVAL;
+    const int rc = make_map(is_a ? &maps.a[i] : &maps.b[i - n_a], m, es, is_a ? (p.a_mn ? bk : 128) : (p.b_mn ? bk : b_box));
     if (rc != DMOQ_OK) return rc;
   }
-  if (pair) {
-    Args args = p.args;
-    args.vec = 1;
-    for (int e = 0; e < outputs_of(p.epi); ++e) {
-      const Matrix o = {args.out[e], args.M, args.N, args.ld_out};
-      args.vec = args.vec && tma_ok(o, 2);
-    }
-    for (int e = 0; args.vec && e < outputs_of(p.epi); ++e) {
-      const int rc = make_map(&maps.out[e], {args.out[e], args.M, args.N, args.ld_out}, 2, 32, 64);
+  return DMOQ_OK;
+}
+// The pair kernel's arguments: outputs leave as 16-byte stores of eight columns where their memory allows.
+Args pair_args(const Product& p) {
+  Args args = p.args;
+  args.vec = args.N % 8 == 0;
+  for (int e = 0; e < outputs_of(p.epi); ++e) args.vec = args.vec && aligned16(args.out[e]) && args.ld_out % 8 == 0;
+  return args;
+}
+long long pair_tiles(const Product& p) {
+  return (long long)dmoq_ceil_div(p.args.M, 256) * dmoq_ceil_div(p.args.N, is_dual(p.epi) ? 128 : 256);
+}
+long long steps_of(const Product& p) { return (long long)dmoq_ceil_div(p.args.K, p.kind == KIND_I8 ? 128 : 64) * p.args.segs; }
+
+int run(const Product& p, cudaStream_t s) {
+  Maps maps;
+  if (pair_tiles(p) * 4 >= dmoq_sm_count()) {
+    const int rc = make_maps(maps, p, 128);
+    return rc != DMOQ_OK ? rc : pair_product(p.kind, p.a_mn, p.b_mn, p.epi, maps, pair_args(p), s);
+  }
+  const int cols = is_dual(p.epi) ? 64 : 128;
+  const long long tiles = (long long)dmoq_ceil_div(p.args.M, 128) * dmoq_ceil_div(p.args.N, cols), steps = steps_of(p);
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= dmoq_sm_count() && steps >= splits * 8) splits *= 2;
+  const int rc = make_maps(maps, p, cols);
+  return rc != DMOQ_OK ? rc : tile_product(p.kind, p.a_mn, p.b_mn, p.epi, maps, p.args, splits, s);
+}
+
+// Three independent products (MN-major B, plain outputs).  In one launch their tiles fill the SMs together, as long as no single
+// tile is longer than the share of the work that a pair of blocks gets; then that product is better split along K by itself.
+int run_three(const Product (&p)[3], cudaStream_t s) {
+  const int pairs = dmoq_sm_count() / 2;
+  long long total = 0, longest = 0, shortest = 1LL << 60;
+  for (const Product& q : p) {
+    total += pair_tiles(q) * steps_of(q);
+    longest = std::max(longest, steps_of(q));
+    shortest = std::min(shortest, steps_of(q));
+  }
+  if (longest * pairs * 4 > total * 5) {
+    for (const Product& q : p) {
+      const int rc = run(q, s);
       if (rc != DMOQ_OK) return rc;
     }
-    return pair_product(p.kind, p.a_mn, p.b_mn, p.epi, maps, args, s);
+    return DMOQ_OK;
   }
-  return tile_product(p.kind, p.a_mn, p.b_mn, p.epi, maps, p.args, splits, s);
+  Maps maps[3];
+  Args args[3];
+  bool a_mn[3];
+  int n = 0, n_long = 0;
+  for (int side = 0; side < 2; ++side) {      // the products with the longer tiles first
+    for (const Product& q : p) {
+      if ((2 * steps_of(q) >= longest + shortest) != (side == 0)) continue;
+      const int rc = make_maps(maps[n], q, 128);
+      if (rc != DMOQ_OK) return rc;
+      args[n] = pair_args(q);
+      a_mn[n++] = q.a_mn;
+    }
+    if (side == 0) n_long = n;
+  }
+  return pair_group(maps, args, a_mn, n_long, s);
 }
 
 // four-element accesses to a 16-bit matrix
@@ -285,35 +323,48 @@ extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const v
     p.args.ld_out = 2 * (long long)I;
     if ((rc = run(p, s)) != DMOQ_OK) return rc;
   }
-  if (dx) {      // dx = dg Wg + du Wu: one sum over two K segments
-    Product p;
-    p.b_mn = true;
-    p.a[0] = {dg, T, I, 2 * (long long)I};
-    p.a[1] = {dg + I, T, I, 2 * (long long)I};
-    p.b[0] = {w_gate, I, H, H};
-    p.b[1] = {w_up, I, H, H};
-    p.args.M = T, p.args.N = H, p.args.K = I, p.args.segs = 2, p.args.bf16 = is_bf16, p.args.vec = 1;
-    p.args.out[0] = static_cast<uint16_t*>(dx);
-    p.args.ld_out = H;
-    if ((rc = run(p, s)) != DMOQ_OK) return rc;
+  Product px, pg, pd;   // dx, dw_gate and dw_up, dw_down
+  auto output = [&](Product& p, int M, int N, int K, int segs, void* out) {
+    p.args.M = M, p.args.N = N, p.args.K = K, p.args.segs = segs, p.args.bf16 = is_bf16, p.args.vec = 1;
+    p.args.out[0] = static_cast<uint16_t*>(out);
+    p.args.ld_out = N;
+  };
+  const long long dg_pitch = 2 * (long long)I;
+  if (dx) {             // dg Wg + du Wu: one sum over two K segments
+    px.b_mn = true;
+    px.a[0] = {dg, T, I, dg_pitch};
+    px.a[1] = {dg + I, T, I, dg_pitch};
+    px.b[0] = {w_gate, I, H, H};
+    px.b[1] = {w_up, I, H, H};
+    output(px, T, H, I, 2, dx);
   }
-  auto weight_grad = [&](const Matrix& a, const Matrix& b, void* out) {   // a^T b, both along the tokens
-    Product p;
+  auto weight_grad = [&](Product& p, const Matrix& a, const Matrix& b, void* out) {   // a^T b, both along the tokens
     p.a_mn = p.b_mn = true;
     p.a[0] = a;
     p.b[0] = b;
-    p.args.M = (int)a.cols, p.args.N = (int)b.cols, p.args.K = T, p.args.segs = 1, p.args.bf16 = is_bf16, p.args.vec = 1;
-    p.args.out[0] = static_cast<uint16_t*>(out);
-    p.args.ld_out = b.cols;
-    return run(p, s);
+    output(p, (int)a.cols, (int)b.cols, T, 1, out);
   };
   const Matrix xm = {x, T, H, x_pitch};
-  if (dw_gate && dw_up && static_cast<char*>(dw_up) == static_cast<char*>(dw_gate) + w_bytes) {   // one product for both halves
-    if ((rc = weight_grad({dg, T, 2 * (long long)I, 2 * (long long)I}, xm, dw_gate)) != DMOQ_OK) return rc;
-  } else {
-    if (dw_gate && (rc = weight_grad({dg, T, I, 2 * (long long)I}, xm, dw_gate)) != DMOQ_OK) return rc;
-    if (dw_up && (rc = weight_grad({dg + I, T, I, 2 * (long long)I}, xm, dw_up)) != DMOQ_OK) return rc;
+  const bool joined = dw_gate && dw_up && static_cast<char*>(dw_up) == static_cast<char*>(dw_gate) + w_bytes;
+  if (joined) weight_grad(pg, {dg, T, dg_pitch, dg_pitch}, xm, dw_gate);   // one product for both halves
+  if (dw_down) weight_grad(pd, {dy, T, H, dy_pitch}, {h, T, I, I}, dw_down);
+  if (dx && joined && dw_down) {
+    const Product all[3] = {px, pg, pd};
+    return run_three(all, s);
   }
-  if (dw_down) rc = weight_grad({dy, T, H, dy_pitch}, {h, T, I, I}, dw_down);
-  return rc;
+  if (dx && (rc = run(px, s)) != DMOQ_OK) return rc;
+  if (joined) {
+    if ((rc = run(pg, s)) != DMOQ_OK) return rc;
+  } else {
+    Product p;
+    if (dw_gate) {
+      weight_grad(p, {dg, T, I, dg_pitch}, xm, dw_gate);
+      if ((rc = run(p, s)) != DMOQ_OK) return rc;
+    }
+    if (dw_up) {
+      weight_grad(p, {dg + I, T, I, dg_pitch}, xm, dw_up);
+      if ((rc = run(p, s)) != DMOQ_OK) return rc;
+    }
+  }
+  return dw_down ? run(pd, s) : DMOQ_OK;
 }

@@ -4,10 +4,13 @@
 // Each block of a pair holds 128 of the tile's rows: it loads its own 128 rows of A and one half of the tile's 256 columns of B
 // (when dual: the first block the gate's 128 columns, the second the up projection's), the leader's MMA thread multiplies both
 // halves, and each block finds its 128 rows x 256 columns of sums in its own TMEM.  Two such accumulators fill TMEM, so the
-// epilogue of a tile runs beside the products of the next one.
-//   warp 0      loads the operands by TMA (five steps of 128 bytes of K ahead)
+// epilogue of a tile runs beside the products of the next one.  One launch may hold several products (GROUP): the gradients of a
+// block, whose tiles differ in length, share the SMs.
+//   warp 0      loads the operands by TMA (six steps of 128 bytes of K ahead)
 //   warp 1      issues tcgen05.mma (leader only)
-//   warps 4-11  take the sums out of TMEM, finish them, and write 32 x 32 blocks out through shared memory and TMA stores
+//   warps 4-11  take the sums out of TMEM, finish them, and write 32 x 32 blocks out through shared memory (plain
+//               stores of 64-byte rows: a TMA store costs each warp a proxy fence of about 500 cycles a block, which made the
+//               epilogue the longer half of tiles with a short K)
 #include "dense.cuh"
 
 #include <algorithm>
@@ -17,11 +20,11 @@ __device__ int g_dmoq_dense_pair_status = 0;
 namespace dense {
 namespace {
 
-constexpr int kStages = 5;
+constexpr int kStages = 6;
 constexpr int kStageBytes = 2 * 128 * 128;
 constexpr int kEpiWarps = 8;
 constexpr int kUnitBytes = 32 * 64;                       // 32 rows of 32 16-bit outputs on their way out
-constexpr int kUnits = 4;                                 // per epilogue warp
+constexpr int kUnits = 2;                                 // per epilogue warp
 constexpr int kUnitBase = kStages * kStageBytes;
 constexpr int kBarBase = kUnitBase + kEpiWarps * kUnits * kUnitBytes;
 constexpr int kSmem = kBarBase + 256 + 1024;
@@ -34,16 +37,6 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(leader_bar)
       : "memory");
 }
-__device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int x, int y) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x),
-               "r"(y), "r"(src)
-               : "memory");
-  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-}
-template <int N>
-__device__ __forceinline__ void tma_store_wait_read() {
-  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
-}
 // completes on the barrier at this address in both blocks of the pair
 __device__ __forceinline__ void commit_pair(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
@@ -51,9 +44,21 @@ __device__ __forceinline__ void commit_pair(uint32_t bar) {
                : "memory");
 }
 
-template <int KIND, bool AMN, bool BMN, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    dense_pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args a) {
+// NP products of one launch.  Their tiles come in two lengths (steps of K): first the long ones go round the pairs, then the
+// pairs that got one fewer take `fill` short tiles each, which is about as long, and the rest of the short ones goes round.
+template <int NP>
+struct Work {
+  Maps maps[NP];
+  Args p[NP];
+  int a_mn[NP];
+  int tiles[NP];             // 256-row tiles of each product
+  int n_long;                // products 0 .. n_long - 1 have the long tiles
+  int long_tiles, fill;
+};
+
+// AMN is that of a single product; a group's products say it themselves.
+template <int KIND, bool AMN, bool BMN, int EPI, int NP>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) dense_pair_kernel(const __grid_constant__ Work<NP> work) {
   constexpr bool kDual = is_dual(EPI);
   constexpr int kCols = kDual ? 128 : 256;                 // output columns of a tile
   constexpr int kBK = KIND == KIND_I8 ? 128 : 64;
@@ -72,14 +77,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const uint32_t rank = cluster_rank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int tiles_m = (a.M + 255) / 256, tiles_n = (a.N + kCols - 1) / kCols;
-  const int tiles = tiles_m * tiles_n;
-  const int seg_steps = (a.K + kBK - 1) / kBK, steps = seg_steps * a.segs;
-  auto tile_at = [&](int t, int& m0, int& n0) {            // columns of up to kGroupM tile rows, one tile column after the other
+  struct Tile {
+    int q, m0, n0, seg_steps, steps;                       // product, first row of this block, first column, steps of K
+  };
+  auto next_tile = [&](int i, Tile& o) {                   // the pair's i-th tile; false after the last one
+    int t = pair + i * pairs, q = 0;
+    if (NP > 1) {
+      const int ahead = work.long_tiles % pairs;           // pairs that have one long tile more than the others
+      const int mine = work.long_tiles / pairs + (pair < ahead ? 1 : 0);
+      int last = work.n_long;
+      if (i >= mine) {
+        const int j = i - mine, fill = pair < ahead ? 0 : work.fill, others = pairs - ahead;
+        t = j < fill ? j * others + pair - ahead : work.fill * others + (j - fill) * pairs + pair;
+        q = work.n_long;
+        last = NP;
+      }
+      while (q < last && t >= work.tiles[q]) t -= work.tiles[q++];
+      if (q >= last) return false;
+    } else if (t >= work.tiles[0]) {
+      return false;
+    }
+    const Args& a = work.p[q];
+    const int tiles_n = (a.N + kCols - 1) / kCols, tiles_m = (a.M + 255) / 256;
+    // columns of up to kGroupM tile rows, one tile column after the other
     const int group = t / (kGroupM * tiles_n), first = group * kGroupM;
     const int height = min(kGroupM, tiles_m - first), local = t - group * kGroupM * tiles_n;
-    m0 = (first + local % height) * 256 + (int)rank * 128;
-    n0 = local / height * kCols;
+    o.q = q;
+    o.m0 = (first + local % height) * 256 + (int)rank * 128;
+    o.n0 = local / height * kCols;
+    o.seg_steps = (a.K + kBK - 1) / kBK;
+    o.steps = o.seg_steps * a.segs;
+    return true;
   };
 
   if (tid == 0) {
@@ -110,10 +138,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       uint32_t done = 0;
       bool ok = true;
-      for (int t = pair; t < tiles && ok; t += pairs) {
-        int m0, n0;
-        tile_at(t, m0, n0);
-        for (int it = 0; it < steps; ++it, ++done) {
+      Tile w;
+      for (int i = 0; ok && next_tile(i, w); ++i) {
+        const Maps& maps = work.maps[w.q];
+        const bool a_mn = NP > 1 ? work.a_mn[w.q] != 0 : AMN;
+        const int m0 = w.m0, n0 = w.n0, seg_steps = w.seg_steps;
+        for (int it = 0; it < w.steps; ++it, ++done) {
           const uint32_t s = done % kStages;
           if (done >= kStages && !mbar_wait(bar_empty(s), (done / kStages - 1) & 1, abort_flag, status)) {
             ok = false;
@@ -122,7 +152,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const uint32_t full = map_to_rank(bar_full(s), 0);
           if (rank == 0) mbar_arrive_expect_tx(bar_full(s), 2 * kStageBytes);
           const int seg = it >= seg_steps ? 1 : 0, k = (it - seg * seg_steps) * kBK;
-          if (AMN) {
+          if (a_mn) {
             tma_load_pair(stage_a(s), &maps.a[seg], m0, k, full);
             tma_load_pair(stage_a(s) + 8192, &maps.a[seg], m0 + 64, k, full);
           } else {
@@ -145,27 +175,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
       constexpr uint32_t shape = (32u << 17) | (16u << 24);
-      const uint32_t type = a.bf16 ? 1u : 0u;
-      const uint32_t idesc = KIND == KIND_I8 ? (2u << 4) | (1u << 7) | (1u << 10) | shape
-                                             : (1u << 4) | (type << 7) | (type << 10) | (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u) | shape;
-      constexpr uint32_t step_a = AMN ? 128 : 2, step_b = BMN ? 128 : 2;
-      uint32_t done = 0, i = 0;
+      const uint32_t type = work.p[0].bf16 ? 1u : 0u;
+      constexpr uint32_t step_b = BMN ? 128 : 2;
+      uint32_t done = 0, ready = 0;
       bool ok = true;
-      for (int t = pair; t < tiles && ok; t += pairs, ++i) {
+      Tile w;
+      for (int i = 0; ok && next_tile(i, w); ++i) {
+        const bool a_mn = NP > 1 ? work.a_mn[w.q] != 0 : AMN;
+        const uint32_t step_a = a_mn ? 128 : 2, lead_a = a_mn ? 8192 : 16;
+        const uint32_t idesc = KIND == KIND_I8 ? (2u << 4) | (1u << 7) | (1u << 10) | shape
+                                               : (1u << 4) | (type << 7) | (type << 10) | (a_mn ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u) | shape;
         const uint32_t b = i & 1, d = tmem + b * 256;
         if (i >= 2 && !mbar_wait(bar_acc_empty(b), (i / 2 - 1) & 1, abort_flag, status)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        for (int it = 0; it < steps; ++it, ++done) {
+        for (int it = 0; it < w.steps; ++it, ++done) {
           const uint32_t s = done % kStages;
-          if (!mbar_wait(bar_full(s), (done / kStages) & 1, abort_flag, status)) {
+          if (!ready && !mbar_wait(bar_full(s), (done / kStages) & 1, abort_flag, status)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint64_t da = operand_desc(stage_a(s), AMN ? 8192 : 16), db = operand_desc(stage_b(s), BMN ? 8192 : 16);
+          // look at the next step now and use the answer after this one's products: the barrier's latency (about 110 cycles of
+          // the 512 that a step takes) would otherwise stand between them
+          ready = mbar_peek(bar_full((done + 1) % kStages), ((done + 1) / kStages) & 1);
+          const uint64_t da = operand_desc(stage_a(s), lead_a), db = operand_desc(stage_b(s), BMN ? 8192 : 16);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t acc = (it > 0 || k > 0) ? 1u : 0u;
@@ -191,10 +227,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp >= 4) {
     const int e = warp - 4, quarter = e & 3, side = e >> 2;
     const uint32_t units = sb + kUnitBase + e * (kUnits * kUnitBytes);
-    uint32_t i = 0, n_out = 0;
-    for (int t = pair; t < tiles; t += pairs, ++i) {
-      int m0, n0;
-      tile_at(t, m0, n0);
+    uint32_t n_out = 0;
+    Tile at_tile;
+    for (int i = 0; next_tile(i, at_tile); ++i) {
+      const Args& a = work.p[at_tile.q];
+      const int m0 = at_tile.m0, n0 = at_tile.n0;
       const uint32_t b = i & 1;
       const int row0 = m0 + quarter * 32;
       const long long row = row0 + lane;
@@ -278,29 +315,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int p = 0; p < outputs_of(EPI); ++p, ++n_out) {
           const uint32_t unit = units + (n_out % kUnits) * kUnitBytes;
-          if (lane == 0) tma_store_wait_read<kUnits - 1>();   // the store that used this unit four stores ago has read it
-          __syncwarp();
           const uint32_t line = unit + lane * 64, swz = (lane >> 1) & 3;
 #pragma unroll
           for (int j = 0; j < 4; ++j) st_shared_v4(line + ((j ^ swz) << 4), o[p][4 * j], o[p][4 * j + 1], o[p][4 * j + 2], o[p][4 * j + 3]);
+          __syncwarp();                                    // also: what this unit held two outputs ago has been read
           if (a.vec) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) tma_store(&maps.out[p], unit, col0, row0);
+            const int q = lane & 3, col = col0 + 8 * q;    // 16 bytes a thread: eight rows of 64 bytes an instruction
+            uint16_t* dst = a.out[p] + (long long)(row0 + (lane >> 2)) * a.ld_out + col;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int at = 8 * r + (lane >> 2);
+              const uint4 val = ld_shared_v4(unit + at * 64 + ((q ^ ((at >> 1) & 3)) << 4));
+              if (row0 + at < a.M && col < a.N) *reinterpret_cast<uint4*>(dst + 8 * r * a.ld_out) = val;
+            }
           } else {                                         // rows that are not 16-byte aligned: 64-byte runs of a row at a time
-            __syncwarp();
             for (int r = 0; r < 32 && row0 + r < a.M; ++r) {
               const uint32_t at = unit + r * 64 + ((((uint32_t)lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2;
               uint16_t val;
               asm volatile("ld.shared.u16 %0, [%1];" : "=h"(val) : "r"(at) : "memory");
               if (col0 + lane < a.N) a.out[p][(row0 + r) * a.ld_out + col0 + lane] = val;
             }
-            __syncwarp();
           }
         }
       }
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
@@ -311,22 +349,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int KIND, bool AMN, bool BMN, int EPI>
-int launch(const Maps& maps, const Args& a, cudaStream_t s) {
+template <int KIND, bool AMN, bool BMN, int EPI, int NP>
+int launch(Work<NP>& work, cudaStream_t s) {
   static DmoqOncePerDevice once;
   bool* configured = once.slot();
   if (configured == nullptr) return DMOQ_EDEVICE;
-  auto* kernel = dense_pair_kernel<KIND, AMN, BMN, EPI>;
+  auto* kernel = dense_pair_kernel<KIND, AMN, BMN, EPI, NP>;
   if (!*configured) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return DMOQ_ELAUNCH;
     *configured = true;
   }
   constexpr int kCols = is_dual(EPI) ? 128 : 256;
-  const long long tiles = (long long)dmoq_ceil_div(a.M, 256) * dmoq_ceil_div(a.N, kCols);
-  if (tiles > 0x3fffffffLL) return DMOQ_ESIZE;
+  long long tiles = 0;
+  for (int q = 0; q < NP; ++q) {
+    const long long t = (long long)dmoq_ceil_div(work.p[q].M, 256) * dmoq_ceil_div(work.p[q].N, kCols);
+    tiles += t;
+    if (tiles > 0x3fffffffLL) return DMOQ_ESIZE;
+    work.tiles[q] = (int)t;
+  }
   const int pairs = (int)std::min<long long>(tiles, dmoq_sm_count() / 2);
-  kernel<<<2 * pairs, kThreads, kSmem, s>>>(maps, a);
+  if (NP > 1) {
+    auto steps = [&](int q) { return (long long)dmoq_ceil_div(work.p[q].K, 64) * work.p[q].segs; };
+    work.long_tiles = 0;
+    for (int q = 0; q < work.n_long; ++q) work.long_tiles += work.tiles[q];
+    const long long shorts = tiles - work.long_tiles;
+    const int ahead = work.long_tiles % pairs;
+    work.fill = ahead == 0 || shorts == 0 ? 0 : (int)std::min<long long>(steps(0) / steps(NP - 1), shorts / (pairs - ahead));
+  }
+  kernel<<<2 * pairs, kThreads, kSmem, s>>>(work);
   return dmoq_launch_status();
+}
+
+template <int KIND, bool AMN, bool BMN, int EPI>
+int launch1(const Maps& maps, const Args& a, cudaStream_t s) {
+  Work<1> w{};
+  w.maps[0] = maps;
+  w.p[0] = a;
+  return launch<KIND, AMN, BMN, EPI, 1>(w, s);
 }
 
 }  // namespace
@@ -334,16 +393,28 @@ int launch(const Maps& maps, const Args& a, cudaStream_t s) {
 int pair_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, const Args& a, cudaStream_t s) {
   const int key = kind * 1000 + a_mn * 200 + b_mn * 100 + epi;
   switch (key) {
-    case EPI_OUT: return launch<KIND_16, false, false, EPI_OUT>(maps, a, s);
-    case EPI_SILU: return launch<KIND_16, false, false, EPI_SILU>(maps, a, s);
-    case EPI_SILU_SAVE: return launch<KIND_16, false, false, EPI_SILU_SAVE>(maps, a, s);
-    case 100 + EPI_OUT: return launch<KIND_16, false, true, EPI_OUT>(maps, a, s);
-    case 100 + EPI_GRAD: return launch<KIND_16, false, true, EPI_GRAD>(maps, a, s);
-    case 300 + EPI_OUT: return launch<KIND_16, true, true, EPI_OUT>(maps, a, s);
-    case 1000 + EPI_SCALE: return launch<KIND_I8, false, false, EPI_SCALE>(maps, a, s);
-    case 1000 + EPI_SILU: return launch<KIND_I8, false, false, EPI_SILU>(maps, a, s);
+    case EPI_OUT: return launch1<KIND_16, false, false, EPI_OUT>(maps, a, s);
+    case EPI_SILU: return launch1<KIND_16, false, false, EPI_SILU>(maps, a, s);
+    case EPI_SILU_SAVE: return launch1<KIND_16, false, false, EPI_SILU_SAVE>(maps, a, s);
+    case 100 + EPI_OUT: return launch1<KIND_16, false, true, EPI_OUT>(maps, a, s);
+    case 100 + EPI_GRAD: return launch1<KIND_16, false, true, EPI_GRAD>(maps, a, s);
+    case 300 + EPI_OUT: return launch1<KIND_16, true, true, EPI_OUT>(maps, a, s);
+    case 1000 + EPI_SCALE: return launch1<KIND_I8, false, false, EPI_SCALE>(maps, a, s);
+    case 1000 + EPI_SILU: return launch1<KIND_I8, false, false, EPI_SILU>(maps, a, s);
     default: return DMOQ_EINVAL;
   }
+}
+
+// Three 16-bit products with MN-major B in one launch, ordered so that the first n_long have the longer tiles.
+int pair_group(const Maps* maps, const Args* p, const bool* a_mn, int n_long, cudaStream_t s) {
+  Work<3> w{};
+  for (int q = 0; q < 3; ++q) {
+    w.maps[q] = maps[q];
+    w.p[q] = p[q];
+    w.a_mn[q] = a_mn[q];
+  }
+  w.n_long = n_long;
+  return launch<KIND_16, false, true, EPI_OUT, 3>(w, s);
 }
 
 }  // namespace dense

@@ -100,10 +100,12 @@ __global__ void __launch_bounds__(256, 1) dense_tile_kernel(const __grid_constan
                                              : (1u << 4) | (type << 7) | (type << 10) | (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u) | shape;
       // 32 bytes of K an instruction: 32 bytes along a K-major row, sixteen 128-byte rows of an MN-major tile
       constexpr uint32_t step_a = AMN ? 128 : 2, step_b = BMN ? 128 : 2;
+      uint32_t ready = 0;
       for (int done = 0; done < it1 - it0; ++done) {
         const uint32_t s = done % kStages;
-        if (!mbar_wait(bar_full(s), (done / kStages) & 1, abort_flag, &g_dmoq_dense_status)) break;
+        if (!ready && !mbar_wait(bar_full(s), (done / kStages) & 1, abort_flag, &g_dmoq_dense_status)) break;
         tc_fence_after();
+        ready = mbar_peek(bar_full((done + 1) % kStages), ((done + 1) / kStages) & 1);   // used after this step's products
         const uint64_t da = operand_desc(stage_a(s), AMN ? 8192 : 16), db = operand_desc(stage_b(s), BMN ? 8192 : 16);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
