@@ -70,4 +70,69 @@ __device__ __forceinline__ void finish(const Args& a, long long row, int col, ui
   }
 }
 
+// Rows row_lo .. row_hi - 1 of a tile whose sums lie in shared memory (rows `pitch` bytes apart, kCols 32-bit columns and, when
+// dual, kCols more of the second product), split over the cluster's blocks: joined, finished and written, four columns a
+// thread.  Neighbouring threads read neighbouring columns: a warp's read of another block's memory is whole lines (a row a
+// lane made joining eight blocks slower than leaving the product unsplit).
+template <int KIND, int EPI, int kCols>
+__device__ __forceinline__ void finish_rows(const Args& a, uint32_t sums, uint32_t pitch, int row_lo, int row_hi, int m0, int n0,
+                                            uint32_t blocks, int tid) {
+  constexpr int kQuads = kCols / 4;
+  constexpr bool kDual = is_dual(EPI);
+#pragma unroll 2
+  for (int i = row_lo * kQuads + tid; i < row_hi * kQuads; i += 256) {
+    const int r = i / kQuads, c = i % kQuads * 4;
+    const long long row = m0 + r;
+    const int col = n0 + c;
+    if (row >= a.M || col >= a.N) continue;
+    uint32_t v[4], u[4] = {0u, 0u, 0u, 0u};
+    const uint32_t at = sums + r * pitch + c * 4;
+    sum_over_cluster<KIND == KIND_I8>(at, blocks, v);
+    if (kDual) sum_over_cluster<KIND == KIND_I8>(at + kCols * 4, blocks, u);
+    const int n = min(4, a.N - col);
+    const float sa = KIND == KIND_I8 ? a.a_scale[row] : 1.f;
+    const long long at_out = row * a.ld_out + col;
+    float o[3][4];
+    if (EPI == EPI_GRAD) {
+      const long long at_in = row * a.ld_in + col;   // the planes' rows are whole groups of four (sizes are multiples of 8)
+      uint2 pl[3];
+#pragma unroll
+      for (int e = 0; e < 3; ++e) pl[e] = *reinterpret_cast<const uint2*>(a.in[e] + at_in);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        auto half = [&](const uint2 w) { return ((j < 2 ? w.x : w.y) >> (16 * (j & 1))) & 0xffffu; };
+        const float dh = __uint_as_float(v[j]);
+        o[0][j] = dh * saved_slope(half(pl[1]), half(pl[2]));
+        o[1][j] = dh * saved_silu(half(pl[0]), half(pl[2]));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float e[3] = {0.f, 0.f, 0.f};
+        if (j < n) finish<KIND, EPI>(a, row, col + j, v[j], u[j], sa, e);
+        o[0][j] = e[0], o[1][j] = e[1], o[2][j] = e[2];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < outputs_of(EPI); ++e) {
+      uint32_t lo, hi;
+      if (EPI == EPI_SILU_SAVE && e > 0) {
+        auto word = [&](int j) {
+          return e == 3 ? saved_low(o[1][j], o[2][j]) : __float_as_uint(o[e < 3 ? e : 0][j]) >> 16;
+        };
+        lo = word(0) | (word(1) << 16), hi = word(2) | (word(3) << 16);
+      } else {
+        lo = pack16(o[e < 3 ? e : 0][0], o[e < 3 ? e : 0][1], a.bf16), hi = pack16(o[e < 3 ? e : 0][2], o[e < 3 ? e : 0][3], a.bf16);
+      }
+      uint16_t* dst = a.out[e] + at_out;
+      if (a.vec) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+      } else {
+        const uint32_t h[4] = {lo & 0xffffu, lo >> 16, hi & 0xffffu, hi >> 16};
+        for (int j = 0; j < n; ++j) dst[j] = (uint16_t)h[j];
+      }
+    }
+  }
+}
+
 }  // namespace dense

@@ -11,12 +11,19 @@ int tile_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, cons
 int pair_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, const Args& a, cudaStream_t s);
 int pair_group(const Maps* maps, const Args* p, const bool* a_mn, int n_long, cudaStream_t s);
 
+int mid_product(int kind, int epi, const Maps& maps, const Args& a, int splits, cudaStream_t s);
+int mid_token_box(int tokens);
 int few_product(int kind, int epi, const void* x, long long x_pitch, const void* w0, const void* w1, const Args& a, cudaStream_t s);
 bool few_can_fuse(int T, int K);
 
 namespace {
 
-constexpr int kFewTokens = 16;   // up to here the kernel that streams the weights through registers
+constexpr int kMidTokens = 256;  // up to here the kernel whose M operand is the weights
+
+// The kernel that streams the weights through registers: always up to 8 tokens, and up to 16 (its second token tile halves the
+// loads it keeps in flight) where there are so few weights that latency counts.  16 tokens, gate and up: 4 MB 4.8 us against
+// 6.4, 67 MB 24.9 us against 16.7.
+bool few_tokens(int T, long long weight_bytes) { return T <= 8 || (T <= 16 && weight_bytes <= (16LL << 20)); }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -100,9 +107,28 @@ long long pair_tiles(const Product& p) {
 }
 long long steps_of(const Product& p) { return (long long)dmoq_ceil_div(p.args.K, p.kind == KIND_I8 ? 128 : 64) * p.args.segs; }
 
+// The kernel for a product.  Pairs of blocks need enough 256-wide tiles to go round (half the pairs; fewer tiles are faster
+// unpaired with K split: 512 x 4096 by 8192, 32 tiles, 22.4 us against 18.8).  Up to 128 tokens reading the weights is all
+// that counts; up to 256 it still beats 128-wide tiles (130 x 4096 by 8192: 27 us against 32), but not full pairs (130 x 5120 by
+// 27648: 90 us against 77).
 int run(const Product& p, cudaStream_t s) {
   Maps maps;
-  if (pair_tiles(p) * 4 >= dmoq_sm_count()) {
+  const bool pair = pair_tiles(p) * 4 >= dmoq_sm_count();
+  if (p.args.M <= (pair ? 128 : kMidTokens) && !p.a_mn && !p.b_mn && p.args.segs == 1) {
+    const int es = p.kind == KIND_I8 ? 1 : 2, rows = is_dual(p.epi) ? 64 : 128;
+    const long long tiles = dmoq_ceil_div(p.args.N, rows), steps = steps_of(p);
+    // Up to two blocks an SM stream at once.  Below half the SMs a split pays from 2 steps a block on, above from 8: 32 tiles of
+    // 32 steps take 10.4 us in 4 parts and 11.6 in 8; 64 tiles of 64 steps 22.4 us in 2 and 19.3 in 4; 216 tiles of 80 steps
+    // 50 us whole and 56 in 2.
+    int splits = 1;
+    const int most = p.args.M <= 128 ? dmoq_sm_count() : dmoq_sm_count() / 2;
+    while (splits < 8 && tiles * splits <= most && steps >= splits * (tiles * splits * 2 < dmoq_sm_count() ? 4 : 16)) splits *= 2;
+    int rc = tma_ok(p.a[0], es) && tma_ok(p.b[0], es) ? make_map(&maps.b[0], p.a[0], es, mid_token_box(p.args.M)) : DMOQ_EINVAL;
+    if (rc == DMOQ_OK) rc = make_map(&maps.a[0], p.b[0], es, rows);
+    if (rc == DMOQ_OK && is_dual(p.epi)) rc = tma_ok(p.b[1], es) ? make_map(&maps.a[1], p.b[1], es, rows) : DMOQ_EINVAL;
+    return rc != DMOQ_OK ? rc : mid_product(p.kind, p.epi, maps, p.args, splits, s);
+  }
+  if (pair) {
     const int rc = make_maps(maps, p, 128);
     return rc != DMOQ_OK ? rc : pair_product(p.kind, p.a_mn, p.b_mn, p.epi, maps, pair_args(p), s);
   }
@@ -175,7 +201,7 @@ int check_ffn(int T, int H, int I) {
 // the kernel makes them itself.
 int int8_product(const void* x, long long x_pitch, int8_t* codes, float* scales, const int8_t* w0, const float* s0, const int8_t* w1,
                  const float* s1, const void* bias, int bf16, int T, int N, int K, void* out, cudaStream_t s) {
-  const bool few = T <= kFewTokens, fuse = x != nullptr && few && few_can_fuse(T, K);
+  const bool few = few_tokens(T, (long long)N * K * (w1 ? 2 : 1)), fuse = x != nullptr && few_can_fuse(T, K);   // fuse implies few
   if (x != nullptr && !fuse) {
     const int rc = dmoq_token_quant_launch(x, bf16, T, K, x_pitch, codes, scales, s);
     if (rc != DMOQ_OK) return rc;
@@ -274,8 +300,8 @@ extern "C" int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, c
   up.args.out[0] = static_cast<uint16_t*>(h);
   for (int e = 0; saved && e < 3; ++e) up.args.out[1 + e] = static_cast<uint16_t*>(saved) + e * (size_t)T * I;
   up.args.ld_out = I;
-  const bool few = T <= kFewTokens;
-  int rc = few && !saved ? few_product(KIND_16, EPI_SILU, x, 2 * x_pitch, w_gate, w_up, up.args, s) : run(up, s);
+  const long long w_bytes = 2LL * H * I;
+  int rc = few_tokens(T, 2 * w_bytes) && !saved ? few_product(KIND_16, EPI_SILU, x, 2 * x_pitch, w_gate, w_up, up.args, s) : run(up, s);
   if (rc != DMOQ_OK) return rc;
   Product down;
   down.a[0] = {h, T, I, I};
@@ -283,7 +309,7 @@ extern "C" int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, c
   down.args.M = T, down.args.N = H, down.args.K = I, down.args.segs = 1, down.args.bf16 = is_bf16, down.args.vec = 1;
   down.args.out[0] = static_cast<uint16_t*>(y);
   down.args.ld_out = H;
-  return few ? few_product(KIND_16, EPI_OUT, h, 2 * (long long)I, w_down, nullptr, down.args, s) : run(down, s);
+  return few_tokens(T, w_bytes) ? few_product(KIND_16, EPI_OUT, h, 2 * (long long)I, w_down, nullptr, down.args, s) : run(down, s);
 }
 
 extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate,

@@ -4,7 +4,7 @@
 // ends with the gate and the up value of the same output), and go from global memory straight to registers.  A thread's 16
 // bytes of a row hold consecutive k and feed two MMA steps: the order of k inside a step is permuted the same way for both
 // operands, which leaves the sums as they are.  The eight warps split K in steps of 128 bytes; their partial sums are joined
-// in a fixed order.  8-bit: with FUSE the block makes the tokens' codes itself, in shared memory, while its first weights are
+// in a fixed order.  8-bit: with FUSE the block makes the codes of up to 8 tokens itself, in shared memory, while its first weights are
 // on their way (as long as they fit in 17 KB), which saves a launch.
 #include "token_codes.cuh"
 
@@ -59,8 +59,8 @@ __global__ void __launch_bounds__(32 * kWarps) dense_few_kernel(const __grid_con
   const Args& a = f.p;
   __shared__ uint32_t part[kWarps][16][NT * 8 + 1];
   __shared__ __align__(16) uint8_t codes[FUSE ? kFuseBytes : 16];
-  __shared__ uint32_t top[16];
-  __shared__ float token_scale[16];
+  __shared__ uint32_t top[8];
+  __shared__ float token_scale[8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * kRows;
   const int kb = kKind == KIND_I8 ? a.K : 2 * a.K;         // bytes of a row
@@ -83,9 +83,9 @@ __global__ void __launch_bounds__(32 * kWarps) dense_few_kernel(const __grid_con
   load_weights(warp * 128);
 
   if (FUSE) {
-    if (tid < 16) top[tid] = 0u;
+    if (tid < 8) top[tid] = 0u;
     __syncthreads();
-    const int per = 32 * kWarps / (a.M <= 1 ? 1 : a.M <= 2 ? 2 : a.M <= 4 ? 4 : a.M <= 8 ? 8 : 16);   // threads of a token
+    const int per = 32 * kWarps / (a.M <= 1 ? 1 : a.M <= 2 ? 2 : a.M <= 4 ? 4 : 8);   // threads of a token
     const int token = tid / per, j0 = tid % per, n8 = a.K / 8;
     const uint4* src = reinterpret_cast<const uint4*>(f.x + token * f.x_pitch);
     if (token < a.M) {
@@ -160,14 +160,14 @@ __global__ void __launch_bounds__(32 * kWarps) dense_few_kernel(const __grid_con
 template <int TYPE, int EPI, bool FUSE>
 int launch(const FewArgs& f, cudaStream_t s) {
   const int blocks = dmoq_ceil_div(f.p.N, is_dual(EPI) ? 8 : 16);
-  if (f.p.M <= 8) dense_few_kernel<TYPE, EPI, FUSE, 1><<<blocks, 32 * kWarps, 0, s>>>(f);
-  else dense_few_kernel<TYPE, EPI, FUSE, 2><<<blocks, 32 * kWarps, 0, s>>>(f);
+  if (FUSE || f.p.M <= 8) dense_few_kernel<TYPE, EPI, FUSE, 1><<<blocks, 32 * kWarps, 0, s>>>(f);
+  else dense_few_kernel<TYPE, EPI, false, 2><<<blocks, 32 * kWarps, 0, s>>>(f);
   return dmoq_launch_status();
 }
 
 }  // namespace
 
-bool few_can_fuse(int T, int K) { return T <= 16 && (long long)T * code_pitch(K) <= kFuseBytes; }
+bool few_can_fuse(int T, int K) { return T <= 8 && (long long)T * code_pitch(K) <= kFuseBytes; }
 
 // x: 16-bit rows (pitch in bytes), or codes where a.a_scale is given; w1 only when dual.
 int few_product(int kind, int epi, const void* x, long long x_pitch, const void* w0, const void* w1, const Args& a, cudaStream_t s) {

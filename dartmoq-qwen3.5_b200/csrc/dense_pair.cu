@@ -236,6 +236,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) dense_p
       const int row0 = m0 + quarter * 32;
       const long long row = row0 + lane;
       const float sa = KIND == KIND_I8 && row < a.M ? a.a_scale[row] : 0.f;
+      // The gradient's planes are loaded a block ahead in whole 64-byte row pieces (four lanes a row; a row a lane would touch 32
+      // lines an instruction) and turned into a row a lane through shared memory, like the outputs on their way out.
+      uint4 in[3][4];
+      auto load_planes = [&](int col0) {
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int at = row0 + 8 * r + (lane >> 2), col = col0 + 8 * (lane & 3);   // rows are whole groups of eight elements
+            in[p][r] = at < a.M && col < a.N ? ld_global_v4(a.in[p] + at * a.ld_in + col) : make_uint4(0u, 0u, 0u, 0u);
+          }
+      };
+      if (EPI == EPI_GRAD) load_planes(n0 + side * 128);
       if (!mbar_wait(bar_acc_full(b), (i / 2) & 1, abort_flag, status)) break;
       tc_fence_after();
       const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16) + b * 256;
@@ -246,13 +259,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) dense_p
         uint32_t v[32], w[32];
         tc_ld32(acc + c, v);
         if (kDual) tc_ld32(acc + 128 + c, w);
-        uint4 in[3][4];
-        if (EPI == EPI_GRAD && row < a.M) {                // rows of the planes are whole groups of eight elements
+        uint4 plane[3][4];                                 // of this lane's row
+        if (EPI == EPI_GRAD) {
 #pragma unroll
-          for (int p = 0; p < 3; ++p)
+          for (int p = 0; p < 3; ++p, ++n_out) {
+            const uint32_t unit = units + (n_out % kUnits) * kUnitBytes;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (col0 + 8 * j < a.N) in[p][j] = *reinterpret_cast<const uint4*>(a.in[p] + row * a.ld_in + col0 + 8 * j);
+            for (int r = 0; r < 4; ++r) {
+              const int at = 8 * r + (lane >> 2);
+              st_shared_v4(unit + at * 64 + (((lane & 3) ^ ((at >> 1) & 3)) << 4), in[p][r].x, in[p][r].y, in[p][r].z, in[p][r].w);
+            }
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) plane[p][j] = ld_shared_v4(unit + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4));
+          }
+          if (u + 1 < kBlocks) load_planes(col0 + 32);
         }
         float sc0 = 1.f, sc1 = 1.f, bias = 0.f;            // of column col0 + lane
         if (KIND == KIND_I8 && col0 + lane < a.N) {
@@ -303,7 +324,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) dense_p
             o[3 % outputs_of(EPI)][j] = saved_low(si[0], sl[0]) | (saved_low(si[1], sl[1]) << 16);
           } else {
             auto word = [&](int p) {
-              const uint4 q = in[p][j / 4];
+              const uint4 q = plane[p][j / 4];
               return (j & 3) == 0 ? q.x : (j & 3) == 1 ? q.y : (j & 3) == 2 ? q.z : q.w;
             };
             const uint32_t s2 = word(0), p2 = word(1), l2 = word(2);

@@ -8,6 +8,7 @@
 // Status word of the dense kernels on the current device: bit 0 = a bounded wait ran out.
 int dmoq_dense_status(int* out);
 int dmoq_dense_pair_status(int* out);
+int dmoq_dense_mid_status(int* out);
 
 namespace dense {
 
@@ -135,6 +136,28 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t smem_addr, uint32_t ran
 __device__ __forceinline__ uint4 ld_cluster_v4(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+// The sum over the cluster's blocks of four values at this offset of their shared memory, in rank order.  All loads are issued
+// before the first is used: one round trip, not one a block.
+template <bool INTEGER>
+__device__ __forceinline__ void sum_over_cluster(uint32_t addr, uint32_t blocks, uint32_t (&v)[4]) {
+  uint4 p[8];
+#pragma unroll
+  for (uint32_t q = 0; q < 8; ++q)
+    if (q < blocks) p[q] = ld_cluster_v4(map_to_rank(addr, q));
+  v[0] = p[0].x, v[1] = p[0].y, v[2] = p[0].z, v[3] = p[0].w;
+#pragma unroll
+  for (uint32_t q = 1; q < 8; ++q) {
+    if (q >= blocks) break;
+    const uint32_t e[4] = {p[q].x, p[q].y, p[q].z, p[q].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = INTEGER ? v[j] + e[j] : __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(e[j]));
+  }
+}
+__device__ __forceinline__ uint4 ld_global_v4(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
 __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {

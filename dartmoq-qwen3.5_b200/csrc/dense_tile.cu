@@ -148,70 +148,8 @@ __global__ void __launch_bounds__(256, 1) dense_tile_kernel(const __grid_constan
   }
   if (splits > 1) cluster_sync();
 
-  // join and finish: this block's rows of the tile, four columns a thread
-  constexpr int kQuads = kCols / 4;
-  const int row_lo = 128 * rank / splits, row_hi = 128 * (rank + 1) / splits;
-  for (int i = row_lo * kQuads + tid; i < row_hi * kQuads; i += 256) {
-    const int r = i / kQuads, c = i % kQuads * 4;
-    const long long row = m0 + r;
-    const int col = n0 + c;
-    if (row >= a.M || col >= a.N) continue;
-    uint32_t v[4] = {0u, 0u, 0u, 0u}, u[4] = {0u, 0u, 0u, 0u};
-    for (uint32_t q = 0; q < splits; ++q) {
-      const uint32_t at = map_to_rank(sb, q) + r * C::kPitch + c * 4;
-      auto add = [&](uint32_t(&t)[4], const uint4 p) {
-        const uint32_t e[4] = {p.x, p.y, p.z, p.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          t[j] = KIND == KIND_I8 ? t[j] + e[j] : __float_as_uint(__uint_as_float(t[j]) + __uint_as_float(e[j]));
-      };
-      add(v, ld_cluster_v4(at));
-      if (kDual) add(u, ld_cluster_v4(at + kCols * 4));
-    }
-    const int n = min(4, a.N - col);
-    const float sa = KIND == KIND_I8 ? a.a_scale[row] : 1.f;
-    const long long at_out = row * a.ld_out + col;
-    float o[3][4];
-    if (EPI == EPI_GRAD) {
-      const long long at_in = row * a.ld_in + col;   // the planes' rows are whole groups of four (sizes are multiples of 8)
-      uint2 pl[3];
-#pragma unroll
-      for (int e = 0; e < 3; ++e) pl[e] = *reinterpret_cast<const uint2*>(a.in[e] + at_in);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        auto half = [&](const uint2 w) { return ((j < 2 ? w.x : w.y) >> (16 * (j & 1))) & 0xffffu; };
-        const float dh = __uint_as_float(v[j]);
-        o[0][j] = dh * saved_slope(half(pl[1]), half(pl[2]));
-        o[1][j] = dh * saved_silu(half(pl[0]), half(pl[2]));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float e[3] = {0.f, 0.f, 0.f};
-        if (j < n) finish<KIND, EPI>(a, row, col + j, v[j], u[j], sa, e);
-        o[0][j] = e[0], o[1][j] = e[1], o[2][j] = e[2];
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < outputs_of(EPI); ++e) {
-      uint32_t lo, hi;
-      if (EPI == EPI_SILU_SAVE && e > 0) {
-        auto word = [&](int j) {
-          return e == 3 ? saved_low(o[1][j], o[2][j]) : __float_as_uint(o[e < 3 ? e : 0][j]) >> 16;
-        };
-        lo = word(0) | (word(1) << 16), hi = word(2) | (word(3) << 16);
-      } else {
-        lo = pack16(o[e < 3 ? e : 0][0], o[e < 3 ? e : 0][1], a.bf16), hi = pack16(o[e < 3 ? e : 0][2], o[e < 3 ? e : 0][3], a.bf16);
-      }
-      uint16_t* dst = a.out[e] + at_out;
-      if (a.vec) {
-        *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
-      } else {
-        const uint32_t h[4] = {lo & 0xffffu, lo >> 16, hi & 0xffffu, hi >> 16};
-        for (int j = 0; j < n; ++j) dst[j] = (uint16_t)h[j];
-      }
-    }
-  }
+  // join and finish: this block's rows of the tile
+  finish_rows<KIND, EPI, kCols>(a, sb, C::kPitch, 128 * rank / splits, 128 * (rank + 1) / splits, m0, n0, splits, tid);
   if (splits > 1) cluster_sync();   // a block's shared memory lives until the others have read it
 }
 
@@ -266,9 +204,10 @@ int tile_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, cons
 int dmoq_dense_status(int* out) {
   int v = 0;
   if (cudaMemcpyFromSymbol(&v, g_dmoq_dense_status, sizeof(int)) != cudaSuccess) return DMOQ_EDEVICE;
-  int w = 0;
-  const int rc = dmoq_dense_pair_status(&w);
+  int w = 0, m = 0;
+  int rc = dmoq_dense_pair_status(&w);
+  if (rc == DMOQ_OK) rc = dmoq_dense_mid_status(&m);
   if (rc != DMOQ_OK) return rc;
-  *out = v | w;
+  *out = v | w | m;
   return DMOQ_OK;
 }

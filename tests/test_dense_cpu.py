@@ -49,8 +49,9 @@ def test_int8_products_refuse():
 def test_int8_scratch_size():
     f = _lib.load().dmoq_int8_scratch_bytes
     assert f(40, 128) == 40 * 128 + 40 * 4 and f(1000, 131056) == 1000 * 131056 + 4000
-    assert f(0, 128) == 0 and f(1, 128) == 0 and f(16, 512) == 0        # no tokens; few: the product makes the codes itself
-    assert f(16, 8192) == 16 * 8192 + 64 and f(1, 65536) == 65536 + 4   # few, but too long for that
+    assert f(0, 128) == 0 and f(1, 128) == 0 and f(8, 1024) == 0        # no tokens; few: the product makes the codes itself
+    assert f(8, 8192) == 8 * 8192 + 32 and f(1, 65536) == 65536 + 4     # few, but too long for that
+    assert f(9, 128) == 9 * 128 + 36
     assert f(4, 100) == 0 and f(-1, 128) == 0                           # refused by the calls themselves
 
 

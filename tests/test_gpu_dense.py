@@ -92,9 +92,10 @@ def test_quantize_shapes_and_strides():
 
 # --------------------------------------------------------------------------------------------- 8-bit products
 
-SIZES8 = [(1, 1, 16), (1, 33, 128), (2, 512, 2048), (7, 1001, 144), (16, 256, 2064), (17, 96, 4096), (64, 640, 512), (127, 130, 272),
+SIZES8 = [(1, 1, 16), (1, 33, 128), (2, 512, 2048), (7, 1001, 144), (16, 256, 2064), (17, 96, 4096), (32, 100, 1040), (64, 640, 512), (65, 257, 3600), (127, 130, 272),
           (129, 257, 1024), (300, 1001, 2064), (700, 4096, 256), (1300, 2200, 640), (1545, 2201, 144), (9, 40, 1040),
-          (3, 24, 5200), (16, 33, 9104)]
+          (3, 24, 5200), (16, 33, 9104), (8, 70, 1024), (12, 9000, 2048),
+          (130, 1000, 528), (256, 333, 2064)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -190,9 +191,9 @@ def test_int8_shapes_strides_and_refusals():
 
 # --------------------------------------------------------------------------------------------- gated feed-forward
 
-FFN_SIZES = [(1, 8, 8), (1, 256, 136), (3, 72, 200), (16, 512, 256), (33, 128, 1032), (64, 256, 72), (128, 320, 128), (129, 264, 136),
+FFN_SIZES = [(1, 8, 8), (1, 256, 136), (3, 72, 200), (16, 512, 256), (33, 128, 1032), (31, 1032, 264), (64, 256, 72), (100, 264, 2056), (128, 320, 128), (129, 264, 136),
              (257, 1032, 520), (1000, 256, 128), (640, 520, 1040), (1500, 1032, 1544),
-             (9, 1032, 264), (2, 2056, 4104)]
+             (9, 1032, 264), (2, 2056, 4104), (12, 2056, 4104), (200, 264, 1032), (256, 1032, 136)]
 
 
 def ffn_inputs(t, h, i, dtype, seed=0):
