@@ -287,7 +287,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) dense_p
           __syncwarp();
           if (lane == 0) {
             const uint32_t remote = map_to_rank(bar_acc_empty(b), 0);
-            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
+            // block scope: what is handed over are TMEM columns whose loads have completed; at cluster scope the release would
+            // wait for this warp's outstanding global stores
+            asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
           }
         }
         uint32_t o[outputs_of(EPI)][16];
