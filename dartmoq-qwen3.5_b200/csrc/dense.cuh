@@ -46,27 +46,31 @@ struct Args {
   long long ld_in, ld_out;  // row pitches in elements
 };
 
+// The arithmetic of the epilogues, with its roundings spelled out (no contraction left to the compiler), so that an 8-bit result
+// does not depend on the kernel that a batch's size selects.
+__device__ __forceinline__ float scaled(uint32_t sum, float token_scale, float row_scale) {
+  return __fmul_rn((float)(int)sum, __fmul_rn(token_scale, row_scale));
+}
+__device__ __forceinline__ float gated(float g, float u) { return __fmul_rn(__fmul_rn(g, sigmoid(g)), u); }
+// silu'(g) = s (1 + g (1 - s)) = s + silu(g) (1 - s), s = sigmoid(g)
+__device__ __forceinline__ float slope_of(float s, float silu, float u) { return __fmul_rn(u, __fmaf_rn(silu, __fsub_rn(1.f, s), s)); }
+
 // One output element's value: v0 (and v1 of the second product) are the sums.
-// The gradient of silu: silu'(g) = s (1 + g (1 - s)), s = sigmoid(g).
 template <int KIND, int EPI>
 __device__ __forceinline__ void finish(const Args& a, long long row, int col, uint32_t v0, uint32_t v1, float sa, float (&o)[3]) {
-  float x = (KIND == KIND_I8) ? (float)(int)v0 : __uint_as_float(v0);
-  float y = (KIND == KIND_I8) ? (float)(int)v1 : __uint_as_float(v1);
-  if (KIND == KIND_I8) {
-    x *= sa * a.b_scale[0][col];
-    if (is_dual(EPI)) y *= sa * a.b_scale[1][col];
-  }
+  const float x = (KIND == KIND_I8) ? scaled(v0, sa, a.b_scale[0][col]) : __uint_as_float(v0);
+  const float y = !is_dual(EPI) ? 0.f : (KIND == KIND_I8) ? scaled(v1, sa, a.b_scale[1][col]) : __uint_as_float(v1);
   if (EPI == EPI_OUT || EPI == EPI_GRAD) {
     o[0] = x;
   } else if (EPI == EPI_SCALE) {
-    o[0] = a.bias ? x + unpack16(a.bias[col], a.bf16) : x;
+    o[0] = a.bias ? __fadd_rn(x, unpack16(a.bias[col], a.bf16)) : x;
   } else if (EPI == EPI_SILU) {
-    o[0] = x * sigmoid(x) * y;
+    o[0] = gated(x, y);
   } else if (EPI == EPI_SILU_SAVE) {
-    const float s = sigmoid(x), si = x * s;
-    o[0] = si * y;
+    const float s = sigmoid(x), si = __fmul_rn(x, s);
+    o[0] = __fmul_rn(si, y);
     o[1] = si;
-    o[2] = y * (s + si * (1.f - s));
+    o[2] = slope_of(s, si, y);
   }
 }
 

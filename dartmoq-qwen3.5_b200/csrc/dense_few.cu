@@ -27,11 +27,7 @@ struct FewArgs {
 
 enum Type { BF16 = 0, FP16 = 1, INT8 = 2 };
 
-__device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {   // weights are read once
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
+__device__ __forceinline__ void prefetch_l2(const uint8_t* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 template <int TYPE>
 __device__ __forceinline__ void mma(uint32_t (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -76,10 +72,14 @@ __global__ void __launch_bounds__(32 * kWarps) dense_few_kernel(const __grid_con
       for (int h = 0; h < 2; ++h) {
         const int b = base + i * (kWarps * 128) + 64 * h;
         const bool in = b + 16 * t < kb;
-        wa[i][h] = in ? ld_stream(row_a + b) : make_uint4(0u, 0u, 0u, 0u);
-        wb[i][h] = in ? ld_stream(row_b + b) : make_uint4(0u, 0u, 0u, 0u);
+        wa[i][h] = in ? ld_global_v4(row_a + b) : make_uint4(0u, 0u, 0u, 0u);
+        wb[i][h] = in ? ld_global_v4(row_b + b) : make_uint4(0u, 0u, 0u, 0u);
       }
   };
+  for (int b = warp * 128; b < kb; b += kWarps * 128) {     // brings the block's weights into L2 while the kernel before this one ends
+    if (t == 0) prefetch_l2(row_a + b), prefetch_l2(row_b + b);   // 128 bytes of either row
+  }
+  overlap_point();
   load_weights(warp * 128);
 
   if (FUSE) {
@@ -90,14 +90,14 @@ __global__ void __launch_bounds__(32 * kWarps) dense_few_kernel(const __grid_con
     const uint4* src = reinterpret_cast<const uint4*>(f.x + token * f.x_pitch);
     if (token < a.M) {
       uint32_t top2 = 0u;
-      for (int i = j0; i < n8; i += per) top2 = magnitude_max(top2, __ldg(src + i));
+      for (int i = j0; i < n8; i += per) top2 = magnitude_max(top2, src[i]);
       atomicMax(&top[token], magnitude_join(top2));        // a maximum: the order does not matter
     }
     __syncthreads();
     if (token < a.M) {
       const RowScale s = row_scale(top[token], a.bf16);
       if (j0 == 0) token_scale[token] = s.scale;
-      for (int i = j0; i < n8; i += per) *reinterpret_cast<uint2*>(codes + token * code_pitch(a.K) + 8 * i) = codes8(__ldg(src + i), s, a.bf16);
+      for (int i = j0; i < n8; i += per) *reinterpret_cast<uint2*>(codes + token * code_pitch(a.K) + 8 * i) = codes8(src[i], s, a.bf16);
     }
     __syncthreads();
   }
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(32 * kWarps) dense_few_kernel(const __grid_con
           uint4 v = make_uint4(0u, 0u, 0u, 0u);
           if (token < a.M && b < kb)
             v = FUSE ? *reinterpret_cast<const uint4*>(codes + token * code_pitch(a.K) + b)
-                     : __ldg(reinterpret_cast<const uint4*>(f.x + token * f.x_pitch + b));
+                     : *reinterpret_cast<const uint4*>(f.x + token * f.x_pitch + b);
           xb[n][i][h] = v;
         }
 #pragma unroll
@@ -160,9 +160,8 @@ __global__ void __launch_bounds__(32 * kWarps) dense_few_kernel(const __grid_con
 template <int TYPE, int EPI, bool FUSE>
 int launch(const FewArgs& f, cudaStream_t s) {
   const int blocks = dmoq_ceil_div(f.p.N, is_dual(EPI) ? 8 : 16);
-  if (FUSE || f.p.M <= 8) dense_few_kernel<TYPE, EPI, FUSE, 1><<<blocks, 32 * kWarps, 0, s>>>(f);
-  else dense_few_kernel<TYPE, EPI, false, 2><<<blocks, 32 * kWarps, 0, s>>>(f);
-  return dmoq_launch_status();
+  if (FUSE || f.p.M <= 8) return launch_overlapped(dense_few_kernel<TYPE, EPI, FUSE, 1>, blocks, 32 * kWarps, 0, 0, s, f);
+  return launch_overlapped(dense_few_kernel<TYPE, EPI, false, 2>, blocks, 32 * kWarps, 0, 0, s, f);
 }
 
 }  // namespace

@@ -133,6 +133,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) dense_p
   tc_fence_after();
   uint32_t tmem;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+  overlap_point();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -300,9 +301,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) dense_p
           for (int h = 0; h < 2; ++h) {
             const int q = 2 * j + h;
             if (KIND == KIND_I8) {
-              x[h] = (float)(int)v[q] * (sa * __shfl_sync(0xffffffffu, sc0, q));
-              if (kDual) y[h] = (float)(int)w[q] * (sa * __shfl_sync(0xffffffffu, sc1, q));
-              if (EPI == EPI_SCALE) x[h] += __shfl_sync(0xffffffffu, bias, q);
+              x[h] = scaled(v[q], sa, __shfl_sync(0xffffffffu, sc0, q));
+              if (kDual) y[h] = scaled(w[q], sa, __shfl_sync(0xffffffffu, sc1, q));
+              if (EPI == EPI_SCALE && a.bias) x[h] = __fadd_rn(x[h], __shfl_sync(0xffffffffu, bias, q));
             } else {
               x[h] = __uint_as_float(v[q]);
               if (kDual) y[h] = __uint_as_float(w[q]);
@@ -311,14 +312,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) dense_p
           if (EPI == EPI_OUT || EPI == EPI_SCALE) {
             o[0][j] = pack16(x[0], x[1], a.bf16);
           } else if (EPI == EPI_SILU) {
-            o[0][j] = pack16(x[0] * sigmoid(x[0]) * y[0], x[1] * sigmoid(x[1]) * y[1], a.bf16);
+            o[0][j] = pack16(gated(x[0], y[0]), gated(x[1], y[1]), a.bf16);
           } else if (EPI == EPI_SILU_SAVE) {
             float si[2], sl[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const float s = sigmoid(x[h]);
-              si[h] = x[h] * s;
-              sl[h] = y[h] * (s + si[h] * (1.f - s));
+              si[h] = __fmul_rn(x[h], s);
+              sl[h] = slope_of(s, si[h], y[h]);
             }
             o[0][j] = pack16(si[0] * y[0], si[1] * y[1], a.bf16);
             o[1 % outputs_of(EPI)][j] = (__float_as_uint(si[0]) >> 16) | (__float_as_uint(si[1]) & 0xffff0000u);
@@ -399,8 +400,7 @@ int launch(Work<NP>& work, cudaStream_t s) {
     const int ahead = work.long_tiles % pairs;
     work.fill = ahead == 0 || shorts == 0 ? 0 : (int)std::min<long long>(steps(0) / steps(NP - 1), shorts / (pairs - ahead));
   }
-  kernel<<<2 * pairs, kThreads, kSmem, s>>>(work);
-  return dmoq_launch_status();
+  return launch_overlapped(kernel, 2 * pairs, kThreads, kSmem, 0, s, work);
 }
 
 template <int KIND, bool AMN, bool BMN, int EPI>

@@ -15,6 +15,35 @@ namespace dense {
 constexpr uint32_t kSpinLimit = 1u << 26;
 constexpr long long kWaitCycles = 2000000000LL;   // about one second
 
+// The kernels of the dense operators are launched so that one may be set up while its predecessor in the stream still runs
+// (launch_overlapped).  overlap_point stands behind a kernel's set-up, which touches no global memory but for L2 prefetches:
+// every block waits there until all that comes before the kernel in the stream has completed, and only then lets the next
+// kernel's blocks in, so that at most two kernels overlap.  TMEM is allocated in front of it: the blocks that come in early
+// never take columns that this kernel has yet to get.  What is read behind it is read with ordinary loads, not as constant.
+__device__ __forceinline__ void overlap_point() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+template <class Kernel, class... Params>
+int launch_overlapped(Kernel* kernel, unsigned grid, unsigned block, size_t smem, unsigned cluster, cudaStream_t s, const Params&... params) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;   // 0: as the kernel was compiled
+  return cudaLaunchKernelEx(&cfg, kernel, params...) == cudaSuccess ? DMOQ_OK : DMOQ_ELAUNCH;
+}
+
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
 }
@@ -157,7 +186,7 @@ __device__ __forceinline__ void sum_over_cluster(uint32_t addr, uint32_t blocks,
 }
 __device__ __forceinline__ uint4 ld_global_v4(const void* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
   return v;
 }
 __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {

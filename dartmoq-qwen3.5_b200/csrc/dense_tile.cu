@@ -64,6 +64,7 @@ __global__ void __launch_bounds__(256, 1) dense_tile_kernel(const __grid_constan
   tc_fence_after();
   uint32_t tmem;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+  overlap_point();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -167,19 +168,7 @@ int launch(const Maps& maps, const Args& a, int splits, cudaStream_t s) {
   constexpr int kCols = is_dual(EPI) ? BN / 2 : BN;
   const long long blocks = (long long)dmoq_ceil_div(a.M, 128) * dmoq_ceil_div(a.N, kCols) * splits;
   if (blocks > 0x7fffffffLL) return DMOQ_ESIZE;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = C::kSmem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = splits;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, maps, a) == cudaSuccess ? DMOQ_OK : DMOQ_ELAUNCH;
+  return launch_overlapped(kernel, (unsigned)blocks, 256, C::kSmem, splits, s, maps, a);
 }
 
 }  // namespace

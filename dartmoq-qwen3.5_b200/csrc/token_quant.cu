@@ -12,6 +12,7 @@ __global__ void __launch_bounds__(256) token_quant_kernel(const uint16_t* x, int
                                                           float* scales) {
   constexpr int kThreads = 32 * WARPS;                     // threads of a row
   const int tid = threadIdx.x % kThreads, n8 = K / 8;
+  overlap_point();
   const long long row = (long long)blockIdx.x * (256 / kThreads) + threadIdx.x / kThreads;
   if (WARPS == 1 && row >= rows) return;
   const uint4* src = reinterpret_cast<const uint4*>(x + row * pitch);
@@ -19,7 +20,7 @@ __global__ void __launch_bounds__(256) token_quant_kernel(const uint16_t* x, int
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int i = tid + j * kThreads;
-    v[j] = i < n8 ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+    v[j] = i < n8 ? src[i] : make_uint4(0u, 0u, 0u, 0u);
   }
   uint32_t top2 = 0u;
 #pragma unroll
@@ -46,11 +47,12 @@ __global__ void __launch_bounds__(256) token_quant_kernel(const uint16_t* x, int
 __global__ void __launch_bounds__(256) token_quant_long_kernel(const uint16_t* x, int bf16, int K, long long pitch, int8_t* codes,
                                                                float* scales) {
   __shared__ uint32_t part[8];
+  overlap_point();
   const long long row = blockIdx.x;
   const int tid = threadIdx.x, n8 = K / 8;
   const uint4* src = reinterpret_cast<const uint4*>(x + row * pitch);
   uint32_t top2 = 0u;
-  for (int i = tid; i < n8; i += 256) top2 = magnitude_max(top2, __ldg(src + i));
+  for (int i = tid; i < n8; i += 256) top2 = magnitude_max(top2, src[i]);
   uint32_t top = __reduce_max_sync(0xffffffffu, magnitude_join(top2));
   if ((tid & 31) == 0) part[tid >> 5] = top;
   __syncthreads();
@@ -59,12 +61,12 @@ __global__ void __launch_bounds__(256) token_quant_long_kernel(const uint16_t* x
   const RowScale s = row_scale(top, bf16);
   if (tid == 0) scales[row] = s.scale;
   uint2* dst = reinterpret_cast<uint2*>(codes + row * (long long)K);
-  for (int i = tid; i < n8; i += 256) dst[i] = codes8(__ldg(src + i), s, bf16);
+  for (int i = tid; i < n8; i += 256) dst[i] = codes8(src[i], s, bf16);
 }
 
 template <int NV, int WARPS>
-void launch(const uint16_t* x, int bf16, int T, int K, long long pitch, int8_t* codes, float* scales, cudaStream_t s) {
-  token_quant_kernel<NV, WARPS><<<dmoq_ceil_div(T, 8 / WARPS), 256, 0, s>>>(x, bf16, T, K, pitch, codes, scales);
+int launch(const uint16_t* x, int bf16, int T, int K, long long pitch, int8_t* codes, float* scales, cudaStream_t s) {
+  return launch_overlapped(token_quant_kernel<NV, WARPS>, dmoq_ceil_div(T, 8 / WARPS), 256, 0, 0, s, x, bf16, T, K, pitch, codes, scales);
 }
 
 }  // namespace
@@ -75,19 +77,13 @@ int dmoq_token_quant_launch(const void* xv, int bf16, int T, int K, long long pi
   const uint16_t* x = static_cast<const uint16_t*>(xv);
   // A warp a row streams best; few rows, or rows beyond a warp's registers, get a block each.
   if (T >= 4 * dmoq_sm_count() && K <= 4096) {
-    if (K <= 1024) launch<4, 1>(x, bf16, T, K, pitch, codes, scales, s);
-    else if (K <= 2048) launch<8, 1>(x, bf16, T, K, pitch, codes, scales, s);
-    else launch<16, 1>(x, bf16, T, K, pitch, codes, scales, s);
-  } else if (K <= 2048) {
-    launch<1, 8>(x, bf16, T, K, pitch, codes, scales, s);
-  } else if (K <= 4096) {
-    launch<2, 8>(x, bf16, T, K, pitch, codes, scales, s);
-  } else if (K <= 8192) {
-    launch<4, 8>(x, bf16, T, K, pitch, codes, scales, s);
-  } else if (K <= 16384) {
-    launch<8, 8>(x, bf16, T, K, pitch, codes, scales, s);
-  } else {
-    token_quant_long_kernel<<<T, 256, 0, s>>>(x, bf16, K, pitch, codes, scales);
+    if (K <= 1024) return launch<4, 1>(x, bf16, T, K, pitch, codes, scales, s);
+    if (K <= 2048) return launch<8, 1>(x, bf16, T, K, pitch, codes, scales, s);
+    return launch<16, 1>(x, bf16, T, K, pitch, codes, scales, s);
   }
-  return dmoq_launch_status();
+  if (K <= 2048) return launch<1, 8>(x, bf16, T, K, pitch, codes, scales, s);
+  if (K <= 4096) return launch<2, 8>(x, bf16, T, K, pitch, codes, scales, s);
+  if (K <= 8192) return launch<4, 8>(x, bf16, T, K, pitch, codes, scales, s);
+  if (K <= 16384) return launch<8, 8>(x, bf16, T, K, pitch, codes, scales, s);
+  return launch_overlapped(token_quant_long_kernel, T, 256, 0, 0, s, x, bf16, K, pitch, codes, scales);
 }

@@ -460,3 +460,16 @@ def test_modules(dtype):
     grads = R.ffn_grads(x, *(p.weight for p in (block.gate_proj, block.up_proj, block.down_proj)), 2 * y)
     for p, name in ((block.gate_proj, "dw_gate"), (block.up_proj, "dw_up"), (block.down_proj, "dw_down")):
         R.close(p.weight.grad, grads[name], ROUNDINGS[name], name)
+
+
+def test_int8_results_do_not_depend_on_the_batch():
+    """A token's 8-bit results are the same in every kernel that its batch's size may select."""
+    g = rng(77)
+    k, n = 1040, 6000
+    x, (w, ws), (w2, ws2) = acts(g, 5000, k, torch.bfloat16), weight8(g, n, k), weight8(g, n, k)
+    b = randn(g, n, dtype=torch.bfloat16)
+    lin, gated = dense.int8_linear(x, w, ws, b), dense.int8_gated_linear(x, w, ws, w2, ws2)
+    for t in (1, 3, 8, 9, 16, 17, 40, 70, 129, 200, 300, 700, 1500):
+        assert torch.equal(dense.int8_linear(x[:t], w, ws, b), lin[:t]), t
+        assert torch.equal(dense.int8_gated_linear(x[:t], w, ws, w2, ws2), gated[:t]), t
+        assert torch.equal(dense.int8_linear(x[:t], w[:500], ws[:500]), dense.int8_linear(x, w[:500], ws[:500])[:t]), t
