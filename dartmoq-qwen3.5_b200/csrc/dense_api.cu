@@ -14,7 +14,7 @@ int pair_group(const Maps* maps, const Args* p, const bool* a_mn, int n_long, cu
 int mid_product(int kind, int epi, const Maps& maps, const Args& a, int splits, cudaStream_t s);
 int mid_token_box(int tokens);
 int few_product(int kind, int epi, const void* x, long long x_pitch, const void* w0, const void* w1, const Args& a, cudaStream_t s);
-bool few_can_fuse(int T, int K);
+bool few_can_fuse(int T, int K, int N, bool dual);
 
 namespace {
 
@@ -201,7 +201,7 @@ int check_ffn(int T, int H, int I) {
 // the kernel makes them itself.
 int int8_product(const void* x, long long x_pitch, int8_t* codes, float* scales, const int8_t* w0, const float* s0, const int8_t* w1,
                  const float* s1, const void* bias, int bf16, int T, int N, int K, void* out, cudaStream_t s) {
-  const bool few = few_tokens(T, (long long)N * K * (w1 ? 2 : 1)), fuse = x != nullptr && few_can_fuse(T, K);   // fuse implies few
+  const bool few = few_tokens(T, (long long)N * K * (w1 ? 2 : 1)), fuse = x != nullptr && few_can_fuse(T, K, N, w1 != nullptr);   // fuse implies few
   if (x != nullptr && !fuse) {
     const int rc = dmoq_token_quant_launch(x, bf16, T, K, x_pitch, codes, scales, s);
     if (rc != DMOQ_OK) return rc;
@@ -257,8 +257,8 @@ extern "C" int dmoq_int8_gated_gemm(const int8_t* codes, const float* scales, co
 }
 
 // scratch of the two calls below: the codes, then the scales (T K is a multiple of 16)
-extern "C" size_t dmoq_int8_scratch_bytes(int32_t T, int32_t K) {
-  if (check_sizes8(T, 1, K) != DMOQ_OK || few_can_fuse(T, K)) return 0;
+extern "C" size_t dmoq_int8_scratch_bytes(int32_t T, int32_t N, int32_t K, int32_t gated) {
+  if (check_sizes8(T, N, K) != DMOQ_OK || few_can_fuse(T, K, N, gated != 0)) return 0;
   return (size_t)T * K + (size_t)T * sizeof(float);
 }
 
@@ -266,7 +266,7 @@ extern "C" int dmoq_int8_linear(const void* x, int32_t is_bf16, int64_t x_pitch,
                                 int32_t T, int32_t N, int32_t K, void* scratch, void* out, void* stream) {
   const int rc = check_sizes8(T, N, K);
   if (rc != DMOQ_OK || T == 0) return rc;
-  DMOQ_CHECK_ARG(rows_usable(x, x_pitch, K) && weight8_ok(w, w_scale) && out && (few_can_fuse(T, K) || usable(scratch)));
+  DMOQ_CHECK_ARG(rows_usable(x, x_pitch, K) && weight8_ok(w, w_scale) && out && (few_can_fuse(T, K, N, false) || usable(scratch)));
   int8_t* codes = static_cast<int8_t*>(scratch);
   return int8_product(x, x_pitch, codes, reinterpret_cast<float*>(codes + (size_t)T * K), w, w_scale, nullptr, nullptr, bias, is_bf16, T, N, K,
                       out, static_cast<cudaStream_t>(stream));
@@ -278,7 +278,7 @@ extern "C" int dmoq_int8_gated_linear(const void* x, int32_t is_bf16, int64_t x_
   const int rc = check_sizes8(T, I, K);
   if (rc != DMOQ_OK || T == 0) return rc;
   DMOQ_CHECK_ARG(rows_usable(x, x_pitch, K) && weight8_ok(w_gate, gate_scale) && weight8_ok(w_up, up_scale) && out &&
-                 (few_can_fuse(T, K) || usable(scratch)));
+                 (few_can_fuse(T, K, I, true) || usable(scratch)));
   int8_t* codes = static_cast<int8_t*>(scratch);
   return int8_product(x, x_pitch, codes, reinterpret_cast<float*>(codes + (size_t)T * K), w_gate, gate_scale, w_up, up_scale, nullptr, is_bf16, T,
                       I, K, out, static_cast<cudaStream_t>(stream));

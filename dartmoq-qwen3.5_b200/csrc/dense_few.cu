@@ -23,6 +23,7 @@ struct FewArgs {
   const uint8_t* w[2];
   const uint8_t* x;          // 16-bit rows, or codes
   long long x_pitch;         // bytes
+  int first_blocks;          // that run at once
 };
 
 enum Type { BF16 = 0, FP16 = 1, INT8 = 2 };
@@ -76,7 +77,9 @@ __global__ void __launch_bounds__(32 * kWarps) dense_few_kernel(const __grid_con
         wb[i][h] = in ? ld_global_v4(row_b + b) : make_uint4(0u, 0u, 0u, 0u);
       }
   };
-  for (int b = warp * 128; b < kb; b += kWarps * 128) {     // brings the block's weights into L2 while the kernel before this one ends
+  // The first blocks bring their weights into L2 while the kernel before this one ends (2048 / 4096, one token: 14.4 us a block
+  // for 15.0); later ones would only load everything twice (8192 / 8192: 66 us became 78).
+  for (int b = warp * 128; b < kb && (int)blockIdx.x < f.first_blocks; b += kWarps * 128) {
     if (t == 0) prefetch_l2(row_a + b), prefetch_l2(row_b + b);   // 128 bytes of either row
   }
   overlap_point();
@@ -166,11 +169,16 @@ int launch(const FewArgs& f, cudaStream_t s) {
 
 }  // namespace
 
-bool few_can_fuse(int T, int K) { return T <= 8 && (long long)T * code_pitch(K) <= kFuseBytes; }
+// Every block makes all codes again.  In a graph the quantiser's own launch costs 0.2 us more than that saves at the least (2048
+// x 512, one token: 3.5 us fused, 3.3 not; 2048 x 4096 twice: 8.1 and 6.8), but a call by itself has 5 us less to do on the
+// host; so only as long as the blocks' codes are few in all.
+bool few_can_fuse(int T, int K, int N, bool dual) {
+  return T <= 8 && (long long)T * code_pitch(K) <= kFuseBytes && (long long)T * K * dmoq_ceil_div(N, dual ? 8 : 16) <= 1 << 20;
+}
 
 // x: 16-bit rows (pitch in bytes), or codes where a.a_scale is given; w1 only when dual.
 int few_product(int kind, int epi, const void* x, long long x_pitch, const void* w0, const void* w1, const Args& a, cudaStream_t s) {
-  const FewArgs f = {a, {static_cast<const uint8_t*>(w0), static_cast<const uint8_t*>(w1)}, static_cast<const uint8_t*>(x), x_pitch};
+  const FewArgs f = {a, {static_cast<const uint8_t*>(w0), static_cast<const uint8_t*>(w1)}, static_cast<const uint8_t*>(x), x_pitch, 2 * dmoq_sm_count()};
   if (kind == KIND_I8) {
     const bool fuse = a.a_scale == nullptr;
     if (epi == EPI_SCALE) return fuse ? launch<INT8, EPI_SCALE, true>(f, s) : launch<INT8, EPI_SCALE, false>(f, s);

@@ -162,15 +162,15 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     n = w.shape[0]
     bias, bias_ptr = _bias_ptr(bias, n, x.dtype, index)
     rows, t, pitch = _rows(x, k)
-    scratch = _int8_scratch(x, t, k)
+    scratch = _int8_scratch(x, t, n, k, False)
     out = x.new_empty(shape[:-1] + (n,))
     _call("dmoq_int8_linear", index, rows.data_ptr(), x.dtype is _BF16, pitch, w.data_ptr(), ws.data_ptr(), bias_ptr, t, n, k,
           _ptr(scratch), out.data_ptr())
     return out
 
 
-def _int8_scratch(x: torch.Tensor, t: int, k: int) -> Optional[torch.Tensor]:
-    need = _lib.load().dmoq_int8_scratch_bytes(t, k)
+def _int8_scratch(x: torch.Tensor, t: int, n: int, k: int, gated: bool) -> Optional[torch.Tensor]:
+    need = _lib.load().dmoq_int8_scratch_bytes(t, n, k, gated)
     return x.new_empty((need,), dtype=torch.uint8) if need else None
 
 
@@ -188,7 +188,7 @@ def int8_gated_linear(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.T
     if wu.shape[0] != n:
         raise ValueError(f"w_gate and w_up must have one shape, got {tuple(wg.shape)} and {tuple(wu.shape)}")
     rows, t, pitch = _rows(x, k)
-    scratch = _int8_scratch(x, t, k)
+    scratch = _int8_scratch(x, t, n, k, True)
     out = x.new_empty(shape[:-1] + (n,))
     _call("dmoq_int8_gated_linear", index, rows.data_ptr(), x.dtype is _BF16, pitch, wg.data_ptr(), sg.data_ptr(), wu.data_ptr(),
           su.data_ptr(), t, n, k, _ptr(scratch), out.data_ptr())

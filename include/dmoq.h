@@ -367,7 +367,7 @@ int dmoq_quantize_packed(const void* w, int32_t w_kind, int32_t N, int32_t K, in
  *   int8_gemm:   out[t][n] = scales[t] w_scale[n] sum_k codes[t][k] w[n][k] (+ bias[n]), rounded once to 16 bits
  *   int8_gated_gemm: out = silu(g) u, g and u the products with w_gate and w_up, rounded once
  *   int8_linear, int8_gated_linear: the same with token_quant in front; scratch (16-byte aligned, for the codes and scales) has
- *                int8_scratch_bytes(T, K) bytes, which is 0 where the tokens are few enough for the product to make their codes
+ *                int8_scratch_bytes(T, N or I, K, 0 or 1) bytes, which is 0 where the tokens are few enough for the product to make their codes
  */
 int dmoq_token_quant(const void* x, int32_t is_bf16, int32_t T, int32_t K, int64_t x_pitch, int8_t* codes, float* scales,
                      void* stream);
@@ -381,7 +381,7 @@ int dmoq_int8_gated_gemm(const int8_t* codes, const float* scales, const int8_t*
 int dmoq_int8_gated_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w_gate, const float* gate_scale,
                            const int8_t* w_up, const float* up_scale, int32_t T, int32_t I, int32_t K, void* scratch,
                            void* out, void* stream);
-size_t dmoq_int8_scratch_bytes(int32_t T, int32_t K);
+size_t dmoq_int8_scratch_bytes(int32_t T, int32_t N, int32_t K, int32_t gated);
 
 /*
  * Gated feed-forward block: h = silu(x w_gate^T) * (x w_up^T), y = h w_down^T; x, y (T, H), w_gate and w_up (I, H), w_down (H, I),

@@ -48,11 +48,12 @@ def test_int8_products_refuse():
 
 def test_int8_scratch_size():
     f = _lib.load().dmoq_int8_scratch_bytes
-    assert f(40, 128) == 40 * 128 + 40 * 4 and f(1000, 131056) == 1000 * 131056 + 4000
-    assert f(0, 128) == 0 and f(1, 128) == 0 and f(8, 1024) == 0        # no tokens; few: the product makes the codes itself
-    assert f(8, 8192) == 8 * 8192 + 32 and f(1, 65536) == 65536 + 4     # few, but too long for that
-    assert f(9, 128) == 9 * 128 + 36
-    assert f(4, 100) == 0 and f(-1, 128) == 0                           # refused by the calls themselves
+    assert f(40, 33, 128, 0) == 40 * 128 + 40 * 4 and f(1000, 1, 131056, 1) == 1000 * 131056 + 4000
+    assert f(0, 33, 128, 0) == 0 and f(1, 33, 128, 1) == 0 and f(8, 512, 1024, 0) == 0   # none; few: the product makes the codes
+    assert f(8, 64, 8192, 0) == 8 * 8192 + 32 and f(1, 8, 65536, 0) == 65536 + 4         # few, but too long for that
+    assert f(1, 16384, 1024, 0) == 0 and f(1, 16400, 1024, 0) == 1028 and f(1, 16384, 1024, 1) == 1028   # or too many blocks
+    assert f(9, 33, 128, 0) == 9 * 128 + 36
+    assert f(4, 33, 100, 0) == 0 and f(-1, 33, 128, 0) == 0                              # refused by the calls themselves
 
 
 def test_gated_ffn_refuses():

@@ -318,7 +318,7 @@ def test_outputs_stay_inside_their_memory():
         g = rng(n)
         x, (w, ws) = acts(g, t, k, torch.bfloat16), weight8(g, n, k)
         out = torch.full((t + 2, n), 7.0, dtype=torch.bfloat16, device=DEV)
-        need = max(int(lib.dmoq_int8_scratch_bytes(t, k)), 16)
+        need = max(int(lib.dmoq_int8_scratch_bytes(t, n, k, 0)), int(lib.dmoq_int8_scratch_bytes(t, n, k, 1)), 16)
         scratch = torch.full((need + 256,), 99, dtype=torch.uint8, device=DEV)
         p = lambda v: C.c_void_p(v.data_ptr())  # noqa: E731
         for name, extra in (("dmoq_int8_linear", (p(w), p(ws), None)), ("dmoq_int8_gated_linear", (p(w), p(ws), p(w), p(ws)))):
