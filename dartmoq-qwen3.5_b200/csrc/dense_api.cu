@@ -183,6 +183,9 @@ bool usable(const void* p) { return p != nullptr && aligned16(p); }
 bool rows_usable(const void* p, long long pitch, int cols) { return usable(p) && pitch >= cols && pitch % 8 == 0; }   // 16-bit rows
 
 constexpr int kMaxDim = 1 << 30;   // rows and columns: tile coordinates stay inside 32 bits
+// The weights' gradients sum over the tokens in one pass: at this many a tile takes a third of the second after which a wait
+// inside a kernel gives up.
+constexpr int kMaxGradTokens = 1 << 26;
 
 int check_sizes8(int T, int N, int K) {
   if (T < 0 || N < 1 || K < 16 || K % 16 != 0) return DMOQ_EINVAL;
@@ -318,6 +321,7 @@ extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const v
                                        void* dw_down, void* stream) {
   const int size = check_ffn(T, H, I);
   if (size != DMOQ_OK) return size;
+  if (T > kMaxGradTokens) return DMOQ_ESIZE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const size_t w_bytes = (size_t)H * I * 2;
   if (T == 0) {   // no tokens: the weights' gradients are zero

@@ -41,7 +41,9 @@ int launch_overlapped(Kernel* kernel, unsigned grid, unsigned block, size_t smem
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 0 ? 2 : 1;   // 0: as the kernel was compiled
-  return cudaLaunchKernelEx(&cfg, kernel, params...) == cudaSuccess ? DMOQ_OK : DMOQ_ELAUNCH;
+  if (cudaLaunchKernelEx(&cfg, kernel, params...) == cudaSuccess) return DMOQ_OK;
+  (void)cudaGetLastError();   // reported by the return value; the next call on this thread starts clean
+  return DMOQ_ELAUNCH;
 }
 
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {

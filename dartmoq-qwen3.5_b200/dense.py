@@ -218,7 +218,6 @@ class _GatedFeedForward(torch.autograd.Function):
         need_x, need_g, need_u, need_d = ctx.needs_input_grad
         y, h, saved = _ffn_forward(rows, t, pitch, w_gate, w_up, w_down, need_x or need_g or need_u)
         ctx.save_for_backward(rows, w_gate, w_up, w_down, h if need_d else None, saved)
-        ctx.pitch = pitch
         return y
 
     @staticmethod
@@ -228,6 +227,10 @@ class _GatedFeedForward(torch.autograd.Function):
         need_x, need_g, need_u, need_d = ctx.needs_input_grad
         hidden, inter = wd.shape
         dy, t, dy_pitch = _rows(dy, hidden)
+        # saved-tensor hooks may have laid them out anew
+        x, _, x_pitch = _rows(x, hidden)
+        wg, wu, wd = _packed(wg), _packed(wu), _packed(wd)
+        h, saved = h if h is None else _packed(h), saved if saved is None else _packed(saved)
         dgu = x.new_empty((t, 2 * inter)) if need_x or need_g or need_u else None
         dx = x.new_empty((t, hidden)) if need_x else None
         # the two halves of one buffer: one product computes both
@@ -235,7 +238,7 @@ class _GatedFeedForward(torch.autograd.Function):
         dwg = dw[0] if need_g else None
         dwu = dw[-1] if need_u else None
         dwd = x.new_empty((hidden, inter)) if need_d else None
-        _call("dmoq_gated_ffn_backward", x.get_device(), dy.data_ptr(), dy_pitch, x.data_ptr(), x.dtype is _BF16, ctx.pitch, wg.data_ptr(),
+        _call("dmoq_gated_ffn_backward", x.get_device(), dy.data_ptr(), dy_pitch, x.data_ptr(), x.dtype is _BF16, x_pitch, wg.data_ptr(),
               wu.data_ptr(), wd.data_ptr(), t, hidden, inter, _ptr(h), _ptr(saved), _ptr(dgu), _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd))
         return dx, dwg, dwu, dwd
 
@@ -244,7 +247,7 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     """(silu(x w_gate^T) * (x w_up^T)) w_down^T for x (..., H), w_gate and w_up (I, H), w_down (H, I), all bf16 or all fp16; H and I
     multiples of 8.  Sums in fp32; the hidden values are rounded to the 16-bit type between the two kernels (they are the second
     product's operand), so fp16 hidden values beyond 65504 become infinite.  Differentiable once in every argument; each gradient
-    that is not needed is not computed."""
+    that is not needed is not computed (at most 2^26 tokens then)."""
     _check_input(x)
     dt, index = x.dtype, x.get_device()
     hidden = x.shape[-1]

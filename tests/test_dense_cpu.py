@@ -71,6 +71,7 @@ def test_gated_ffn_refuses():
         assert lib.dmoq_gated_ffn_backward(*(good[:i] + [None] + good[i + 1:]), None) == EINVAL, i
     for i, v in ((1, 60), (4, 60), (9, 4), (10, 12), (0, ODD), (2, ODD), (11, ODD), (12, ODD), (13, ODD), (14, ODD), (15, ODD), (17, ODD)):
         assert lib.dmoq_gated_ffn_backward(*(good[:i] + [v] + good[i + 1:]), None) == EINVAL, (i, v)
+    assert lib.dmoq_gated_ffn_backward(*(good[:8] + [(1 << 26) + 1] + good[9:]), None) == ESIZE
 
 
 def test_functions_refuse_cpu_tensors():

@@ -299,6 +299,37 @@ def test_ffn_empty_shapes_strides_and_refusals():
         double.sum().backward()                                      # once differentiable
 
 
+def test_ffn_with_saved_tensors_moved_and_from_other_threads():
+    """What is saved may come back from a hook laid out anew; calls may come from several threads and streams at once."""
+    import threading
+
+    x, wg, wu, wd, dy = ffn_inputs(90, 264, 136, torch.bfloat16, seed=8)
+    wide = torch.zeros(90, 400, dtype=torch.bfloat16, device=DEV)
+    wide[:, 64:328] = x
+    leaves = [wide[:, 64:328].requires_grad_(True)] + [v.requires_grad_(True) for v in (wg, wu, wd)]
+    want = torch.autograd.grad(dense.gated_feed_forward(*leaves), leaves, dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = dense.gated_feed_forward(*leaves)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, dy), want))
+    results = [None] * 4
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            mine = [v.detach().clone().requires_grad_(True) for v in leaves]
+            for _ in range(10):
+                results[i] = torch.autograd.grad(dense.gated_feed_forward(*mine), mine, dy)
+            torch.cuda.current_stream().synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    for r in results:
+        assert all(torch.equal(a, b) for a, b in zip(r, want))
+
+
 def test_ffn_infinities_and_nan_stay_in_their_rows():
     x, wg, wu, wd, _ = ffn_inputs(140, 264, 136, torch.bfloat16, seed=6)
     clean = dense.gated_feed_forward(x, wg, wu, wd)
