@@ -1,5 +1,6 @@
 // C entry points of the dense operators: argument checks, tensor maps, choice of the kernel.
 #include <algorithm>
+#include <cmath>
 
 #include "dense.cuh"
 
@@ -8,6 +9,7 @@ int dmoq_token_quant_launch(const void* x, int bf16, int T, int K, long long pit
 namespace dense {
 
 int tile_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, const Args& a, int splits, cudaStream_t s);
+int tile_blocks_at_once(int splits);
 int pair_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, const Args& a, cudaStream_t s);
 int pair_group(const Maps* maps, const Args* p, const bool* a_mn, int n_long, cudaStream_t s);
 
@@ -107,52 +109,97 @@ long long pair_tiles(const Product& p) {
 }
 long long steps_of(const Product& p) { return (long long)dmoq_ceil_div(p.args.K, p.kind == KIND_I8 ? 128 : 64) * p.args.segs; }
 
-// The kernel for a product.  Pairs of blocks need enough 256-wide tiles to go round (half the pairs; fewer tiles are faster
-// unpaired with K split: 512 x 4096 by 8192, 32 tiles, 22.4 us against 18.8).  Up to 128 tokens reading the weights is all
-// that counts; up to 256 it still beats 128-wide tiles (130 x 4096 by 8192: 27 us against 32), but not full pairs (130 x 5120 by
-// 27648: 90 us against 77).
-int run(const Product& p, cudaStream_t s) {
-  Maps maps;
-  const bool pair = pair_tiles(p) * 4 >= dmoq_sm_count();
-  if (p.args.M <= (pair ? 128 : kMidTokens) && !p.a_mn && !p.b_mn && p.args.segs == 1) {
-    const int es = p.kind == KIND_I8 ? 1 : 2, rows = is_dual(p.epi) ? 64 : 128;
-    const long long tiles = dmoq_ceil_div(p.args.N, rows), steps = steps_of(p);
-    // Up to two blocks an SM stream at once.  Below half the SMs a split pays from 2 steps a block on, above from 8: 32 tiles of
-    // 32 steps take 10.4 us in 4 parts and 11.6 in 8; 64 tiles of 64 steps 22.4 us in 2 and 19.3 in 4; 216 tiles of 80 steps
-    // 50 us whole and 56 in 2.
-    int splits = 1;
-    const int most = p.args.M <= 128 ? dmoq_sm_count() : dmoq_sm_count() / 2;
-    while (splits < 8 && tiles * splits <= most && steps >= splits * (tiles * splits * 2 < dmoq_sm_count() ? 4 : 16)) splits *= 2;
-    int rc = tma_ok(p.a[0], es) && tma_ok(p.b[0], es) ? make_map(&maps.b[0], p.a[0], es, mid_token_box(p.args.M)) : DMOQ_EINVAL;
-    if (rc == DMOQ_OK) rc = make_map(&maps.a[0], p.b[0], es, rows);
-    if (rc == DMOQ_OK && is_dual(p.epi)) rc = tma_ok(p.b[1], es) ? make_map(&maps.a[1], p.b[1], es, rows) : DMOQ_EINVAL;
-    return rc != DMOQ_OK ? rc : mid_product(p.kind, p.epi, maps, p.args, splits, s);
-  }
-  if (pair) {
-    const int rc = make_maps(maps, p, 128);
-    return rc != DMOQ_OK ? rc : pair_product(p.kind, p.a_mn, p.b_mn, p.epi, maps, pair_args(p), s);
-  }
-  const int cols = is_dual(p.epi) ? 64 : 128;
-  const long long tiles = (long long)dmoq_ceil_div(p.args.M, 128) * dmoq_ceil_div(p.args.N, cols), steps = steps_of(p);
-  int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= dmoq_sm_count() && steps >= splits * 8) splits *= 2;
-  const int rc = make_maps(maps, p, cols);
-  return rc != DMOQ_OK ? rc : tile_product(p.kind, p.a_mn, p.b_mn, p.epi, maps, p.args, splits, s);
+// What a product costs in each kernel, in microseconds, to choose among them: fits to measurements on a B200 of products
+// of 64 to 16384 rows by 512 to 5456 columns and 1 to 256 steps of K (a step is 128 bytes), about 15 % off at worst.  Whole
+// tiles go round the SMs, so a product that fills them badly in wide tiles may be better off in narrow ones or with K split:
+//                                            pairs    tiles (K in parts)
+//   300 x 4096 by K = 4096 (64 steps)        23.7     21.5 (2)     1000 x 4096, K = 4096    26.2     34.1 (1)
+//   1024 x 2048 by K = 16384 (256)           77.0     64.1 (2)     2048 x 2048, K = 16384   94.6    119.8 (1)
+//   257 x 1032 by K = 5456 (86)              31.1     13.0 (4)     1000 x 2728, K = 1032    12.1     20.3 (1)
+double pair_cost(const Product& p) {
+  const double rounds = std::ceil((double)pair_tiles(p) / (dmoq_sm_count() / 2));
+  return 4.6 + rounds * 0.30 * steps_of(p) + (rounds - 1) * 2.0;
+}
+double join_cost(int splits) { return splits == 1 ? 0.0 : splits == 2 ? 0.7 : splits == 4 ? 1.0 : 1.8; }
+double tile_cost(const Product& p, int splits) {
+  const double blocks = (double)dmoq_ceil_div(p.args.M, 128) * dmoq_ceil_div(p.args.N, is_dual(p.epi) ? 64 : 128) * splits;
+  const double steps = std::ceil((double)steps_of(p) / splits);
+  if (blocks <= tile_blocks_at_once(splits)) return 5.0 + 0.29 * steps + join_cost(splits);
+  const double rounds = std::ceil(blocks / (2 * tile_blocks_at_once(splits)));                             // two blocks an SM
+  return 2.0 + rounds * (5.0 + 0.45 * steps) + join_cost(splits);   // a round's start and end are not covered by the next
+}
+double mid_cost(const Product& p, int splits) {   // 129 to 256 tokens
+  const double blocks = (double)dmoq_ceil_div(p.args.N, is_dual(p.epi) ? 64 : 128) * splits;
+  return std::ceil(blocks / dmoq_sm_count()) * (5.0 + 0.38 * std::ceil((double)steps_of(p) / splits)) + join_cost(splits);
 }
 
-// Three independent products (MN-major B, plain outputs).  In one launch their tiles fill the SMs together, as long as no single
-// tile is longer than the share of the work that a pair of blocks gets; then that product is better split along K by itself.
-int run_three(const Product (&p)[3], cudaStream_t s) {
-  const int pairs = dmoq_sm_count() / 2;
-  long long total = 0, longest = 0, shortest = 1LL << 60;
-  for (const Product& q : p) {
-    total += pair_tiles(q) * steps_of(q);
-    longest = std::max(longest, steps_of(q));
-    shortest = std::min(shortest, steps_of(q));
+struct Choice {
+  enum Kernel { PAIR, TILE, MID } kernel;
+  int splits;
+  double cost;
+};
+Choice choose(const Product& p) {
+  const long long steps = steps_of(p);
+  Choice best = {Choice::PAIR, 1, pair_cost(p)};
+  for (int splits = 1; splits <= 8 && splits <= steps; splits *= 2) {
+    const double c = tile_cost(p, splits);
+    if (c < best.cost) best = {Choice::TILE, splits, c};
   }
-  if (longest * pairs * 4 > total * 5) {
-    for (const Product& q : p) {
-      const int rc = run(q, s);
+  if (p.args.M <= kMidTokens && !p.a_mn && !p.b_mn && p.args.segs == 1) {
+    if (p.args.M <= 128) {
+      // Reading the weights is all that counts.  Up to two blocks an SM stream at once.  Below half the SMs a split pays from
+      // 2 steps a block on, above from 8: 32 tiles of 32 steps take 10.4 us in 4 parts and 11.6 in 8; 64 tiles of 64 steps
+      // 22.4 us in 2 and 19.3 in 4; 216 tiles of 80 steps 50 us whole and 56 in 2.
+      const long long tiles = dmoq_ceil_div(p.args.N, is_dual(p.epi) ? 64 : 128);
+      int splits = 1;
+      while (splits < 8 && tiles * splits <= dmoq_sm_count() && steps >= splits * (tiles * splits * 2 < dmoq_sm_count() ? 4 : 16)) splits *= 2;
+      return {Choice::MID, splits, 0.0};
+    }
+    for (int splits = 1; splits <= 8 && splits <= steps; splits *= 2) {
+      const double c = mid_cost(p, splits);
+      if (c < best.cost) best = {Choice::MID, splits, c};
+    }
+  }
+  return best;
+}
+
+int run(const Product& p, const Choice& choice, cudaStream_t s) {
+  Maps maps;
+  int rc;
+  switch (choice.kernel) {
+    case Choice::PAIR:
+      rc = make_maps(maps, p, 128);
+      return rc != DMOQ_OK ? rc : pair_product(p.kind, p.a_mn, p.b_mn, p.epi, maps, pair_args(p), s);
+    case Choice::TILE:
+      rc = make_maps(maps, p, is_dual(p.epi) ? 64 : 128);
+      return rc != DMOQ_OK ? rc : tile_product(p.kind, p.a_mn, p.b_mn, p.epi, maps, p.args, choice.splits, s);
+    default: {
+      const int es = p.kind == KIND_I8 ? 1 : 2, rows = is_dual(p.epi) ? 64 : 128;
+      rc = tma_ok(p.a[0], es) && tma_ok(p.b[0], es) ? make_map(&maps.b[0], p.a[0], es, mid_token_box(p.args.M)) : DMOQ_EINVAL;
+      if (rc == DMOQ_OK) rc = make_map(&maps.a[0], p.b[0], es, rows);
+      if (rc == DMOQ_OK && is_dual(p.epi)) rc = tma_ok(p.b[1], es) ? make_map(&maps.a[1], p.b[1], es, rows) : DMOQ_EINVAL;
+      return rc != DMOQ_OK ? rc : mid_product(p.kind, p.epi, maps, p.args, choice.splits, s);
+    }
+  }
+}
+int run(const Product& p, cudaStream_t s) { return run(p, choose(p), s); }
+
+// Three independent products (MN-major B, plain outputs): in one launch their tiles fill the SMs together, which takes as long
+// as a pair's share of all steps, or the longest tile.
+int run_three(const Product (&p)[3], cudaStream_t s) {
+  long long total = 0, longest = 0, shortest = 1LL << 60;
+  Choice alone[3];
+  double apart = 0.0;
+  for (int i = 0; i < 3; ++i) {
+    alone[i] = choose(p[i]);
+    apart += alone[i].cost;
+    total += pair_tiles(p[i]) * steps_of(p[i]);
+    longest = std::max(longest, steps_of(p[i]));
+    shortest = std::min(shortest, steps_of(p[i]));
+  }
+  if (apart < 6.6 + 0.30 * std::max((double)total / (dmoq_sm_count() / 2), (double)longest)) {
+    for (int i = 0; i < 3; ++i) {
+      const int rc = run(p[i], alone[i], s);
       if (rc != DMOQ_OK) return rc;
     }
     return DMOQ_OK;

@@ -12,30 +12,35 @@ __device__ int g_dmoq_dense_status = 0;
 namespace dense {
 namespace {
 
-template <int BN>
-struct TileCfg {
-  static constexpr int kStageBytes = 128 * 128 + BN * 128;
-  static constexpr int kStages = BN == 256 ? 4 : 6;
-  static constexpr int kPitch = BN * 4 + 16;              // accumulator rows in shared memory: 16 bytes of padding against bank conflicts
-  static constexpr int kBar = kStages * kStageBytes;      // barriers after the stages
-  static constexpr int kSmem = kBar + 256 + 1024;
-  static_assert(128 * kPitch <= kBar, "the accumulator rows lie over the operand stages");
-};
+constexpr int BN = 128;                                   // columns of a tile
+constexpr int kStageBytes = 128 * 128 + BN * 128;
+// Six operand stages where the blocks have an SM each, three where two share one: what is on its way into an SM is the same, and
+// one block's products cover the other's start and end.
+constexpr int kMostStages = 6;
+constexpr int kPitch = BN * 4 + 16;                       // accumulator rows in shared memory: 16 bytes of padding against bank conflicts
+constexpr int smem_bytes(int stages) { return 1024 + 256 + stages * kStageBytes; }
+static_assert(128 * kPitch <= 3 * kStageBytes, "the accumulator rows lie over the operand stages");
+static_assert(2 * (smem_bytes(3) + 1024) <= 228 * 1024, "two blocks an SM");
 
-template <int KIND, bool AMN, bool BMN, int EPI, int BN>
-__global__ void __launch_bounds__(256, 1) dense_tile_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args a) {
-  using C = TileCfg<BN>;
+template <int KIND, bool AMN, bool BMN, int EPI>
+__global__ void __launch_bounds__(256, 2) dense_tile_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args a, int stages) {
   constexpr bool kDual = is_dual(EPI);
   constexpr int kCols = kDual ? BN / 2 : BN;              // output columns of the tile
   constexpr int kBK = KIND == KIND_I8 ? 128 : 64;         // elements of K in a step
-  constexpr int kStages = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t sb = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  auto stage_a = [&](uint32_t s) { return sb + s * C::kStageBytes; };
-  auto stage_b = [&](uint32_t s) { return sb + s * C::kStageBytes + 128 * 128; };
-  auto bar_full = [&](uint32_t s) { return sb + C::kBar + 8 * s; };
-  auto bar_empty = [&](uint32_t s) { return sb + C::kBar + 64 + 8 * s; };
-  const uint32_t bar_acc = sb + C::kBar + 128, tmem_slot = sb + C::kBar + 136, abort_flag = sb + C::kBar + 140;
+  const uint32_t bars = sb + stages * kStageBytes;
+  auto stage_a = [&](uint32_t s) { return sb + s * kStageBytes; };
+  auto stage_b = [&](uint32_t s) { return sb + s * kStageBytes + 128 * 128; };
+  auto bar_full = [&](uint32_t s) { return bars + 8 * s; };
+  auto bar_empty = [&](uint32_t s) { return bars + 64 + 8 * s; };
+  const uint32_t bar_acc = bars + 128, tmem_slot = bars + 136, abort_flag = bars + 140;
+  struct Ring {                                            // a position in the ring of stages and the parity of its use
+    uint32_t s = 0, parity = 0;
+    __device__ __forceinline__ void next(int stages) {
+      if (++s == (uint32_t)stages) s = 0, parity ^= 1;
+    }
+  };
 
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const uint32_t rank = cluster_rank(), splits = cluster_size();
@@ -47,7 +52,7 @@ __global__ void __launch_bounds__(256, 1) dense_tile_kernel(const __grid_constan
   const int it0 = (int)((long long)steps * rank / splits), it1 = (int)((long long)steps * (rank + 1) / splits);
 
   if (tid == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(bar_full(s), 1);
       mbar_init(bar_empty(s), 1);
     }
@@ -69,11 +74,12 @@ __global__ void __launch_bounds__(256, 1) dense_tile_kernel(const __grid_constan
   if (warp == 0) {
     if (lane == 0) {
       int done = 0;
-      for (int it = it0; it < it1; ++it, ++done) {
-        const uint32_t s = done % kStages;
-        if (done >= kStages && !mbar_wait(bar_empty(s), (done / kStages - 1) & 1, abort_flag, &g_dmoq_dense_status)) break;
+      Ring at;
+      for (int it = it0; it < it1; ++it, ++done, at.next(stages)) {
+        const uint32_t s = at.s;
+        if (done >= stages && !mbar_wait(bar_empty(s), at.parity ^ 1, abort_flag, &g_dmoq_dense_status)) break;
         const int seg = it >= seg_steps ? 1 : 0, k = (it - seg * seg_steps) * kBK;
-        mbar_arrive_expect_tx(bar_full(s), C::kStageBytes);
+        mbar_arrive_expect_tx(bar_full(s), kStageBytes);
         if (AMN) {
           tma_load(stage_a(s), &maps.a[seg], m0, k, bar_full(s));
           tma_load(stage_a(s) + 8192, &maps.a[seg], m0 + 64, k, bar_full(s));
@@ -91,7 +97,7 @@ __global__ void __launch_bounds__(256, 1) dense_tile_kernel(const __grid_constan
         }
       }
       // nothing may still be on its way into this block's shared memory when it is reused or the block ends (matters after an abort)
-      for (int j = done > kStages ? done - kStages : 0; j < done; ++j) mbar_wait_quiet(bar_full(j % kStages), (j / kStages) & 1);
+      for (int j = done > stages ? done - stages : 0; j < done; ++j) mbar_wait_quiet(bar_full(j % stages), (j / stages) & 1);
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -102,11 +108,13 @@ __global__ void __launch_bounds__(256, 1) dense_tile_kernel(const __grid_constan
       // 32 bytes of K an instruction: 32 bytes along a K-major row, sixteen 128-byte rows of an MN-major tile
       constexpr uint32_t step_a = AMN ? 128 : 2, step_b = BMN ? 128 : 2;
       uint32_t ready = 0;
+      Ring at;
       for (int done = 0; done < it1 - it0; ++done) {
-        const uint32_t s = done % kStages;
-        if (!ready && !mbar_wait(bar_full(s), (done / kStages) & 1, abort_flag, &g_dmoq_dense_status)) break;
+        const uint32_t s = at.s;
+        if (!ready && !mbar_wait(bar_full(s), at.parity, abort_flag, &g_dmoq_dense_status)) break;
         tc_fence_after();
-        ready = mbar_peek(bar_full((done + 1) % kStages), ((done + 1) / kStages) & 1);   // used after this step's products
+        at.next(stages);
+        ready = mbar_peek(bar_full(at.s), at.parity);      // used after this step's products
         const uint64_t da = operand_desc(stage_a(s), AMN ? 8192 : 16), db = operand_desc(stage_b(s), BMN ? 8192 : 16);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -130,7 +138,7 @@ __global__ void __launch_bounds__(256, 1) dense_tile_kernel(const __grid_constan
     if (flag_get(abort_flag)) mbar_wait_quiet(bar_acc, 0);
     tc_fence_after();
     const int w = warp - 4;
-    const uint32_t row = sb + (uint32_t)(w * 32 + lane) * C::kPitch;
+    const uint32_t row = sb + (uint32_t)(w * 32 + lane) * kPitch;
 #pragma unroll 1
     for (int c = 0; c < BN; c += 32) {
       uint32_t v[32];
@@ -150,25 +158,62 @@ __global__ void __launch_bounds__(256, 1) dense_tile_kernel(const __grid_constan
   if (splits > 1) cluster_sync();
 
   // join and finish: this block's rows of the tile
-  finish_rows<KIND, EPI, kCols>(a, sb, C::kPitch, 128 * rank / splits, 128 * (rank + 1) / splits, m0, n0, splits, tid);
+  finish_rows<KIND, EPI, kCols>(a, sb, kPitch, 128 * rank / splits, 128 * (rank + 1) / splits, m0, n0, splits, tid);
   if (splits > 1) cluster_sync();   // a block's shared memory lives until the others have read it
 }
 
-template <int KIND, bool AMN, bool BMN, int EPI, int BN>
+}  // namespace
+
+// Blocks of this kernel that run at once in clusters of `splits` (a power of two up to 8), an SM each: clusters do not fill
+// every processing cluster of the device, so this is less than there are SMs.  With three stages twice as many fit.
+int tile_blocks_at_once(int splits) {
+  static int known[64][4] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return dmoq_sm_count();
+  int log = 0;
+  while ((1 << log) < splits) ++log;
+  int& n = known[dev][log];
+  if (n == 0) {
+    auto* kernel = dense_tile_kernel<KIND_16, false, false, EPI_OUT>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(splits);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = smem_bytes(kMostStages);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = splits;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(kMostStages)) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters < 1) {
+      (void)cudaGetLastError();
+      clusters = dmoq_sm_count() / splits;
+    }
+    n = clusters * splits;
+  }
+  return n;
+}
+
+namespace {
+
+template <int KIND, bool AMN, bool BMN, int EPI>
 int launch(const Maps& maps, const Args& a, int splits, cudaStream_t s) {
-  using C = TileCfg<BN>;
   static DmoqOncePerDevice once;
   bool* configured = once.slot();
   if (configured == nullptr) return DMOQ_EDEVICE;
-  auto* kernel = dense_tile_kernel<KIND, AMN, BMN, EPI, BN>;
+  auto* kernel = dense_tile_kernel<KIND, AMN, BMN, EPI>;
   if (!*configured) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess) return DMOQ_ELAUNCH;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(kMostStages)) != cudaSuccess) return DMOQ_ELAUNCH;
     *configured = true;
   }
   constexpr int kCols = is_dual(EPI) ? BN / 2 : BN;
   const long long blocks = (long long)dmoq_ceil_div(a.M, 128) * dmoq_ceil_div(a.N, kCols) * splits;
   if (blocks > 0x7fffffffLL) return DMOQ_ESIZE;
-  return launch_overlapped(kernel, (unsigned)blocks, 256, C::kSmem, splits, s, maps, a);
+  const int stages = blocks <= tile_blocks_at_once(splits) ? kMostStages : 3;
+  return launch_overlapped(kernel, (unsigned)blocks, 256, smem_bytes(stages), splits, s, maps, a, stages);
 }
 
 }  // namespace
@@ -176,14 +221,14 @@ int launch(const Maps& maps, const Args& a, int splits, cudaStream_t s) {
 int tile_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, const Args& a, int splits, cudaStream_t s) {
   const int key = kind * 1000 + a_mn * 200 + b_mn * 100 + epi;
   switch (key) {
-    case EPI_OUT: return launch<KIND_16, false, false, EPI_OUT, 128>(maps, a, splits, s);
-    case EPI_SILU: return launch<KIND_16, false, false, EPI_SILU, 128>(maps, a, splits, s);
-    case EPI_SILU_SAVE: return launch<KIND_16, false, false, EPI_SILU_SAVE, 128>(maps, a, splits, s);
-    case 100 + EPI_OUT: return launch<KIND_16, false, true, EPI_OUT, 128>(maps, a, splits, s);
-    case 100 + EPI_GRAD: return launch<KIND_16, false, true, EPI_GRAD, 128>(maps, a, splits, s);
-    case 300 + EPI_OUT: return launch<KIND_16, true, true, EPI_OUT, 128>(maps, a, splits, s);
-    case 1000 + EPI_SCALE: return launch<KIND_I8, false, false, EPI_SCALE, 128>(maps, a, splits, s);
-    case 1000 + EPI_SILU: return launch<KIND_I8, false, false, EPI_SILU, 128>(maps, a, splits, s);
+    case EPI_OUT: return launch<KIND_16, false, false, EPI_OUT>(maps, a, splits, s);
+    case EPI_SILU: return launch<KIND_16, false, false, EPI_SILU>(maps, a, splits, s);
+    case EPI_SILU_SAVE: return launch<KIND_16, false, false, EPI_SILU_SAVE>(maps, a, splits, s);
+    case 100 + EPI_OUT: return launch<KIND_16, false, true, EPI_OUT>(maps, a, splits, s);
+    case 100 + EPI_GRAD: return launch<KIND_16, false, true, EPI_GRAD>(maps, a, splits, s);
+    case 300 + EPI_OUT: return launch<KIND_16, true, true, EPI_OUT>(maps, a, splits, s);
+    case 1000 + EPI_SCALE: return launch<KIND_I8, false, false, EPI_SCALE>(maps, a, splits, s);
+    case 1000 + EPI_SILU: return launch<KIND_I8, false, false, EPI_SILU>(maps, a, splits, s);
     default: return DMOQ_EINVAL;
   }
 }
