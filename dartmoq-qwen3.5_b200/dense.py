@@ -22,7 +22,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 
-_BF16, _FP16 = torch.bfloat16, torch.float16
+_BF16, _FP16, _FP32, _INT8 = torch.bfloat16, torch.float16, torch.float32, torch.int8
 _MAX_ROWS = 1 << 30
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
@@ -81,16 +81,16 @@ def _check_k8(k: int) -> None:
 
 def _weight8(w: torch.Tensor, scale: torch.Tensor, k: int, index: int, what: str) -> Tuple[torch.Tensor, torch.Tensor]:
     """The weight and its scales as the kernels take them."""
-    if w.dtype is not torch.int8 or scale.dtype is not torch.float32:
+    if w.dtype is not _INT8 or scale.dtype is not _FP32:
         raise TypeError(f"{what} must be int8 with an fp32 scale, got {w.dtype} and {scale.dtype}")
     shape = w.shape
     if len(shape) != 2 or shape[1] != k or shape[0] < 1:
         raise ValueError(f"{what} must have shape (outputs, {k}), got {tuple(shape)}")
     if scale.shape != shape[:1]:
         raise ValueError(f"{what} needs one scale a row: {shape[0]} rows, scales of shape {tuple(scale.shape)}")
-    if not (w.is_cuda and scale.is_cuda and w.get_device() == index and scale.get_device() == index):
+    if w.get_device() != index or scale.get_device() != index:      # -1 on the CPU
         raise ValueError(f"{what} and its scale must be on cuda:{index}")
-    return _packed(w), scale.contiguous()
+    return _packed(w), scale if scale.is_contiguous() else scale.contiguous()
 
 
 def _bias_ptr(bias: Optional[torch.Tensor], n: int, dtype: torch.dtype, index: int):
@@ -259,9 +259,8 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
                          f"{tuple(w_up.shape)}, {tuple(w_down.shape)}")
     if hidden < 8 or inter < 8 or (hidden | inter) & 7:
         raise ValueError(f"hidden and intermediate sizes must be multiples of 8, got {hidden} and {inter}")
-    for w in (w_gate, w_up, w_down):
-        if not w.is_cuda or w.get_device() != index:
-            raise ValueError(f"all weights must be on cuda:{index}")
+    if w_gate.get_device() != index or w_up.get_device() != index or w_down.get_device() != index:
+        raise ValueError(f"all weights must be on cuda:{index}")
     w_gate, w_up, w_down = _packed(w_gate), _packed(w_up), _packed(w_down)
     rows = x if x.dim() == 2 else x.reshape(-1, hidden)
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):

@@ -504,3 +504,36 @@ def test_int8_results_do_not_depend_on_the_batch():
         assert torch.equal(dense.int8_linear(x[:t], w, ws, b), lin[:t]), t
         assert torch.equal(dense.int8_gated_linear(x[:t], w, ws, w2, ws2), gated[:t]), t
         assert torch.equal(dense.int8_linear(x[:t], w[:500], ws[:500]), dense.int8_linear(x, w[:500], ws[:500])[:t]), t
+
+
+FIRST_USE = """
+import sys
+sys.path.insert(0, %r)
+import torch
+from dartmoq_b200 import dense
+torch.manual_seed(0)
+w, s = torch.randint(-100, 100, (640, 512), device="cuda", dtype=torch.int8), torch.rand(640, device="cuda")
+f = [torch.randn(640, 512, device="cuda").bfloat16() * 0.05 for _ in range(2)] + [torch.randn(512, 640, device="cuda").bfloat16() * 0.05]
+xs = [torch.randn(t, 512, device="cuda").bfloat16() for t in (4, 40, 300, 3000)]
+work = lambda x: (dense.int8_linear(x, w, s), dense.int8_gated_linear(x, w, s, w, s), dense.gated_feed_forward(x, *f))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = [work(x) for x in xs]
+graph.replay()
+torch.cuda.synchronize()
+for x, g in zip(xs, got):
+    assert all(torch.equal(a, b) for a, b in zip(work(x), g)), x.shape
+print("same")
+"""
+
+
+def test_first_use_inside_a_capture():
+    """A fresh process whose first call of every kernel is made while a stream is being captured."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_USE % root], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "same", r.stderr[-2000:]
