@@ -98,9 +98,11 @@ EXPORTS = {
     "dmoq_int8_gated_gemm": (C.c_int, [C.c_void_p] * 6 + [C.c_int32] * 4 + [C.c_void_p] * 2),
     "dmoq_int8_gated_linear": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64] + [C.c_void_p] * 4 + [C.c_int32] * 3
                                + [C.c_void_p] * 3),
-    "dmoq_gated_ffn": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64] + [C.c_void_p] * 3 + [C.c_int32] * 3 + [C.c_void_p] * 4),
+    "dmoq_gated_ffn": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64] + [C.c_void_p] * 3 + [C.c_int32] * 3
+                       + [C.c_void_p, C.c_int64] + [C.c_void_p] * 3),
     "dmoq_gated_ffn_backward": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_int64] + [C.c_void_p] * 3
-                                + [C.c_int32] * 3 + [C.c_void_p] * 8),
+                                + [C.c_int32] * 3 + [C.c_void_p, C.c_int64] + [C.c_void_p] * 2 + [C.c_int64]
+                                + [C.c_void_p] * 5),
 }
 
 _lib = None

@@ -43,7 +43,8 @@ struct Args {
   const uint16_t* bias;     // 8-bit, optional, type of the output
   const uint16_t* in[3];    // the saved planes
   uint16_t* out[4];
-  long long ld_in, ld_out;  // row pitches in elements
+  long long ld_in, ld_out;  // row pitches in elements (ld_in: of the planes that are read)
+  long long ld_saved;       // of the planes that are written, out[1] to out[3]
 };
 
 // The arithmetic of the epilogues, with its roundings spelled out (no contraction left to the compiler), so that an 8-bit result
@@ -128,7 +129,7 @@ __device__ __forceinline__ void finish_rows(const Args& a, uint32_t sums, uint32
       } else {
         lo = pack16(o[e < 3 ? e : 0][0], o[e < 3 ? e : 0][1], a.bf16), hi = pack16(o[e < 3 ? e : 0][2], o[e < 3 ? e : 0][3], a.bf16);
       }
-      uint16_t* dst = a.out[e] + at_out;
+      uint16_t* dst = a.out[e] + (EPI == EPI_SILU_SAVE && e > 0 ? row * a.ld_saved + col : at_out);
       if (a.vec) {
         *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
       } else {

@@ -4,7 +4,8 @@
 
 #include "dense.cuh"
 
-int dmoq_token_quant_launch(const void* x, int bf16, int T, int K, long long pitch, int8_t* codes, float* scales, cudaStream_t s);
+int dmoq_token_quant_launch(const void* x, int bf16, int T, int K, long long pitch, int8_t* codes, long long code_pitch, float* scales,
+                            cudaStream_t s);
 
 namespace dense {
 
@@ -249,11 +250,11 @@ int check_ffn(int T, int H, int I) {
 
 // The products of `codes`, or of the 16-bit rows x (pitch in elements), whose codes then go into `codes` / `scales` first unless
 // the kernel makes them itself.
-int int8_product(const void* x, long long x_pitch, int8_t* codes, float* scales, const int8_t* w0, const float* s0, const int8_t* w1,
+int int8_product(const void* x, long long x_pitch, int8_t* codes, long long code_pitch, float* scales, const int8_t* w0, const float* s0, const int8_t* w1,
                  const float* s1, const void* bias, int bf16, int T, int N, int K, void* out, cudaStream_t s) {
   const bool few = few_tokens(T, (long long)N * K * (w1 ? 2 : 1)), fuse = x != nullptr && few_can_fuse(T, K, N, w1 != nullptr);   // fuse implies few
   if (x != nullptr && !fuse) {
-    const int rc = dmoq_token_quant_launch(x, bf16, T, K, x_pitch, codes, scales, s);
+    const int rc = dmoq_token_quant_launch(x, bf16, T, K, x_pitch, codes, code_pitch, scales, s);
     if (rc != DMOQ_OK) return rc;
   }
   Product p;
@@ -266,8 +267,8 @@ int int8_product(const void* x, long long x_pitch, int8_t* codes, float* scales,
   a.out[0] = static_cast<uint16_t*>(out);
   a.ld_out = N;
   a.vec = vec4(out, N, N);
-  if (few) return few_product(KIND_I8, p.epi, fuse ? x : codes, fuse ? 2 * x_pitch : K, w0, w1, a, s);
-  p.a[0] = {codes, T, K, K};
+  if (few) return few_product(KIND_I8, p.epi, fuse ? x : codes, fuse ? 2 * x_pitch : code_pitch, w0, w1, a, s);
+  p.a[0] = {codes, T, K, code_pitch};
   p.b[0] = {w0, N, K, K};
   if (w1) p.b[1] = {w1, N, K, K};
   return run(p, s);
@@ -284,7 +285,7 @@ extern "C" int dmoq_token_quant(const void* x, int32_t is_bf16, int32_t T, int32
   if (T > kMaxDim) return DMOQ_ESIZE;
   if (T == 0) return DMOQ_OK;
   DMOQ_CHECK_ARG(quant_ok(x, x_pitch, K, codes, scales));
-  return dmoq_token_quant_launch(x, is_bf16, T, K, x_pitch, codes, scales, static_cast<cudaStream_t>(stream));
+  return dmoq_token_quant_launch(x, is_bf16, T, K, x_pitch, codes, K, scales, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int dmoq_int8_gemm(const int8_t* codes, const float* scales, const int8_t* w, const float* w_scale, const void* bias,
@@ -292,7 +293,7 @@ extern "C" int dmoq_int8_gemm(const int8_t* codes, const float* scales, const in
   const int rc = check_sizes8(T, N, K);
   if (rc != DMOQ_OK || T == 0) return rc;
   DMOQ_CHECK_ARG(usable(codes) && scales && weight8_ok(w, w_scale) && out);
-  return int8_product(nullptr, 0, const_cast<int8_t*>(codes), const_cast<float*>(scales), w, w_scale, nullptr, nullptr, bias, is_bf16, T, N, K,
+  return int8_product(nullptr, 0, const_cast<int8_t*>(codes), K, const_cast<float*>(scales), w, w_scale, nullptr, nullptr, bias, is_bf16, T, N, K,
                       out, static_cast<cudaStream_t>(stream));
 }
 
@@ -302,14 +303,22 @@ extern "C" int dmoq_int8_gated_gemm(const int8_t* codes, const float* scales, co
   const int rc = check_sizes8(T, I, K);
   if (rc != DMOQ_OK || T == 0) return rc;
   DMOQ_CHECK_ARG(usable(codes) && scales && weight8_ok(w_gate, gate_scale) && weight8_ok(w_up, up_scale) && out);
-  return int8_product(nullptr, 0, const_cast<int8_t*>(codes), const_cast<float*>(scales), w_gate, gate_scale, w_up, up_scale, nullptr, is_bf16,
+  return int8_product(nullptr, 0, const_cast<int8_t*>(codes), K, const_cast<float*>(scales), w_gate, gate_scale, w_up, up_scale, nullptr, is_bf16,
                       T, I, K, out, static_cast<cudaStream_t>(stream));
 }
 
-// scratch of the two calls below: the codes, then the scales (T K is a multiple of 16)
+namespace {
+// Scratch of the two calls below: the codes, then the scales.  A row of codes starts on a 128-byte line whatever K is: a box row
+// that straddles two lines costs the L2 a quarter more sectors (1111 tokens, 10936 x 4112 twice: 98 us became 83).
+long long scratch_pitch(int K) { return (K + 127) / 128 * 128; }
+float* scratch_scales(void* scratch, int T, int K) {
+  return reinterpret_cast<float*>(static_cast<char*>(scratch) + (size_t)T * scratch_pitch(K));
+}
+}  // namespace
+
 extern "C" size_t dmoq_int8_scratch_bytes(int32_t T, int32_t N, int32_t K, int32_t gated) {
   if (check_sizes8(T, N, K) != DMOQ_OK || few_can_fuse(T, K, N, gated != 0)) return 0;
-  return (size_t)T * K + (size_t)T * sizeof(float);
+  return (size_t)T * scratch_pitch(K) + (size_t)T * sizeof(float);
 }
 
 extern "C" int dmoq_int8_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w, const float* w_scale, const void* bias,
@@ -317,8 +326,7 @@ extern "C" int dmoq_int8_linear(const void* x, int32_t is_bf16, int64_t x_pitch,
   const int rc = check_sizes8(T, N, K);
   if (rc != DMOQ_OK || T == 0) return rc;
   DMOQ_CHECK_ARG(rows_usable(x, x_pitch, K) && weight8_ok(w, w_scale) && out && (few_can_fuse(T, K, N, false) || usable(scratch)));
-  int8_t* codes = static_cast<int8_t*>(scratch);
-  return int8_product(x, x_pitch, codes, reinterpret_cast<float*>(codes + (size_t)T * K), w, w_scale, nullptr, nullptr, bias, is_bf16, T, N, K,
+  return int8_product(x, x_pitch, static_cast<int8_t*>(scratch), scratch_pitch(K), scratch_scales(scratch, T, K), w, w_scale, nullptr, nullptr, bias, is_bf16, T, N, K,
                       out, static_cast<cudaStream_t>(stream));
 }
 
@@ -329,16 +337,15 @@ extern "C" int dmoq_int8_gated_linear(const void* x, int32_t is_bf16, int64_t x_
   if (rc != DMOQ_OK || T == 0) return rc;
   DMOQ_CHECK_ARG(rows_usable(x, x_pitch, K) && weight8_ok(w_gate, gate_scale) && weight8_ok(w_up, up_scale) && out &&
                  (few_can_fuse(T, K, I, true) || usable(scratch)));
-  int8_t* codes = static_cast<int8_t*>(scratch);
-  return int8_product(x, x_pitch, codes, reinterpret_cast<float*>(codes + (size_t)T * K), w_gate, gate_scale, w_up, up_scale, nullptr, is_bf16, T,
+  return int8_product(x, x_pitch, static_cast<int8_t*>(scratch), scratch_pitch(K), scratch_scales(scratch, T, K), w_gate, gate_scale, w_up, up_scale, nullptr, is_bf16, T,
                       I, K, out, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate, const void* w_up, const void* w_down,
-                              int32_t T, int32_t H, int32_t I, void* h, void* saved, void* y, void* stream) {
+                              int32_t T, int32_t H, int32_t I, void* h, int64_t h_pitch, void* saved, void* y, void* stream) {
   const int size = check_ffn(T, H, I);
   if (size != DMOQ_OK || T == 0) return size;
-  DMOQ_CHECK_ARG(rows_usable(x, x_pitch, H) && usable(w_gate) && usable(w_up) && usable(w_down) && usable(h) && usable(y));
+  DMOQ_CHECK_ARG(rows_usable(x, x_pitch, H) && usable(w_gate) && usable(w_up) && usable(w_down) && rows_usable(h, h_pitch, I) && usable(y));
   DMOQ_CHECK_ARG(aligned16(saved));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   Product up;
@@ -349,22 +356,23 @@ extern "C" int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, c
   up.args.M = T, up.args.N = I, up.args.K = H, up.args.segs = 1, up.args.bf16 = is_bf16, up.args.vec = 1;
   up.args.out[0] = static_cast<uint16_t*>(h);
   for (int e = 0; saved && e < 3; ++e) up.args.out[1 + e] = static_cast<uint16_t*>(saved) + e * (size_t)T * I;
-  up.args.ld_out = I;
+  up.args.ld_out = h_pitch;
+  up.args.ld_saved = I;
   const long long w_bytes = 2LL * H * I;
   int rc = few_tokens(T, 2 * w_bytes) && !saved ? few_product(KIND_16, EPI_SILU, x, 2 * x_pitch, w_gate, w_up, up.args, s) : run(up, s);
   if (rc != DMOQ_OK) return rc;
   Product down;
-  down.a[0] = {h, T, I, I};
+  down.a[0] = {h, T, I, h_pitch};
   down.b[0] = {w_down, H, I, I};
   down.args.M = T, down.args.N = H, down.args.K = I, down.args.segs = 1, down.args.bf16 = is_bf16, down.args.vec = 1;
   down.args.out[0] = static_cast<uint16_t*>(y);
   down.args.ld_out = H;
-  return few_tokens(T, w_bytes) ? few_product(KIND_16, EPI_OUT, h, 2 * (long long)I, w_down, nullptr, down.args, s) : run(down, s);
+  return few_tokens(T, w_bytes) ? few_product(KIND_16, EPI_OUT, h, 2 * h_pitch, w_down, nullptr, down.args, s) : run(down, s);
 }
 
 extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate,
                                        const void* w_up, const void* w_down, int32_t T, int32_t H, int32_t I, const void* h,
-                                       const void* saved, void* d_gate_up, void* dx, void* dw_gate, void* dw_up,
+                                       int64_t h_pitch, const void* saved, void* d_gate_up, int64_t d_pitch, void* dx, void* dw_gate, void* dw_up,
                                        void* dw_down, void* stream) {
   const int size = check_ffn(T, H, I);
   if (size != DMOQ_OK) return size;
@@ -380,8 +388,8 @@ extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const v
   const bool inner = dx || dw_gate || dw_up;    // anything behind the hidden values
   DMOQ_CHECK_ARG(aligned16(dx) && aligned16(dw_gate) && aligned16(dw_up) && aligned16(dw_down));
   DMOQ_CHECK_ARG(!(inner || dw_down) || rows_usable(dy, dy_pitch, H));
-  DMOQ_CHECK_ARG(!dw_down || usable(h));
-  DMOQ_CHECK_ARG(!inner || (usable(w_down) && usable(saved) && usable(d_gate_up)));
+  DMOQ_CHECK_ARG(!dw_down || rows_usable(h, h_pitch, I));
+  DMOQ_CHECK_ARG(!inner || (usable(w_down) && usable(saved) && rows_usable(d_gate_up, d_pitch, 2 * I)));
   DMOQ_CHECK_ARG(!dx || (usable(w_gate) && usable(w_up)));
   DMOQ_CHECK_ARG(!(dw_gate || dw_up) || rows_usable(x, x_pitch, H));
   uint16_t* dg = static_cast<uint16_t*>(d_gate_up);
@@ -397,7 +405,7 @@ extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const v
     p.args.ld_in = I;
     p.args.out[0] = dg;
     p.args.out[1] = dg + I;
-    p.args.ld_out = 2 * (long long)I;
+    p.args.ld_out = d_pitch;
     if ((rc = run(p, s)) != DMOQ_OK) return rc;
   }
   Product px, pg, pd;   // dx, dw_gate and dw_up, dw_down
@@ -406,11 +414,10 @@ extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const v
     p.args.out[0] = static_cast<uint16_t*>(out);
     p.args.ld_out = N;
   };
-  const long long dg_pitch = 2 * (long long)I;
   if (dx) {             // dg Wg + du Wu: one sum over two K segments
     px.b_mn = true;
-    px.a[0] = {dg, T, I, dg_pitch};
-    px.a[1] = {dg + I, T, I, dg_pitch};
+    px.a[0] = {dg, T, I, d_pitch};
+    px.a[1] = {dg + I, T, I, d_pitch};
     px.b[0] = {w_gate, I, H, H};
     px.b[1] = {w_up, I, H, H};
     output(px, T, H, I, 2, dx);
@@ -423,8 +430,8 @@ extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const v
   };
   const Matrix xm = {x, T, H, x_pitch};
   const bool joined = dw_gate && dw_up && static_cast<char*>(dw_up) == static_cast<char*>(dw_gate) + w_bytes;
-  if (joined) weight_grad(pg, {dg, T, dg_pitch, dg_pitch}, xm, dw_gate);   // one product for both halves
-  if (dw_down) weight_grad(pd, {dy, T, H, dy_pitch}, {h, T, I, I}, dw_down);
+  if (joined) weight_grad(pg, {dg, T, 2 * (long long)I, d_pitch}, xm, dw_gate);   // one product for both halves
+  if (dw_down) weight_grad(pd, {dy, T, H, dy_pitch}, {h, T, I, h_pitch}, dw_down);
   if (dx && joined && dw_down) {
     const Product all[3] = {px, pg, pd};
     return run_three(all, s);
@@ -435,11 +442,11 @@ extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const v
   } else {
     Product p;
     if (dw_gate) {
-      weight_grad(p, {dg, T, I, dg_pitch}, xm, dw_gate);
+      weight_grad(p, {dg, T, I, d_pitch}, xm, dw_gate);
       if ((rc = run(p, s)) != DMOQ_OK) return rc;
     }
     if (dw_up) {
-      weight_grad(p, {dg + I, T, I, dg_pitch}, xm, dw_up);
+      weight_grad(p, {dg + I, T, I, d_pitch}, xm, dw_up);
       if ((rc = run(p, s)) != DMOQ_OK) return rc;
     }
   }

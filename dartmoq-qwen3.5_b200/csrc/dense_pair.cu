@@ -344,13 +344,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) dense_p
           for (int j = 0; j < 4; ++j) st_shared_v4(line + ((j ^ swz) << 4), o[p][4 * j], o[p][4 * j + 1], o[p][4 * j + 2], o[p][4 * j + 3]);
           __syncwarp();                                    // also: what this unit held two outputs ago has been read
           if (a.vec) {
+            const long long ld = EPI == EPI_SILU_SAVE && p > 0 ? a.ld_saved : a.ld_out;
             const int q = lane & 3, col = col0 + 8 * q;    // 16 bytes a thread: eight rows of 64 bytes an instruction
-            uint16_t* dst = a.out[p] + (long long)(row0 + (lane >> 2)) * a.ld_out + col;
+            uint16_t* dst = a.out[p] + (row0 + (lane >> 2)) * ld + col;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const int at = 8 * r + (lane >> 2);
               const uint4 val = ld_shared_v4(unit + at * 64 + ((q ^ ((at >> 1) & 3)) << 4));
-              if (row0 + at < a.M && col < a.N) *reinterpret_cast<uint4*>(dst + 8 * r * a.ld_out) = val;
+              if (row0 + at < a.M && col < a.N) *reinterpret_cast<uint4*>(dst + 8 * r * ld) = val;
             }
           } else {                                         // rows that are not 16-byte aligned: 64-byte runs of a row at a time
             for (int r = 0; r < 32 && row0 + r < a.M; ++r) {

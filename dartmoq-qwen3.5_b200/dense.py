@@ -198,11 +198,11 @@ def int8_gated_linear(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.T
 def _ffn_forward(x: torch.Tensor, t: int, pitch: int, wg: torch.Tensor, wu: torch.Tensor, wd: torch.Tensor, save: bool):
     """y, and the hidden values h; with ``save`` also what the gradients need of them."""
     hidden, inter = wd.shape
-    h = x.new_empty((t, inter))
+    h = x.new_empty((t, (inter + 63) & -64))       # rows on whole 128-byte lines
     saved = x.new_empty((3, t, inter), dtype=torch.int16) if save else None
     y = x.new_empty((t, hidden))
     _call("dmoq_gated_ffn", x.get_device(), x.data_ptr(), x.dtype is _BF16, pitch, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), t, hidden,
-          inter, h.data_ptr(), _ptr(saved), y.data_ptr())
+          inter, h.data_ptr(), h.shape[1], _ptr(saved), y.data_ptr())
     return y, h, saved
 
 
@@ -231,7 +231,8 @@ class _GatedFeedForward(torch.autograd.Function):
         x, _, x_pitch = _rows(x, hidden)
         wg, wu, wd = _packed(wg), _packed(wu), _packed(wd)
         h, saved = h if h is None else _packed(h), saved if saved is None else _packed(saved)
-        dgu = x.new_empty((t, 2 * inter)) if need_x or need_g or need_u else None
+        d_pitch = (2 * inter + 63) & -64
+        dgu = x.new_empty((t, d_pitch)) if need_x or need_g or need_u else None
         dx = x.new_empty((t, hidden)) if need_x else None
         # the two halves of one buffer: one product computes both
         dw = x.new_empty((int(need_g) + int(need_u), inter, hidden)) if need_g or need_u else None
@@ -239,7 +240,8 @@ class _GatedFeedForward(torch.autograd.Function):
         dwu = dw[-1] if need_u else None
         dwd = x.new_empty((hidden, inter)) if need_d else None
         _call("dmoq_gated_ffn_backward", x.get_device(), dy.data_ptr(), dy_pitch, x.data_ptr(), x.dtype is _BF16, x_pitch, wg.data_ptr(),
-              wu.data_ptr(), wd.data_ptr(), t, hidden, inter, _ptr(h), _ptr(saved), _ptr(dgu), _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd))
+              wu.data_ptr(), wd.data_ptr(), t, hidden, inter, _ptr(h), 0 if h is None else h.shape[1], _ptr(saved),
+              _ptr(dgu), d_pitch, _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd))
         return dx, dwg, dwu, dwd
 
 

@@ -387,15 +387,16 @@ size_t dmoq_int8_scratch_bytes(int32_t T, int32_t N, int32_t K, int32_t gated);
  * Gated feed-forward block: h = silu(x w_gate^T) * (x w_up^T), y = h w_down^T; x, y (T, H), w_gate and w_up (I, H), w_down (H, I),
  * h (T, I); H and I multiples of 8.  saved (optional), three planes (T, I) of 16 bits, receives what the gradients need: the upper
  * 24 bits of the 32-bit silu(g) and u silu'(g) (upper halves in planes 0 and 1, the next eight bits of both in plane 2).
- * backward (at most 2^26 tokens): dh = dy w_down, dg = dh * u silu'(g), du = dh * silu(g); d_gate_up (T, 2 I) scratch = [dg | du];
+ * backward (at most 2^26 tokens): dh = dy w_down, dg = dh * u silu'(g), du = dh * silu(g); d_gate_up (T, 2 I) scratch = [dg | du].  Pitches of h and
+ * d_gate_up that are multiples of 64 keep their rows on whole 128-byte lines;
  *   dx = dg w_gate + du w_up, dw_gate = dg^T x, dw_up = du^T x, dw_down = dy^T h.  Outputs that are NULL are not computed, and
  *   what only they need may be NULL too.  dw_up = dw_gate + H * I elements lets one product compute both.
  */
 int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate, const void* w_up, const void* w_down,
-                   int32_t T, int32_t H, int32_t I, void* h, void* saved, void* y, void* stream);
+                   int32_t T, int32_t H, int32_t I, void* h, int64_t h_pitch, void* saved, void* y, void* stream);
 int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate,
-                            const void* w_up, const void* w_down, int32_t T, int32_t H, int32_t I, const void* h, const void* saved,
-                            void* d_gate_up, void* dx, void* dw_gate, void* dw_up, void* dw_down, void* stream);
+                            const void* w_up, const void* w_down, int32_t T, int32_t H, int32_t I, const void* h, int64_t h_pitch,
+                            const void* saved, void* d_gate_up, int64_t d_pitch, void* dx, void* dw_gate, void* dw_up, void* dw_down, void* stream);
 
 #ifdef __cplusplus
 }

@@ -48,28 +48,29 @@ def test_int8_products_refuse():
 
 def test_int8_scratch_size():
     f = _lib.load().dmoq_int8_scratch_bytes
-    assert f(40, 33, 128, 0) == 40 * 128 + 40 * 4 and f(1000, 1, 131056, 1) == 1000 * 131056 + 4000
+    assert f(40, 33, 128, 0) == 40 * 128 + 40 * 4 and f(1000, 1, 131056, 1) == 1000 * 131072 + 4000   # whole 128-byte lines
     assert f(0, 33, 128, 0) == 0 and f(1, 33, 128, 1) == 0 and f(8, 512, 1024, 0) == 0   # none; few: the product makes the codes
     assert f(8, 64, 8192, 0) == 8 * 8192 + 32 and f(1, 8, 65536, 0) == 65536 + 4         # few, but too long for that
-    assert f(1, 16384, 1024, 0) == 0 and f(1, 16400, 1024, 0) == 1028 and f(1, 16384, 1024, 1) == 1028   # or too many blocks
+    assert f(1, 16384, 1024, 0) == 0 and f(20, 8, 16, 1) == 20 * 132 and f(1, 16400, 1024, 0) == 1028 and f(1, 16384, 1024, 1) == 1028   # or too many blocks
     assert f(9, 33, 128, 0) == 9 * 128 + 36
     assert f(4, 33, 100, 0) == 0 and f(-1, 33, 128, 0) == 0                              # refused by the calls themselves
 
 
 def test_gated_ffn_refuses():
     lib = _lib.load()
-    good = [P, 1, 64, P, P, P, 4, 64, 32, P, None, P]
+    good = [P, 1, 64, P, P, P, 4, 64, 32, P, 64, None, P]
     assert lib.dmoq_gated_ffn(*(good[:6] + [0] + good[7:]), None) == OK
-    for i in (0, 3, 4, 5, 9, 11):
+    for i in (0, 3, 4, 5, 9, 12):
         assert lib.dmoq_gated_ffn(*(good[:i] + [None] + good[i + 1:]), None) == EINVAL, i
-    for i, v in ((2, 60), (2, 68), (7, 60), (7, 0), (8, 12), (8, 0), (6, -4), (10, ODD), (0, ODD), (3, ODD), (4, ODD), (5, ODD),
-                 (9, ODD), (11, ODD)):
+    for i, v in ((2, 60), (2, 68), (7, 60), (7, 0), (8, 12), (8, 0), (6, -4), (11, ODD), (10, 24), (10, 36), (0, ODD), (3, ODD), (4, ODD), (5, ODD),
+                 (9, ODD), (12, ODD)):
         assert lib.dmoq_gated_ffn(*(good[:i] + [v] + good[i + 1:]), None) == EINVAL, (i, v)
-    #       dy pitch x bf pitch wg wu wd  T   H   I  h saved dgu dx dwg dwu dwd
-    good = [P, 64, P, 1, 64, P, P, P, 4, 64, 32, P, P, P, P, P, P, P]
-    for i in (0, 2, 5, 6, 7, 11, 12, 13):
+    #       dy pitch x bf pitch wg wu wd  T   H   I  h pitch saved dgu pitch dx dwg dwu dwd
+    good = [P, 64, P, 1, 64, P, P, P, 4, 64, 32, P, 32, P, P, 64, P, P, P, P]
+    for i in (0, 2, 5, 6, 7, 11, 13, 14):
         assert lib.dmoq_gated_ffn_backward(*(good[:i] + [None] + good[i + 1:]), None) == EINVAL, i
-    for i, v in ((1, 60), (4, 60), (9, 4), (10, 12), (0, ODD), (2, ODD), (11, ODD), (12, ODD), (13, ODD), (14, ODD), (15, ODD), (17, ODD)):
+    for i, v in ((1, 60), (4, 60), (9, 4), (10, 12), (0, ODD), (2, ODD), (11, ODD), (12, 24), (13, ODD), (14, ODD), (15, 56), (15, 68),
+                 (16, ODD), (17, ODD), (19, ODD)):
         assert lib.dmoq_gated_ffn_backward(*(good[:i] + [v] + good[i + 1:]), None) == EINVAL, (i, v)
     assert lib.dmoq_gated_ffn_backward(*(good[:8] + [(1 << 26) + 1] + good[9:]), None) == ESIZE
 

@@ -363,8 +363,8 @@ def test_outputs_stay_inside_their_memory():
     hid, saved, y = pad(t, i), pad(3 * t, i), pad(t, h)
     dgu, dx, dw, dwd = pad(t, 2 * i), pad(t, h), pad(2 * i, h), pad(h, i)
     q = lambda v: C.c_void_p(v[1].data_ptr())  # noqa: E731
-    _lib.check(lib.dmoq_gated_ffn(p(x), 1, h, p(wg), p(wu), p(wd), t, h, i, q(hid), q(saved), q(y), None), "ffn")
-    _lib.check(lib.dmoq_gated_ffn_backward(p(dy), h, p(x), 1, h, p(wg), p(wu), p(wd), t, h, i, q(hid), q(saved), q(dgu), q(dx), q(dw),
+    _lib.check(lib.dmoq_gated_ffn(p(x), 1, h, p(wg), p(wu), p(wd), t, h, i, q(hid), i, q(saved), q(y), None), "ffn")
+    _lib.check(lib.dmoq_gated_ffn_backward(p(dy), h, p(x), 1, h, p(wg), p(wu), p(wd), t, h, i, q(hid), i, q(saved), q(dgu), 2 * i, q(dx), q(dw),
                                            C.c_void_p(dw[1 + i].data_ptr()), q(dwd), None), "ffn backward")
     torch.cuda.synchronize()
     for v in (hid, saved, y, dgu, dx, dw, dwd):
@@ -372,7 +372,7 @@ def test_outputs_stay_inside_their_memory():
     R.close(dw[1:1 + 2 * i], torch.cat([R.ffn_grads(x, wg, wu, wd, dy)[k] for k in ("dw_gate", "dw_up")]), 2, "dw")
     # the gradients of the two projections in memory that is not adjacent: two products
     a, b = pad(i, h), pad(i, h)
-    _lib.check(lib.dmoq_gated_ffn_backward(p(dy), h, p(x), 1, h, None, None, p(wd), t, h, i, None, q(saved), q(dgu), None, q(a), q(b),
+    _lib.check(lib.dmoq_gated_ffn_backward(p(dy), h, p(x), 1, h, None, None, p(wd), t, h, i, None, 0, q(saved), q(dgu), 2 * i, None, q(a), q(b),
                                            None, None), "ffn backward")
     torch.cuda.synchronize()
     assert torch.equal(a[1:-1], dw[1:1 + i]) and torch.equal(b[1:-1], dw[1 + i:1 + 2 * i])
