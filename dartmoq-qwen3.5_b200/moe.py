@@ -310,6 +310,7 @@ class _Engine:
         self.E_v = self.E * self.mult
         self.k_v = self.top_k * self.mult
 
+        self.shared_expert = m.shared_expert      # another one assigned later makes a new engine
         shared_packs = m._shared_packs()
         self.has_shared = shared_packs is not None
         self.shared_torch = (m.shared_expert is not None and m.shared_expert_gate is not None
@@ -859,7 +860,7 @@ class WxA16BitPartitionedGroupMoE(nn.Module):
 
     def _get_engine(self, device) -> _Engine:
         eng = self._engine
-        if eng is None or eng.device != device:
+        if eng is None or eng.device != device or eng.shared_expert is not self.shared_expert:
             eng = _Engine(self, device)
             self._engine = eng
             self._graphs = None

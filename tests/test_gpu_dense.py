@@ -458,7 +458,6 @@ def test_as_shared_expert_of_a_packed_layer(tokens, eight_bit):
     expert = D.W8A8GatedFeedForward.from_mlp(block) if eight_bit else block
     moe.shared_expert = expert
     moe.shared_expert_gate = torch.nn.Linear(256, 1, bias=False, dtype=torch.bfloat16, device=DEV)
-    moe._engine = moe._graphs = None
     for _ in range(3):                                              # eager, captured, replayed
         y = moe(x)
         want = routed[0] + expert(x[0]) * torch.sigmoid(moe.shared_expert_gate(x[0]))
