@@ -245,7 +245,8 @@ bool quant_ok(const void* x, long long pitch, int K, const void* codes, const vo
 bool weight8_ok(const void* w, const void* scale) { return usable(w) && scale; }
 int check_ffn(int T, int H, int I) {
   if (T < 0 || H < 8 || I < 8 || H % 8 != 0 || I % 8 != 0) return DMOQ_EINVAL;
-  return T > kMaxDim || H > kMaxDim || I > kMaxDim / 2 ? DMOQ_ESIZE : DMOQ_OK;   // the gradients of both projections are one product of 2 I rows
+  // the gradients of both projections are one product of 2 I rows, and the bytes of a row are counted in 32 bits
+  return T > kMaxDim || H > kMaxDim / 2 || I > kMaxDim / 2 ? DMOQ_ESIZE : DMOQ_OK;
 }
 
 // The products of `codes`, or of the 16-bit rows x (pitch in elements), whose codes then go into `codes` / `scales` first unless

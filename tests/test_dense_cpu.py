@@ -65,6 +65,8 @@ def test_gated_ffn_refuses():
     for i, v in ((2, 60), (2, 68), (7, 60), (7, 0), (8, 12), (8, 0), (6, -4), (11, ODD), (10, 24), (10, 36), (0, ODD), (3, ODD), (4, ODD), (5, ODD),
                  (9, ODD), (12, ODD)):
         assert lib.dmoq_gated_ffn(*(good[:i] + [v] + good[i + 1:]), None) == EINVAL, (i, v)
+    for i in (7, 8):
+        assert lib.dmoq_gated_ffn(*(good[:i] + [(1 << 29) + 8] + good[i + 1:]), None) == ESIZE
     #       dy pitch x bf pitch wg wu wd  T   H   I  h pitch saved dgu pitch dx dwg dwu dwd
     good = [P, 64, P, 1, 64, P, P, P, 4, 64, 32, P, 32, P, P, 64, P, P, P, P]
     for i in (0, 2, 5, 6, 7, 11, 13, 14):

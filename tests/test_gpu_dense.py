@@ -421,6 +421,37 @@ def test_streams_and_captured_graphs():
     healthy()
 
 
+def test_capture_over_two_streams():
+    """Kernels that may overlap their predecessor, captured across a fork and a join and among kernels of others."""
+    g = rng(22)
+    x, (w, ws) = acts(g, 200, 512, torch.bfloat16), weight8(g, 512, 512)
+    fx, wg, wu, wd, _ = ffn_inputs(3000, 512, 640, torch.bfloat16, seed=10)
+
+    def work(side):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        a = dense.int8_linear(x, w, ws)
+        with torch.cuda.stream(side):
+            b = dense.gated_feed_forward(fx, wg, wu, wd)
+            c = dense.gated_feed_forward(b[:7] * 0.5, wg, wu, wd)
+        a = dense.int8_linear(a + 1, w, ws)
+        main.wait_stream(side)
+        return dense.int8_linear(a + b[:200], w, ws), dense.gated_feed_forward(c, wg, wu, wd)
+
+    side = torch.cuda.Stream()
+    want = [v.clone() for v in work(side)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work(side)
+    for _ in range(3):
+        for v in got:
+            v.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(want, got))
+
+
 def test_training_step_in_a_captured_graph():
     x, wg, wu, wd, dy = ffn_inputs(96, 264, 136, torch.bfloat16, seed=12)
     leaves = [v.requires_grad_(True) for v in (x, wg, wu, wd)]
