@@ -221,28 +221,35 @@ class _GatedFeedForward(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, wg, wu, wd, h, saved = ctx.saved_tensors
-        need_x, need_g, need_u, need_d = ctx.needs_input_grad
-        hidden, inter = wd.shape
-        dy, t, dy_pitch = _rows(dy, hidden)
-        # saved-tensor hooks may have laid them out anew
-        x, _, x_pitch = _rows(x, hidden)
-        wg, wu, wd = _packed(wg), _packed(wu), _packed(wd)
-        h, saved = h if h is None else _packed(h), saved if saved is None else _packed(saved)
-        d_pitch = (2 * inter + 63) & -64
-        dgu = x.new_empty((t, d_pitch)) if need_x or need_g or need_u else None
-        dx = x.new_empty((t, hidden)) if need_x else None
-        # the two halves of one buffer: one product computes both
-        dw = x.new_empty((int(need_g) + int(need_u), inter, hidden)) if need_g or need_u else None
-        dwg = dw[0] if need_g else None
-        dwu = dw[-1] if need_u else None
-        dwd = x.new_empty((hidden, inter)) if need_d else None
-        _call("dmoq_gated_ffn_backward", x.get_device(), dy.data_ptr(), dy_pitch, x.data_ptr(), x.dtype is _BF16, x_pitch, wg.data_ptr(),
-              wu.data_ptr(), wd.data_ptr(), t, hidden, inter, _ptr(h), 0 if h is None else h.shape[1], _ptr(saved),
-              _ptr(dgu), d_pitch, _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd))
-        return dx, dwg, dwu, dwd
+        # grad mode is on only where a graph of the backward pass is asked for, which this has none of
+        return _ffn_backward_once(ctx, dy) if torch.is_grad_enabled() else _ffn_backward(ctx, dy)
+
+
+def _ffn_backward(ctx, dy):
+    x, wg, wu, wd, h, saved = ctx.saved_tensors
+    need_x, need_g, need_u, need_d = ctx.needs_input_grad
+    hidden, inter = wd.shape
+    dy, t, dy_pitch = _rows(dy, hidden)
+    # saved-tensor hooks may have laid them out anew
+    x, _, x_pitch = _rows(x, hidden)
+    wg, wu, wd = _packed(wg), _packed(wu), _packed(wd)
+    h, saved = h if h is None else _packed(h), saved if saved is None else _packed(saved)
+    d_pitch = (2 * inter + 63) & -64
+    dgu = x.new_empty((t, d_pitch)) if need_x or need_g or need_u else None
+    dx = x.new_empty((t, hidden)) if need_x else None
+    # the two halves of one buffer: one product computes both
+    dw = x.new_empty((int(need_g) + int(need_u), inter, hidden)) if need_g or need_u else None
+    dwg = dw[0] if need_g else None
+    dwu = dw[-1] if need_u else None
+    dwd = x.new_empty((hidden, inter)) if need_d else None
+    _call("dmoq_gated_ffn_backward", x.get_device(), dy.data_ptr(), dy_pitch, x.data_ptr(), x.dtype is _BF16, x_pitch, wg.data_ptr(),
+          wu.data_ptr(), wd.data_ptr(), t, hidden, inter, _ptr(h), 0 if h is None else h.shape[1], _ptr(saved),
+          _ptr(dgu), d_pitch, _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd))
+    return dx, dwg, dwu, dwd
+
+
+_ffn_backward_once = once_differentiable(_ffn_backward)
 
 
 def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor) -> torch.Tensor:
