@@ -12,7 +12,7 @@ namespace dense {
 int tile_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, const Args& a, int splits, cudaStream_t s);
 int tile_blocks_at_once(int splits);
 int pair_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, const Args& a, cudaStream_t s);
-int pair_group(const Maps* maps, const Args* p, const bool* a_mn, int n_long, cudaStream_t s);
+int pair_group(const Maps* maps, const Args* p, const bool* a_mn, int n, int n_long, cudaStream_t s);
 
 int mid_product(int kind, int epi, const Maps& maps, const Args& a, int splits, cudaStream_t s);
 int mid_token_box(int tokens);
@@ -185,41 +185,52 @@ int run(const Product& p, const Choice& choice, cudaStream_t s) {
 }
 int run(const Product& p, cudaStream_t s) { return run(p, choose(p), s); }
 
-// Three independent products (MN-major B, plain outputs): in one launch their tiles fill the SMs together, which takes as long
-// as a pair's share of all steps, or the longest tile.
-int run_three(const Product (&p)[3], cudaStream_t s) {
-  long long total = 0, longest = 0, shortest = 1LL << 60;
-  Choice alone[3];
-  double apart = 0.0;
-  for (int i = 0; i < 3; ++i) {
-    alone[i] = choose(p[i]);
-    apart += alone[i].cost;
-    total += pair_tiles(p[i]) * steps_of(p[i]);
-    longest = std::max(longest, steps_of(p[i]));
-    shortest = std::min(shortest, steps_of(p[i]));
+// Independent products (MN-major B, plain outputs) in one launch: their tiles fill the SMs together.  That takes as long as a
+// pair's share of all tiles, each with about 2 us that the next one's products do not cover, or the longest tile.
+double group_cost(const Product* const* p, int n) {
+  double all = 0.0, longest = 0.0;
+  for (int i = 0; i < n; ++i) {
+    const double tile = 2.0 + 0.30 * steps_of(*p[i]);
+    all += pair_tiles(*p[i]) * tile;
+    longest = std::max(longest, tile);
   }
-  if (apart < 6.6 + 0.30 * std::max((double)total / (dmoq_sm_count() / 2), (double)longest)) {
-    for (int i = 0; i < 3; ++i) {
-      const int rc = run(p[i], alone[i], s);
-      if (rc != DMOQ_OK) return rc;
-    }
-    return DMOQ_OK;
+  return 4.6 + std::max(all / (dmoq_sm_count() / 2), longest);
+}
+int run_group(const Product* const* p, int n, cudaStream_t s) {
+  long long longest = 0, shortest = 1LL << 60;
+  for (int i = 0; i < n; ++i) {
+    longest = std::max(longest, steps_of(*p[i]));
+    shortest = std::min(shortest, steps_of(*p[i]));
   }
   Maps maps[3];
   Args args[3];
   bool a_mn[3];
-  int n = 0, n_long = 0;
+  int m = 0, n_long = 0;
   for (int side = 0; side < 2; ++side) {      // the products with the longer tiles first
-    for (const Product& q : p) {
+    for (int i = 0; i < n; ++i) {
+      const Product& q = *p[i];
       if ((2 * steps_of(q) >= longest + shortest) != (side == 0)) continue;
-      const int rc = make_maps(maps[n], q, 128);
+      const int rc = make_maps(maps[m], q, 128);
       if (rc != DMOQ_OK) return rc;
-      args[n] = pair_args(q);
-      a_mn[n++] = q.a_mn;
+      args[m] = pair_args(q);
+      a_mn[m++] = q.a_mn;
     }
-    if (side == 0) n_long = n;
+    if (side == 0) n_long = m;
   }
-  return pair_group(maps, args, a_mn, n_long, s);
+  return pair_group(maps, args, a_mn, n, n_long, s);
+}
+// The three products behind dg and du: each by itself, all in one launch, or the two weight gradients in one (8192 tokens of 2048 /
+// 512: 56 us in one launch, 107 in three; 257 tokens of 1032 / 2728: dx is better off with its long K split).
+int run_gradients(const Product& dx, const Product& dw_in, const Product& dw_out, cudaStream_t s) {
+  const Product* all[3] = {&dx, &dw_in, &dw_out};
+  const Choice x = choose(dx), in = choose(dw_in), out = choose(dw_out);
+  const double weights = group_cost(all + 1, 2), apart = in.cost + out.cost;
+  if (group_cost(all, 3) <= x.cost + std::min(weights, apart)) return run_group(all, 3, s);
+  int rc = run(dx, x, s);
+  if (rc != DMOQ_OK) return rc;
+  if (weights <= apart) return run_group(all + 1, 2, s);
+  rc = run(dw_in, in, s);
+  return rc != DMOQ_OK ? rc : run(dw_out, out, s);
 }
 
 // four-element accesses to a 16-bit matrix
@@ -433,10 +444,7 @@ extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const v
   const bool joined = dw_gate && dw_up && static_cast<char*>(dw_up) == static_cast<char*>(dw_gate) + w_bytes;
   if (joined) weight_grad(pg, {dg, T, 2 * (long long)I, d_pitch}, xm, dw_gate);   // one product for both halves
   if (dw_down) weight_grad(pd, {dy, T, H, dy_pitch}, {h, T, I, h_pitch}, dw_down);
-  if (dx && joined && dw_down) {
-    const Product all[3] = {px, pg, pd};
-    return run_three(all, s);
-  }
+  if (dx && joined && dw_down) return run_gradients(px, pg, pd, s);
   if (dx && (rc = run(px, s)) != DMOQ_OK) return rc;
   if (joined) {
     if ((rc = run(pg, s)) != DMOQ_OK) return rc;

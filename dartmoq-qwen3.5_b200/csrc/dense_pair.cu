@@ -399,7 +399,7 @@ int launch(Work<NP>& work, cudaStream_t s) {
     for (int q = 0; q < work.n_long; ++q) work.long_tiles += work.tiles[q];
     const long long shorts = tiles - work.long_tiles;
     const int ahead = work.long_tiles % pairs;
-    work.fill = ahead == 0 || shorts == 0 ? 0 : (int)std::min<long long>(steps(0) / steps(NP - 1), shorts / (pairs - ahead));
+    work.fill = ahead == 0 || shorts == 0 ? 0 : (int)std::min<long long>(steps(0) / steps(work.n_long), shorts / (pairs - ahead));
   }
   return launch_overlapped(kernel, 2 * pairs, kThreads, kSmem, 0, s, work);
 }
@@ -429,10 +429,10 @@ int pair_product(int kind, bool a_mn, bool b_mn, int epi, const Maps& maps, cons
   }
 }
 
-// Three 16-bit products with MN-major B in one launch, ordered so that the first n_long have the longer tiles.
-int pair_group(const Maps* maps, const Args* p, const bool* a_mn, int n_long, cudaStream_t s) {
+// Two or three 16-bit products with MN-major B in one launch, ordered so that the first n_long have the longer tiles.
+int pair_group(const Maps* maps, const Args* p, const bool* a_mn, int n, int n_long, cudaStream_t s) {
   Work<3> w{};
-  for (int q = 0; q < 3; ++q) {
+  for (int q = 0; q < n; ++q) {
     w.maps[q] = maps[q];
     w.p[q] = p[q];
     w.a_mn[q] = a_mn[q];
