@@ -92,17 +92,18 @@ EXPORTS = {
     "dmoq_weight_image_bytes": (C.c_size_t, [C.POINTER(Pool), C.c_int32, C.c_int32]),
     "dmoq_expand_weights": (C.c_int, [C.POINTER(Pool), C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]),
     "dmoq_token_quant": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
-    "dmoq_int8_gemm": (C.c_int, [C.c_void_p] * 5 + [C.c_int32] * 4 + [C.c_void_p] * 2),
+    "dmoq_int8_gemm": (C.c_int, [C.c_void_p] * 3 + [C.c_int64] + [C.c_void_p] * 2 + [C.c_int32] * 4 + [C.c_void_p] * 2),
     "dmoq_int8_scratch_bytes": (C.c_size_t, [C.c_int32] * 4),
-    "dmoq_int8_linear": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64] + [C.c_void_p] * 3 + [C.c_int32] * 3 + [C.c_void_p] * 3),
-    "dmoq_int8_gated_gemm": (C.c_int, [C.c_void_p] * 6 + [C.c_int32] * 4 + [C.c_void_p] * 2),
-    "dmoq_int8_gated_linear": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64] + [C.c_void_p] * 4 + [C.c_int32] * 3
+    "dmoq_int8_linear": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_int64] + [C.c_void_p] * 2 + [C.c_int32] * 3
+                         + [C.c_void_p] * 3),
+    "dmoq_int8_gated_gemm": (C.c_int, [C.c_void_p] * 3 + [C.c_int64] + [C.c_void_p] * 2 + [C.c_int64, C.c_void_p] + [C.c_int32] * 4
+                             + [C.c_void_p] * 2),
+    "dmoq_int8_gated_linear": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64] + [C.c_void_p, C.c_int64, C.c_void_p] * 2 + [C.c_int32] * 3
                                + [C.c_void_p] * 3),
-    "dmoq_gated_ffn": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64] + [C.c_void_p] * 3 + [C.c_int32] * 3
+    "dmoq_gated_ffn": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64] + [C.c_void_p, C.c_int64] * 3 + [C.c_int32] * 3
                        + [C.c_void_p, C.c_int64] + [C.c_void_p] * 3),
-    "dmoq_gated_ffn_backward": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_int64] + [C.c_void_p] * 3
-                                + [C.c_int32] * 3 + [C.c_void_p, C.c_int64] + [C.c_void_p] * 2 + [C.c_int64]
-                                + [C.c_void_p] * 5),
+    "dmoq_gated_ffn_backward": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_int64] + [C.c_void_p, C.c_int64] * 3
+                                + [C.c_int32] * 3 + [C.c_void_p, C.c_int64] + [C.c_void_p] * 2 + [C.c_int64] + [C.c_void_p] * 5),
 }
 
 _lib = None

@@ -16,7 +16,8 @@ int pair_group(const Maps* maps, const Args* p, const bool* a_mn, int n, int n_l
 
 int mid_product(int kind, int epi, const Maps& maps, const Args& a, int splits, cudaStream_t s);
 int mid_token_box(int tokens);
-int few_product(int kind, int epi, const void* x, long long x_pitch, const void* w0, const void* w1, const Args& a, cudaStream_t s);
+int few_product(int kind, int epi, const void* x, long long x_pitch, const void* w0, long long w0_pitch, const void* w1, long long w1_pitch,
+                const Args& a, cudaStream_t s);
 bool few_can_fuse(int T, int K, int N, bool dual);
 
 namespace {
@@ -253,7 +254,12 @@ int check_sizes8(int T, int N, int K) {
 bool quant_ok(const void* x, long long pitch, int K, const void* codes, const void* scales) {
   return rows_usable(x, pitch, K) && usable(codes) && scales;
 }
-bool weight8_ok(const void* w, const void* scale) { return usable(w) && scale; }
+struct Weight8 {   // rows of K codes, `pitch` apart, one scale each
+  const int8_t* w;
+  long long pitch;
+  const float* scale;
+};
+bool weight8_ok(const Weight8& w, int K) { return usable(w.w) && w.scale && w.pitch >= K && w.pitch % 16 == 0; }
 int check_ffn(int T, int H, int I) {
   if (T < 0 || H < 8 || I < 8 || H % 8 != 0 || I % 8 != 0) return DMOQ_EINVAL;
   // the gradients of both projections are one product of 2 I rows, and the bytes of a row are counted in 32 bits
@@ -262,27 +268,28 @@ int check_ffn(int T, int H, int I) {
 
 // The products of `codes`, or of the 16-bit rows x (pitch in elements), whose codes then go into `codes` / `scales` first unless
 // the kernel makes them itself.
-int int8_product(const void* x, long long x_pitch, int8_t* codes, long long code_pitch, float* scales, const int8_t* w0, const float* s0, const int8_t* w1,
-                 const float* s1, const void* bias, int bf16, int T, int N, int K, void* out, cudaStream_t s) {
-  const bool few = few_tokens(T, (long long)N * K * (w1 ? 2 : 1)), fuse = x != nullptr && few_can_fuse(T, K, N, w1 != nullptr);   // fuse implies few
+int int8_product(const void* x, long long x_pitch, int8_t* codes, long long code_pitch, float* scales, const Weight8& w, const Weight8* up,
+                 const void* bias, int bf16, int T, int N, int K, void* out, cudaStream_t s) {
+  const bool few = few_tokens(T, (long long)N * K * (up ? 2 : 1)), fuse = x != nullptr && few_can_fuse(T, K, N, up != nullptr);   // fuse implies few
   if (x != nullptr && !fuse) {
     const int rc = dmoq_token_quant_launch(x, bf16, T, K, x_pitch, codes, code_pitch, scales, s);
     if (rc != DMOQ_OK) return rc;
   }
   Product p;
   p.kind = KIND_I8;
-  p.epi = w1 ? EPI_SILU : EPI_SCALE;
+  p.epi = up ? EPI_SILU : EPI_SCALE;
   Args& a = p.args;
   a.M = T, a.N = N, a.K = K, a.segs = 1, a.bf16 = bf16;
-  a.a_scale = fuse ? nullptr : scales, a.b_scale[0] = s0, a.b_scale[1] = s1;
+  a.a_scale = fuse ? nullptr : scales, a.b_scale[0] = w.scale, a.b_scale[1] = up ? up->scale : nullptr;
   a.bias = static_cast<const uint16_t*>(bias);
   a.out[0] = static_cast<uint16_t*>(out);
   a.ld_out = N;
   a.vec = vec4(out, N, N);
-  if (few) return few_product(KIND_I8, p.epi, fuse ? x : codes, fuse ? 2 * x_pitch : code_pitch, w0, w1, a, s);
+  if (few)
+    return few_product(KIND_I8, p.epi, fuse ? x : codes, fuse ? 2 * x_pitch : code_pitch, w.w, w.pitch, up ? up->w : nullptr, up ? up->pitch : 0, a, s);
   p.a[0] = {codes, T, K, code_pitch};
-  p.b[0] = {w0, N, K, K};
-  if (w1) p.b[1] = {w1, N, K, K};
+  p.b[0] = {w.w, N, K, w.pitch};
+  if (up) p.b[1] = {up->w, N, K, up->pitch};
   return run(p, s);
 }
 
@@ -300,23 +307,25 @@ extern "C" int dmoq_token_quant(const void* x, int32_t is_bf16, int32_t T, int32
   return dmoq_token_quant_launch(x, is_bf16, T, K, x_pitch, codes, K, scales, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int dmoq_int8_gemm(const int8_t* codes, const float* scales, const int8_t* w, const float* w_scale, const void* bias,
+extern "C" int dmoq_int8_gemm(const int8_t* codes, const float* scales, const int8_t* w, int64_t w_pitch, const float* w_scale, const void* bias,
                               int32_t is_bf16, int32_t T, int32_t N, int32_t K, void* out, void* stream) {
   const int rc = check_sizes8(T, N, K);
   if (rc != DMOQ_OK || T == 0) return rc;
-  DMOQ_CHECK_ARG(usable(codes) && scales && weight8_ok(w, w_scale) && out);
-  return int8_product(nullptr, 0, const_cast<int8_t*>(codes), K, const_cast<float*>(scales), w, w_scale, nullptr, nullptr, bias, is_bf16, T, N, K,
-                      out, static_cast<cudaStream_t>(stream));
+  const Weight8 weight = {w, w_pitch, w_scale};
+  DMOQ_CHECK_ARG(usable(codes) && scales && weight8_ok(weight, K) && out);
+  return int8_product(nullptr, 0, const_cast<int8_t*>(codes), K, const_cast<float*>(scales), weight, nullptr, bias, is_bf16, T, N, K, out,
+                      static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int dmoq_int8_gated_gemm(const int8_t* codes, const float* scales, const int8_t* w_gate, const float* gate_scale,
-                                    const int8_t* w_up, const float* up_scale, int32_t is_bf16, int32_t T, int32_t I, int32_t K,
-                                    void* out, void* stream) {
+extern "C" int dmoq_int8_gated_gemm(const int8_t* codes, const float* scales, const int8_t* w_gate, int64_t gate_pitch, const float* gate_scale,
+                                    const int8_t* w_up, int64_t up_pitch, const float* up_scale, int32_t is_bf16, int32_t T, int32_t I,
+                                    int32_t K, void* out, void* stream) {
   const int rc = check_sizes8(T, I, K);
   if (rc != DMOQ_OK || T == 0) return rc;
-  DMOQ_CHECK_ARG(usable(codes) && scales && weight8_ok(w_gate, gate_scale) && weight8_ok(w_up, up_scale) && out);
-  return int8_product(nullptr, 0, const_cast<int8_t*>(codes), K, const_cast<float*>(scales), w_gate, gate_scale, w_up, up_scale, nullptr, is_bf16,
-                      T, I, K, out, static_cast<cudaStream_t>(stream));
+  const Weight8 gate = {w_gate, gate_pitch, gate_scale}, up = {w_up, up_pitch, up_scale};
+  DMOQ_CHECK_ARG(usable(codes) && scales && weight8_ok(gate, K) && weight8_ok(up, K) && out);
+  return int8_product(nullptr, 0, const_cast<int8_t*>(codes), K, const_cast<float*>(scales), gate, &up, nullptr, is_bf16, T, I, K, out,
+                      static_cast<cudaStream_t>(stream));
 }
 
 namespace {
@@ -333,57 +342,61 @@ extern "C" size_t dmoq_int8_scratch_bytes(int32_t T, int32_t N, int32_t K, int32
   return (size_t)T * scratch_pitch(K) + (size_t)T * sizeof(float);
 }
 
-extern "C" int dmoq_int8_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w, const float* w_scale, const void* bias,
-                                int32_t T, int32_t N, int32_t K, void* scratch, void* out, void* stream) {
+extern "C" int dmoq_int8_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w, int64_t w_pitch, const float* w_scale,
+                                const void* bias, int32_t T, int32_t N, int32_t K, void* scratch, void* out, void* stream) {
   const int rc = check_sizes8(T, N, K);
   if (rc != DMOQ_OK || T == 0) return rc;
-  DMOQ_CHECK_ARG(rows_usable(x, x_pitch, K) && weight8_ok(w, w_scale) && out && (few_can_fuse(T, K, N, false) || usable(scratch)));
-  return int8_product(x, x_pitch, static_cast<int8_t*>(scratch), scratch_pitch(K), scratch_scales(scratch, T, K), w, w_scale, nullptr, nullptr, bias, is_bf16, T, N, K,
-                      out, static_cast<cudaStream_t>(stream));
+  const Weight8 weight = {w, w_pitch, w_scale};
+  DMOQ_CHECK_ARG(rows_usable(x, x_pitch, K) && weight8_ok(weight, K) && out && (few_can_fuse(T, K, N, false) || usable(scratch)));
+  return int8_product(x, x_pitch, static_cast<int8_t*>(scratch), scratch_pitch(K), scratch_scales(scratch, T, K), weight, nullptr, bias, is_bf16,
+                      T, N, K, out, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int dmoq_int8_gated_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w_gate, const float* gate_scale,
-                                      const int8_t* w_up, const float* up_scale, int32_t T, int32_t I, int32_t K, void* scratch, void* out,
-                                      void* stream) {
+extern "C" int dmoq_int8_gated_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w_gate, int64_t gate_pitch,
+                                      const float* gate_scale, const int8_t* w_up, int64_t up_pitch, const float* up_scale, int32_t T,
+                                      int32_t I, int32_t K, void* scratch, void* out, void* stream) {
   const int rc = check_sizes8(T, I, K);
   if (rc != DMOQ_OK || T == 0) return rc;
-  DMOQ_CHECK_ARG(rows_usable(x, x_pitch, K) && weight8_ok(w_gate, gate_scale) && weight8_ok(w_up, up_scale) && out &&
+  const Weight8 gate = {w_gate, gate_pitch, gate_scale}, up = {w_up, up_pitch, up_scale};
+  DMOQ_CHECK_ARG(rows_usable(x, x_pitch, K) && weight8_ok(gate, K) && weight8_ok(up, K) && out &&
                  (few_can_fuse(T, K, I, true) || usable(scratch)));
-  return int8_product(x, x_pitch, static_cast<int8_t*>(scratch), scratch_pitch(K), scratch_scales(scratch, T, K), w_gate, gate_scale, w_up, up_scale, nullptr, is_bf16, T,
+  return int8_product(x, x_pitch, static_cast<int8_t*>(scratch), scratch_pitch(K), scratch_scales(scratch, T, K), gate, &up, nullptr, is_bf16, T,
                       I, K, out, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate, const void* w_up, const void* w_down,
-                              int32_t T, int32_t H, int32_t I, void* h, int64_t h_pitch, void* saved, void* y, void* stream) {
+extern "C" int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate, int64_t gate_pitch, const void* w_up,
+                              int64_t up_pitch, const void* w_down, int64_t down_pitch, int32_t T, int32_t H, int32_t I, void* h, int64_t h_pitch, void* saved, void* y, void* stream) {
   const int size = check_ffn(T, H, I);
   if (size != DMOQ_OK || T == 0) return size;
-  DMOQ_CHECK_ARG(rows_usable(x, x_pitch, H) && usable(w_gate) && usable(w_up) && usable(w_down) && rows_usable(h, h_pitch, I) && usable(y));
+  DMOQ_CHECK_ARG(rows_usable(x, x_pitch, H) && rows_usable(w_gate, gate_pitch, H) && rows_usable(w_up, up_pitch, H) &&
+                 rows_usable(w_down, down_pitch, I) && rows_usable(h, h_pitch, I) && usable(y));
   DMOQ_CHECK_ARG(aligned16(saved));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   Product up;
   up.epi = saved ? EPI_SILU_SAVE : EPI_SILU;
   up.a[0] = {x, T, H, x_pitch};
-  up.b[0] = {w_gate, I, H, H};
-  up.b[1] = {w_up, I, H, H};
+  up.b[0] = {w_gate, I, H, gate_pitch};
+  up.b[1] = {w_up, I, H, up_pitch};
   up.args.M = T, up.args.N = I, up.args.K = H, up.args.segs = 1, up.args.bf16 = is_bf16, up.args.vec = 1;
   up.args.out[0] = static_cast<uint16_t*>(h);
   for (int e = 0; saved && e < 3; ++e) up.args.out[1 + e] = static_cast<uint16_t*>(saved) + e * (size_t)T * I;
   up.args.ld_out = h_pitch;
   up.args.ld_saved = I;
   const long long w_bytes = 2LL * H * I;
-  int rc = few_tokens(T, 2 * w_bytes) && !saved ? few_product(KIND_16, EPI_SILU, x, 2 * x_pitch, w_gate, w_up, up.args, s) : run(up, s);
+  int rc = few_tokens(T, 2 * w_bytes) && !saved ? few_product(KIND_16, EPI_SILU, x, 2 * x_pitch, w_gate, 2 * gate_pitch, w_up, 2 * up_pitch, up.args, s)
+                                               : run(up, s);
   if (rc != DMOQ_OK) return rc;
   Product down;
   down.a[0] = {h, T, I, h_pitch};
-  down.b[0] = {w_down, H, I, I};
+  down.b[0] = {w_down, H, I, down_pitch};
   down.args.M = T, down.args.N = H, down.args.K = I, down.args.segs = 1, down.args.bf16 = is_bf16, down.args.vec = 1;
   down.args.out[0] = static_cast<uint16_t*>(y);
   down.args.ld_out = H;
-  return few_tokens(T, w_bytes) ? few_product(KIND_16, EPI_OUT, h, 2 * h_pitch, w_down, nullptr, down.args, s) : run(down, s);
+  return few_tokens(T, w_bytes) ? few_product(KIND_16, EPI_OUT, h, 2 * h_pitch, w_down, 2 * down_pitch, nullptr, 0, down.args, s) : run(down, s);
 }
 
 extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate,
-                                       const void* w_up, const void* w_down, int32_t T, int32_t H, int32_t I, const void* h,
+                                       int64_t gate_pitch, const void* w_up, int64_t up_pitch, const void* w_down, int64_t down_pitch, int32_t T, int32_t H, int32_t I, const void* h,
                                        int64_t h_pitch, const void* saved, void* d_gate_up, int64_t d_pitch, void* dx, void* dw_gate, void* dw_up,
                                        void* dw_down, void* stream) {
   const int size = check_ffn(T, H, I);
@@ -401,8 +414,8 @@ extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const v
   DMOQ_CHECK_ARG(aligned16(dx) && aligned16(dw_gate) && aligned16(dw_up) && aligned16(dw_down));
   DMOQ_CHECK_ARG(!(inner || dw_down) || rows_usable(dy, dy_pitch, H));
   DMOQ_CHECK_ARG(!dw_down || rows_usable(h, h_pitch, I));
-  DMOQ_CHECK_ARG(!inner || (usable(w_down) && usable(saved) && rows_usable(d_gate_up, d_pitch, 2 * I)));
-  DMOQ_CHECK_ARG(!dx || (usable(w_gate) && usable(w_up)));
+  DMOQ_CHECK_ARG(!inner || (rows_usable(w_down, down_pitch, I) && usable(saved) && rows_usable(d_gate_up, d_pitch, 2 * I)));
+  DMOQ_CHECK_ARG(!dx || (rows_usable(w_gate, gate_pitch, H) && rows_usable(w_up, up_pitch, H)));
   DMOQ_CHECK_ARG(!(dw_gate || dw_up) || rows_usable(x, x_pitch, H));
   uint16_t* dg = static_cast<uint16_t*>(d_gate_up);
   int rc = DMOQ_OK;
@@ -411,7 +424,7 @@ extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const v
     p.epi = EPI_GRAD;
     p.b_mn = true;
     p.a[0] = {dy, T, H, dy_pitch};
-    p.b[0] = {w_down, H, I, I};
+    p.b[0] = {w_down, H, I, down_pitch};
     p.args.M = T, p.args.N = I, p.args.K = H, p.args.segs = 1, p.args.bf16 = is_bf16, p.args.vec = 1;
     for (int e = 0; e < 3; ++e) p.args.in[e] = static_cast<const uint16_t*>(saved) + e * (size_t)T * I;
     p.args.ld_in = I;
@@ -430,8 +443,8 @@ extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const v
     px.b_mn = true;
     px.a[0] = {dg, T, I, d_pitch};
     px.a[1] = {dg + I, T, I, d_pitch};
-    px.b[0] = {w_gate, I, H, H};
-    px.b[1] = {w_up, I, H, H};
+    px.b[0] = {w_gate, I, H, gate_pitch};
+    px.b[1] = {w_up, I, H, up_pitch};
     output(px, T, H, I, 2, dx);
   }
   auto weight_grad = [&](Product& p, const Matrix& a, const Matrix& b, void* out) {   // a^T b, both along the tokens

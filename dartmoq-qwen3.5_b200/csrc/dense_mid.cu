@@ -6,6 +6,8 @@
 // finishes.  Where
 // there are few tiles the K axis is split over a cluster's blocks, whose sums are joined through distributed shared memory
 // in rank order.  The accumulator (a lane an output, a column a token) passes through shared memory, a row a token.
+// 64 tokens: 13824 x 5120 twice 50 us = 5.7 TB/s of weights (88 % of the measured bandwidth), 5120 x 13824 in 4 parts 31 us = 4.6 TB/s
+// (40 tiles: their start, join and end show).
 #include "dense.cuh"
 
 __device__ int g_dmoq_dense_mid_status = 0;

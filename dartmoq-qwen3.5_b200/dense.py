@@ -39,11 +39,6 @@ def _call(name: str, index: int, *args) -> None:
         _lib.check(rc, name)
 
 
-def _packed(t: torch.Tensor) -> torch.Tensor:
-    """``t``, copied only if it is not contiguous or not 16-byte aligned."""
-    return t if t.is_contiguous() and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
-
-
 def _rows(t: torch.Tensor, cols: int) -> Tuple[torch.Tensor, int, int]:
     """``t`` as rows of ``cols`` elements that the kernels can read where they lie (unit inner stride, 16-byte aligned rows),
     copied only if they cannot; their number, and the pitch between them in elements."""
@@ -79,8 +74,8 @@ def _check_k8(k: int) -> None:
         raise ValueError(f"8-bit products need an inner size that is a multiple of 16, got {k}")
 
 
-def _weight8(w: torch.Tensor, scale: torch.Tensor, k: int, index: int, what: str) -> Tuple[torch.Tensor, torch.Tensor]:
-    """The weight and its scales as the kernels take them."""
+def _weight8(w: torch.Tensor, scale: torch.Tensor, k: int, index: int, what: str) -> Tuple[torch.Tensor, int, int, torch.Tensor]:
+    """The weight as the kernels take it, its rows and pitch, and its scales."""
     if w.dtype is not _INT8 or scale.dtype is not _FP32:
         raise TypeError(f"{what} must be int8 with an fp32 scale, got {w.dtype} and {scale.dtype}")
     shape = w.shape
@@ -90,7 +85,7 @@ def _weight8(w: torch.Tensor, scale: torch.Tensor, k: int, index: int, what: str
         raise ValueError(f"{what} needs one scale a row: {shape[0]} rows, scales of shape {tuple(scale.shape)}")
     if w.get_device() != index or scale.get_device() != index:      # -1 on the CPU
         raise ValueError(f"{what} and its scale must be on cuda:{index}")
-    return _packed(w), scale if scale.is_contiguous() else scale.contiguous()
+    return *_rows(w, k), scale if scale.is_contiguous() else scale.contiguous()
 
 
 def _bias_ptr(bias: Optional[torch.Tensor], n: int, dtype: torch.dtype, index: int):
@@ -138,15 +133,14 @@ def int8_matmul(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, 
     _check_k8(k)
     _need(scale.shape == codes.shape[:-1] and scale.is_cuda and scale.get_device() == index,
           f"one scale a token on cuda:{index}: got {tuple(scale.shape)}")
-    w, ws = _weight8(weight, weight_scale, k, index, "weight")
-    n = w.shape[0]
+    w, n, w_pitch, ws = _weight8(weight, weight_scale, k, index, "weight")
     bias, bias_ptr = _bias_ptr(bias, n, out_dtype, index)
     a, t, pitch = _rows(codes, k)
     if pitch != k:
         a = a.contiguous()
     scale = scale.contiguous()
     out = torch.empty(codes.shape[:-1] + (n,), dtype=out_dtype, device=codes.device)
-    _call("dmoq_int8_gemm", index, a.data_ptr(), scale.data_ptr(), w.data_ptr(), ws.data_ptr(), bias_ptr, out_dtype is _BF16, t, n, k,
+    _call("dmoq_int8_gemm", index, a.data_ptr(), scale.data_ptr(), w.data_ptr(), w_pitch, ws.data_ptr(), bias_ptr, out_dtype is _BF16, t, n, k,
           out.data_ptr())
     return out
 
@@ -158,13 +152,12 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     shape, index = x.shape, x.get_device()
     k = shape[-1]
     _check_k8(k)
-    w, ws = _weight8(weight, weight_scale, k, index, "weight")
-    n = w.shape[0]
+    w, n, w_pitch, ws = _weight8(weight, weight_scale, k, index, "weight")
     bias, bias_ptr = _bias_ptr(bias, n, x.dtype, index)
     rows, t, pitch = _rows(x, k)
     scratch = _int8_scratch(x, t, n, k, False)
     out = x.new_empty(shape[:-1] + (n,))
-    _call("dmoq_int8_linear", index, rows.data_ptr(), x.dtype is _BF16, pitch, w.data_ptr(), ws.data_ptr(), bias_ptr, t, n, k,
+    _call("dmoq_int8_linear", index, rows.data_ptr(), x.dtype is _BF16, pitch, w.data_ptr(), w_pitch, ws.data_ptr(), bias_ptr, t, n, k,
           _ptr(scratch), out.data_ptr())
     return out
 
@@ -182,27 +175,29 @@ def int8_gated_linear(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.T
     shape, index = x.shape, x.get_device()
     k = shape[-1]
     _check_k8(k)
-    wg, sg = _weight8(w_gate, gate_scale, k, index, "w_gate")
-    wu, su = _weight8(w_up, up_scale, k, index, "w_up")
-    n = wg.shape[0]
-    if wu.shape[0] != n:
-        raise ValueError(f"w_gate and w_up must have one shape, got {tuple(wg.shape)} and {tuple(wu.shape)}")
+    wg, n, gate_pitch, sg = _weight8(w_gate, gate_scale, k, index, "w_gate")
+    wu, n_up, up_pitch, su = _weight8(w_up, up_scale, k, index, "w_up")
+    if n_up != n:
+        raise ValueError(f"w_gate and w_up must have one shape, got {tuple(w_gate.shape)} and {tuple(w_up.shape)}")
     rows, t, pitch = _rows(x, k)
     scratch = _int8_scratch(x, t, n, k, True)
     out = x.new_empty(shape[:-1] + (n,))
-    _call("dmoq_int8_gated_linear", index, rows.data_ptr(), x.dtype is _BF16, pitch, wg.data_ptr(), sg.data_ptr(), wu.data_ptr(),
-          su.data_ptr(), t, n, k, _ptr(scratch), out.data_ptr())
+    _call("dmoq_int8_gated_linear", index, rows.data_ptr(), x.dtype is _BF16, pitch, wg.data_ptr(), gate_pitch, sg.data_ptr(),
+          wu.data_ptr(), up_pitch, su.data_ptr(), t, n, k, _ptr(scratch), out.data_ptr())
     return out
 
 
 def _ffn_forward(x: torch.Tensor, t: int, pitch: int, wg: torch.Tensor, wu: torch.Tensor, wd: torch.Tensor, save: bool):
     """y, and the hidden values h; with ``save`` also what the gradients need of them."""
     hidden, inter = wd.shape
+    wg, _, gate_pitch = _rows(wg, hidden)
+    wu, _, up_pitch = _rows(wu, hidden)
+    wd, _, down_pitch = _rows(wd, inter)
     h = x.new_empty((t, (inter + 63) & -64))       # rows on whole 128-byte lines
     saved = x.new_empty((3, t, inter), dtype=torch.int16) if save else None
     y = x.new_empty((t, hidden))
-    _call("dmoq_gated_ffn", x.get_device(), x.data_ptr(), x.dtype is _BF16, pitch, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), t, hidden,
-          inter, h.data_ptr(), h.shape[1], _ptr(saved), y.data_ptr())
+    _call("dmoq_gated_ffn", x.get_device(), x.data_ptr(), x.dtype is _BF16, pitch, wg.data_ptr(), gate_pitch, wu.data_ptr(), up_pitch,
+          wd.data_ptr(), down_pitch, t, hidden, inter, h.data_ptr(), h.shape[1], _ptr(saved), y.data_ptr())
     return y, h, saved
 
 
@@ -233,8 +228,14 @@ def _ffn_backward(ctx, dy):
     dy, t, dy_pitch = _rows(dy, hidden)
     # saved-tensor hooks may have laid them out anew
     x, _, x_pitch = _rows(x, hidden)
-    wg, wu, wd = _packed(wg), _packed(wu), _packed(wd)
-    h, saved = h if h is None else _packed(h), saved if saved is None else _packed(saved)
+    wg, _, gate_pitch = _rows(wg, hidden)
+    wu, _, up_pitch = _rows(wu, hidden)
+    wd, _, down_pitch = _rows(wd, inter)
+    h_pitch = 0
+    if h is not None:
+        h, _, h_pitch = _rows(h, h.shape[1])
+    if saved is not None:
+        saved = saved.contiguous()
     d_pitch = (2 * inter + 63) & -64
     dgu = x.new_empty((t, d_pitch)) if need_x or need_g or need_u else None
     dx = x.new_empty((t, hidden)) if need_x else None
@@ -244,8 +245,7 @@ def _ffn_backward(ctx, dy):
     dwu = dw[-1] if need_u else None
     dwd = x.new_empty((hidden, inter)) if need_d else None
     _call("dmoq_gated_ffn_backward", x.get_device(), dy.data_ptr(), dy_pitch, x.data_ptr(), x.dtype is _BF16, x_pitch, wg.data_ptr(),
-          wu.data_ptr(), wd.data_ptr(), t, hidden, inter, _ptr(h), 0 if h is None else h.shape[1], _ptr(saved),
-          _ptr(dgu), d_pitch, _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd))
+          gate_pitch, wu.data_ptr(), up_pitch, wd.data_ptr(), down_pitch, t, hidden, inter, _ptr(h), h_pitch, _ptr(saved), _ptr(dgu), d_pitch, _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd))
     return dx, dwg, dwu, dwd
 
 
@@ -270,7 +270,6 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
         raise ValueError(f"hidden and intermediate sizes must be multiples of 8, got {hidden} and {inter}")
     if w_gate.get_device() != index or w_up.get_device() != index or w_down.get_device() != index:
         raise ValueError(f"all weights must be on cuda:{index}")
-    w_gate, w_up, w_down = _packed(w_gate), _packed(w_up), _packed(w_down)
     rows = x if x.dim() == 2 else x.reshape(-1, hidden)
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
         y = _GatedFeedForward.apply(rows, w_gate, w_up, w_down)

@@ -358,8 +358,8 @@ int dmoq_quantize_packed(const void* w, int32_t w_kind, int32_t N, int32_t K, in
 
 /* ------------------------------------------------------------------------------------------------------------------
  * Dense operators beside the packed experts (no counterpart in the reference, which runs them as torch modules).
- * 16-bit tensors are bf16 when is_bf16, else fp16; matrices are row-major; weights, codes and outputs are contiguous and
- * 16-byte aligned; a pitch is the distance between rows in elements (rows 16-byte aligned).  T may be 0.
+ * 16-bit tensors are bf16 when is_bf16, else fp16; matrices are row-major; codes and outputs are contiguous and 16-byte
+ * aligned; a pitch is the distance between rows in elements (rows 16-byte aligned).  T may be 0.
  *
  * 8-bit products: K a multiple of 16, at most 131056 (the int32 sums are exact); any number of outputs.
  *   token_quant: scales[t] = max|x[t]| / 127, codes[t][k] = rint(127 x[t][k] / max|x[t]|), ties to even, correctly rounded; a row
@@ -371,15 +371,15 @@ int dmoq_quantize_packed(const void* w, int32_t w_kind, int32_t N, int32_t K, in
  */
 int dmoq_token_quant(const void* x, int32_t is_bf16, int32_t T, int32_t K, int64_t x_pitch, int8_t* codes, float* scales,
                      void* stream);
-int dmoq_int8_gemm(const int8_t* codes, const float* scales, const int8_t* w, const float* w_scale, const void* bias,
-                   int32_t is_bf16, int32_t T, int32_t N, int32_t K, void* out, void* stream);
-int dmoq_int8_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w, const float* w_scale, const void* bias,
-                     int32_t T, int32_t N, int32_t K, void* scratch, void* out, void* stream);
-int dmoq_int8_gated_gemm(const int8_t* codes, const float* scales, const int8_t* w_gate, const float* gate_scale,
-                         const int8_t* w_up, const float* up_scale, int32_t is_bf16, int32_t T, int32_t I, int32_t K, void* out,
+int dmoq_int8_gemm(const int8_t* codes, const float* scales, const int8_t* w, int64_t w_pitch, const float* w_scale,
+                   const void* bias, int32_t is_bf16, int32_t T, int32_t N, int32_t K, void* out, void* stream);
+int dmoq_int8_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w, int64_t w_pitch, const float* w_scale,
+                     const void* bias, int32_t T, int32_t N, int32_t K, void* scratch, void* out, void* stream);
+int dmoq_int8_gated_gemm(const int8_t* codes, const float* scales, const int8_t* w_gate, int64_t gate_pitch,
+                         const float* gate_scale, const int8_t* w_up, int64_t up_pitch, const float* up_scale, int32_t is_bf16, int32_t T, int32_t I, int32_t K, void* out,
                          void* stream);
-int dmoq_int8_gated_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w_gate, const float* gate_scale,
-                           const int8_t* w_up, const float* up_scale, int32_t T, int32_t I, int32_t K, void* scratch,
+int dmoq_int8_gated_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w_gate, int64_t gate_pitch,
+                           const float* gate_scale, const int8_t* w_up, int64_t up_pitch, const float* up_scale, int32_t T, int32_t I, int32_t K, void* scratch,
                            void* out, void* stream);
 size_t dmoq_int8_scratch_bytes(int32_t T, int32_t N, int32_t K, int32_t gated);
 
@@ -392,10 +392,10 @@ size_t dmoq_int8_scratch_bytes(int32_t T, int32_t N, int32_t K, int32_t gated);
  *   dx = dg w_gate + du w_up, dw_gate = dg^T x, dw_up = du^T x, dw_down = dy^T h.  Outputs that are NULL are not computed, and
  *   what only they need may be NULL too.  dw_up = dw_gate + H * I elements lets one product compute both.
  */
-int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate, const void* w_up, const void* w_down,
-                   int32_t T, int32_t H, int32_t I, void* h, int64_t h_pitch, void* saved, void* y, void* stream);
+int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate, int64_t gate_pitch, const void* w_up,
+                   int64_t up_pitch, const void* w_down, int64_t down_pitch, int32_t T, int32_t H, int32_t I, void* h, int64_t h_pitch, void* saved, void* y, void* stream);
 int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate,
-                            const void* w_up, const void* w_down, int32_t T, int32_t H, int32_t I, const void* h, int64_t h_pitch,
+                            int64_t gate_pitch, const void* w_up, int64_t up_pitch, const void* w_down, int64_t down_pitch, int32_t T, int32_t H, int32_t I, const void* h, int64_t h_pitch,
                             const void* saved, void* d_gate_up, int64_t d_pitch, void* dx, void* dw_gate, void* dw_up, void* dw_down, void* stream);
 
 #ifdef __cplusplus

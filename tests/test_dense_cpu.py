@@ -22,28 +22,33 @@ def test_token_quant_refuses():
         assert f(*bad, None) == EINVAL, bad
 
 
+def each(f, good, want, bad):
+    for i, v in bad:
+        assert f(*(good[:i] + [v] + good[i + 1:]), None) == want, (i, v)
+
+
 def test_int8_products_refuse():
     lib = _lib.load()
-    good = [P, P, P, P, None, 1, 4, 33, 128, P]
-    assert lib.dmoq_int8_gemm(*(good[:6] + [0] + good[7:]), None) == OK
-    for i in (0, 1, 2, 3, 9):
-        assert lib.dmoq_int8_gemm(*(good[:i] + [None] + good[i + 1:]), None) == EINVAL
-    for i, v in ((0, ODD), (2, ODD), (6, -1), (7, 0), (8, 8), (8, 0), (8, 136)):
-        assert lib.dmoq_int8_gemm(*(good[:i] + [v] + good[i + 1:]), None) == EINVAL, (i, v)
-    assert lib.dmoq_int8_gemm(*(good[:8] + [131072] + good[9:]), None) == ESIZE
-    good = [P, P, P, P, P, P, 1, 4, 33, 128, P]
-    assert lib.dmoq_int8_gated_gemm(*(good[:7] + [0] + good[8:]), None) == OK
-    for i in (0, 1, 2, 3, 4, 5, 10):
-        assert lib.dmoq_int8_gated_gemm(*(good[:i] + [None] + good[i + 1:]), None) == EINVAL
-    assert lib.dmoq_int8_gated_gemm(*(good[:9] + [1 << 20] + good[10:]), None) == ESIZE
+    #       codes scales w pitch scale bias bf16 T N K out
+    good = [P, P, P, 128, P, None, 1, 4, 33, 128, P]
+    each(lib.dmoq_int8_gemm, good, OK, [(7, 0)])
+    each(lib.dmoq_int8_gemm, good, EINVAL, [(i, None) for i in (0, 1, 2, 4, 10)])
+    each(lib.dmoq_int8_gemm, good, EINVAL, [(0, ODD), (2, ODD), (3, 112), (3, 136), (7, -1), (8, 0), (9, 8), (9, 0), (9, 136)])
+    each(lib.dmoq_int8_gemm, good, ESIZE, [(9, 131072), (7, (1 << 30) + 1), (8, (1 << 30) + 1)])
+    #       codes scales gate pitch scale up pitch scale bf16 T I K out
+    good = [P, P, P, 128, P, P, 128, P, 1, 4, 33, 128, P]
+    each(lib.dmoq_int8_gated_gemm, good, OK, [(9, 0)])
+    each(lib.dmoq_int8_gated_gemm, good, EINVAL, [(i, None) for i in (0, 1, 2, 4, 5, 7, 12)] + [(3, 112), (6, 136), (2, ODD), (5, ODD)])
+    each(lib.dmoq_int8_gated_gemm, good, ESIZE, [(11, 1 << 20)])
     # with the quantiser in front nothing is launched before everything is known to be right
-    good = [P, 1, 128, P, P, None, 40, 33, 128, P, P]
-    for i, v in ((0, None), (2, 127), (3, None), (4, None), (7, 0), (8, 100), (9, None), (10, None), (3, ODD), (9, ODD)):
-        assert lib.dmoq_int8_linear(*(good[:i] + [v] + good[i + 1:]), None) == EINVAL, (i, v)
-    assert lib.dmoq_int8_linear(*(good[:2] + [131072, P, P, None, 40, 33, 131072] + good[9:]), None) == ESIZE
-    good = [P, 1, 128, P, P, P, P, 40, 33, 128, P, P]
-    for i in (0, 3, 4, 5, 6, 10, 11):
-        assert lib.dmoq_int8_gated_linear(*(good[:i] + [None] + good[i + 1:]), None) == EINVAL, i
+    #       x bf16 pitch w pitch scale bias T N K scratch out
+    good = [P, 1, 128, P, 128, P, None, 40, 33, 128, P, P]
+    each(lib.dmoq_int8_linear, good, EINVAL, [(0, None), (2, 127), (3, None), (4, 100), (5, None), (8, 0), (9, 100), (10, None), (11, None),
+                                              (3, ODD), (10, ODD)])
+    each(lib.dmoq_int8_linear, good, ESIZE, [(9, 131072)])
+    #       x bf16 pitch gate pitch scale up pitch scale T I K scratch out
+    good = [P, 1, 128, P, 128, P, P, 128, P, 40, 33, 128, P, P]
+    each(lib.dmoq_int8_gated_linear, good, EINVAL, [(i, None) for i in (0, 3, 5, 6, 8, 12, 13)] + [(4, 120), (7, 96)])
 
 
 def test_int8_scratch_size():
@@ -58,23 +63,19 @@ def test_int8_scratch_size():
 
 def test_gated_ffn_refuses():
     lib = _lib.load()
-    good = [P, 1, 64, P, P, P, 4, 64, 32, P, 64, None, P]
-    assert lib.dmoq_gated_ffn(*(good[:6] + [0] + good[7:]), None) == OK
-    for i in (0, 3, 4, 5, 9, 12):
-        assert lib.dmoq_gated_ffn(*(good[:i] + [None] + good[i + 1:]), None) == EINVAL, i
-    for i, v in ((2, 60), (2, 68), (7, 60), (7, 0), (8, 12), (8, 0), (6, -4), (11, ODD), (10, 24), (10, 36), (0, ODD), (3, ODD), (4, ODD), (5, ODD),
-                 (9, ODD), (12, ODD)):
-        assert lib.dmoq_gated_ffn(*(good[:i] + [v] + good[i + 1:]), None) == EINVAL, (i, v)
-    for i in (7, 8):
-        assert lib.dmoq_gated_ffn(*(good[:i] + [(1 << 29) + 8] + good[i + 1:]), None) == ESIZE
-    #       dy pitch x bf pitch wg wu wd  T   H   I  h pitch saved dgu pitch dx dwg dwu dwd
-    good = [P, 64, P, 1, 64, P, P, P, 4, 64, 32, P, 32, P, P, 64, P, P, P, P]
-    for i in (0, 2, 5, 6, 7, 11, 13, 14):
-        assert lib.dmoq_gated_ffn_backward(*(good[:i] + [None] + good[i + 1:]), None) == EINVAL, i
-    for i, v in ((1, 60), (4, 60), (9, 4), (10, 12), (0, ODD), (2, ODD), (11, ODD), (12, 24), (13, ODD), (14, ODD), (15, 56), (15, 68),
-                 (16, ODD), (17, ODD), (19, ODD)):
-        assert lib.dmoq_gated_ffn_backward(*(good[:i] + [v] + good[i + 1:]), None) == EINVAL, (i, v)
-    assert lib.dmoq_gated_ffn_backward(*(good[:8] + [(1 << 26) + 1] + good[9:]), None) == ESIZE
+    #       x bf pitch wg  p   wu  p   wd  p   T  H   I   h  p   saved y
+    good = [P, 1, 64, P, 64, P, 64, P, 32, 4, 64, 32, P, 64, None, P]
+    each(lib.dmoq_gated_ffn, good, OK, [(9, 0)])
+    each(lib.dmoq_gated_ffn, good, EINVAL, [(i, v) for i in (0, 3, 5, 7, 12, 15) for v in (None, ODD)] + [(14, ODD)])
+    each(lib.dmoq_gated_ffn, good, EINVAL, [(2, 60), (2, 68), (4, 56), (6, 68), (8, 24), (13, 24), (13, 36), (10, 60), (10, 0), (11, 12), (11, 0),
+                                            (9, -4)])
+    each(lib.dmoq_gated_ffn, good, ESIZE, [(10, (1 << 29) + 8), (11, (1 << 29) + 8)])
+    #       dy p  x bf p  wg  p   wu  p   wd  p   T  H   I   h  p saved dgu p dx dwg dwu dwd
+    good = [P, 64, P, 1, 64, P, 64, P, 64, P, 32, 4, 64, 32, P, 32, P, P, 64, P, P, P, P]
+    each(lib.dmoq_gated_ffn_backward, good, EINVAL, [(i, v) for i in (0, 2, 5, 7, 9, 14, 16, 17) for v in (None, ODD)])
+    each(lib.dmoq_gated_ffn_backward, good, EINVAL, [(19, ODD), (20, ODD), (22, ODD), (1, 60), (4, 60), (6, 56), (8, 68), (10, 24), (12, 4),
+                                                     (13, 12), (15, 24), (18, 56), (18, 68)])
+    each(lib.dmoq_gated_ffn_backward, good, ESIZE, [(11, (1 << 26) + 1)])
 
 
 def test_functions_refuse_cpu_tensors():

@@ -266,6 +266,31 @@ def test_ffn_computes_only_the_gradients_that_are_needed():
                 R.close(v.grad, want[names[i]], ROUNDINGS[names[i]], f"{names[i]} (mask {mask})")
 
 
+@pytest.mark.parametrize("t", (3, 12, 70, 300, 2000))
+def test_weights_that_are_parts_of_larger_matrices(t):
+    """Row pitches of the weights (a shard of the columns of a matrix, halves of a joined one) in every kernel."""
+    g = rng(40 + t)
+    x, (w, ws), (w2, ws2) = acts(g, t, 528, torch.bfloat16), weight8(g, 1050, 1056), weight8(g, 1050, 544)
+    a, b = w[:, 16:544], w2[:, :528]
+    assert torch.equal(dense.int8_linear(x, a, ws), dense.int8_linear(x, a.contiguous(), ws))
+    assert torch.equal(dense.int8_gated_linear(x, a, ws, b, ws2), dense.int8_gated_linear(x, a.contiguous(), ws, b.contiguous(), ws2))
+    codes, scale = dense.quantize_int8_tokens(x)
+    assert torch.equal(dense.int8_matmul(codes, scale, a, ws), dense.int8_linear(x, a, ws))
+    joined = randn(g, 2 * 520, 544, scale=0.05, dtype=torch.bfloat16).requires_grad_(True)
+    down = randn(g, 528, 1040, scale=0.05, dtype=torch.bfloat16).requires_grad_(True)
+    x.requires_grad_(True)
+    dy = randn(g, t, 528, dtype=torch.bfloat16)
+    views = joined[:520, 8:536], joined[520:, 8:536], down[:, 512:1032]
+    y = dense.gated_feed_forward(x, *views)
+    dx, dj, dd = torch.autograd.grad(y, (x, joined, down), dy)
+    flat = [v.detach().contiguous().requires_grad_(True) for v in views]
+    want = dense.gated_feed_forward(x, *flat)
+    grads = torch.autograd.grad(want, [x] + flat, dy)
+    assert torch.equal(y, want) and torch.equal(dx, grads[0])
+    assert torch.equal(dj[:, 8:536], torch.cat(grads[1:3])) and torch.equal(dd[:, 512:1032], grads[3])
+    R.close(y, R.ffn(x, *flat)[3], ROUNDINGS["y"], "y")
+
+
 def test_ffn_empty_shapes_strides_and_refusals():
     x, wg, wu, wd, dy = ffn_inputs(24, 264, 136, torch.float16, seed=4)
     leaves = [v.requires_grad_(True) for v in (x[:0].detach(), wg, wu, wd)]
@@ -352,7 +377,7 @@ def test_outputs_stay_inside_their_memory():
         need = max(int(lib.dmoq_int8_scratch_bytes(t, n, k, 0)), int(lib.dmoq_int8_scratch_bytes(t, n, k, 1)), 16)
         scratch = torch.full((need + 256,), 99, dtype=torch.uint8, device=DEV)
         p = lambda v: C.c_void_p(v.data_ptr())  # noqa: E731
-        for name, extra in (("dmoq_int8_linear", (p(w), p(ws), None)), ("dmoq_int8_gated_linear", (p(w), p(ws), p(w), p(ws)))):
+        for name, extra in (("dmoq_int8_linear", (p(w), k, p(ws), None)), ("dmoq_int8_gated_linear", (p(w), k, p(ws), p(w), k, p(ws)))):
             _lib.check(getattr(lib, name)(p(x), 1, k, *extra, t, n, k, p(scratch[128:]), p(out[1]), None), name)
             torch.cuda.synchronize()
             assert (out[0] == 7.0).all() and (out[-1] == 7.0).all() and torch.isfinite(out).all()
@@ -363,8 +388,8 @@ def test_outputs_stay_inside_their_memory():
     hid, saved, y = pad(t, i), pad(3 * t, i), pad(t, h)
     dgu, dx, dw, dwd = pad(t, 2 * i), pad(t, h), pad(2 * i, h), pad(h, i)
     q = lambda v: C.c_void_p(v[1].data_ptr())  # noqa: E731
-    _lib.check(lib.dmoq_gated_ffn(p(x), 1, h, p(wg), p(wu), p(wd), t, h, i, q(hid), i, q(saved), q(y), None), "ffn")
-    _lib.check(lib.dmoq_gated_ffn_backward(p(dy), h, p(x), 1, h, p(wg), p(wu), p(wd), t, h, i, q(hid), i, q(saved), q(dgu), 2 * i, q(dx), q(dw),
+    _lib.check(lib.dmoq_gated_ffn(p(x), 1, h, p(wg), h, p(wu), h, p(wd), i, t, h, i, q(hid), i, q(saved), q(y), None), "ffn")
+    _lib.check(lib.dmoq_gated_ffn_backward(p(dy), h, p(x), 1, h, p(wg), h, p(wu), h, p(wd), i, t, h, i, q(hid), i, q(saved), q(dgu), 2 * i, q(dx), q(dw),
                                            C.c_void_p(dw[1 + i].data_ptr()), q(dwd), None), "ffn backward")
     torch.cuda.synchronize()
     for v in (hid, saved, y, dgu, dx, dw, dwd):
@@ -372,7 +397,7 @@ def test_outputs_stay_inside_their_memory():
     R.close(dw[1:1 + 2 * i], torch.cat([R.ffn_grads(x, wg, wu, wd, dy)[k] for k in ("dw_gate", "dw_up")]), 2, "dw")
     # the gradients of the two projections in memory that is not adjacent: two products
     a, b = pad(i, h), pad(i, h)
-    _lib.check(lib.dmoq_gated_ffn_backward(p(dy), h, p(x), 1, h, None, None, p(wd), t, h, i, None, 0, q(saved), q(dgu), 2 * i, None, q(a), q(b),
+    _lib.check(lib.dmoq_gated_ffn_backward(p(dy), h, p(x), 1, h, None, 0, None, 0, p(wd), i, t, h, i, None, 0, q(saved), q(dgu), 2 * i, None, q(a), q(b),
                                            None, None), "ffn backward")
     torch.cuda.synchronize()
     assert torch.equal(a[1:-1], dw[1:1 + i]) and torch.equal(b[1:-1], dw[1 + i:1 + 2 * i])
