@@ -61,7 +61,7 @@ template <int KIND, int EPI>
 __device__ __forceinline__ void finish(const Args& a, long long row, int col, uint32_t v0, uint32_t v1, float sa, float (&o)[3]) {
   const float x = (KIND == KIND_I8) ? scaled(v0, sa, a.b_scale[0][col]) : __uint_as_float(v0);
   const float y = !is_dual(EPI) ? 0.f : (KIND == KIND_I8) ? scaled(v1, sa, a.b_scale[1][col]) : __uint_as_float(v1);
-  if (EPI == EPI_OUT || EPI == EPI_GRAD) {
+  if (EPI == EPI_OUT) {
     o[0] = x;
   } else if (EPI == EPI_SCALE) {
     o[0] = a.bias ? __fadd_rn(x, unpack16(a.bias[col], a.bf16)) : x;

@@ -270,7 +270,8 @@ int check_ffn(int T, int H, int I) {
 // the kernel makes them itself.
 int int8_product(const void* x, long long x_pitch, int8_t* codes, long long code_pitch, float* scales, const Weight8& w, const Weight8* up,
                  const void* bias, int bf16, int T, int N, int K, void* out, cudaStream_t s) {
-  const bool few = few_tokens(T, (long long)N * K * (up ? 2 : 1)), fuse = x != nullptr && few_can_fuse(T, K, N, up != nullptr);   // fuse implies few
+  const bool few = few_tokens(T, (long long)N * K * (up ? 2 : 1));
+  const bool fuse = x != nullptr && few_can_fuse(T, K, N, up != nullptr);   // implies few
   if (x != nullptr && !fuse) {
     const int rc = dmoq_token_quant_launch(x, bf16, T, K, x_pitch, codes, code_pitch, scales, s);
     if (rc != DMOQ_OK) return rc;
@@ -286,7 +287,8 @@ int int8_product(const void* x, long long x_pitch, int8_t* codes, long long code
   a.ld_out = N;
   a.vec = vec4(out, N, N);
   if (few)
-    return few_product(KIND_I8, p.epi, fuse ? x : codes, fuse ? 2 * x_pitch : code_pitch, w.w, w.pitch, up ? up->w : nullptr, up ? up->pitch : 0, a, s);
+    return few_product(KIND_I8, p.epi, fuse ? x : codes, fuse ? 2 * x_pitch : code_pitch, w.w, w.pitch, up ? up->w : nullptr,
+                       up ? up->pitch : 0, a, s);
   p.a[0] = {codes, T, K, code_pitch};
   p.b[0] = {w.w, N, K, w.pitch};
   if (up) p.b[1] = {up->w, N, K, up->pitch};
@@ -365,7 +367,8 @@ extern "C" int dmoq_int8_gated_linear(const void* x, int32_t is_bf16, int64_t x_
 }
 
 extern "C" int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate, int64_t gate_pitch, const void* w_up,
-                              int64_t up_pitch, const void* w_down, int64_t down_pitch, int32_t T, int32_t H, int32_t I, void* h, int64_t h_pitch, void* saved, void* y, void* stream) {
+                              int64_t up_pitch, const void* w_down, int64_t down_pitch, int32_t T, int32_t H, int32_t I,
+                              void* h, int64_t h_pitch, void* saved, void* y, void* stream) {
   const int size = check_ffn(T, H, I);
   if (size != DMOQ_OK || T == 0) return size;
   DMOQ_CHECK_ARG(rows_usable(x, x_pitch, H) && rows_usable(w_gate, gate_pitch, H) && rows_usable(w_up, up_pitch, H) &&
@@ -383,8 +386,9 @@ extern "C" int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, c
   up.args.ld_out = h_pitch;
   up.args.ld_saved = I;
   const long long w_bytes = 2LL * H * I;
-  int rc = few_tokens(T, 2 * w_bytes) && !saved ? few_product(KIND_16, EPI_SILU, x, 2 * x_pitch, w_gate, 2 * gate_pitch, w_up, 2 * up_pitch, up.args, s)
-                                               : run(up, s);
+  int rc = few_tokens(T, 2 * w_bytes) && !saved
+               ? few_product(KIND_16, EPI_SILU, x, 2 * x_pitch, w_gate, 2 * gate_pitch, w_up, 2 * up_pitch, up.args, s)
+               : run(up, s);
   if (rc != DMOQ_OK) return rc;
   Product down;
   down.a[0] = {h, T, I, h_pitch};
@@ -396,7 +400,8 @@ extern "C" int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, c
 }
 
 extern "C" int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate,
-                                       int64_t gate_pitch, const void* w_up, int64_t up_pitch, const void* w_down, int64_t down_pitch, int32_t T, int32_t H, int32_t I, const void* h,
+                                       int64_t gate_pitch, const void* w_up, int64_t up_pitch, const void* w_down, int64_t down_pitch, int32_t T,
+                                       int32_t H, int32_t I, const void* h,
                                        int64_t h_pitch, const void* saved, void* d_gate_up, int64_t d_pitch, void* dx, void* dw_gate, void* dw_up,
                                        void* dw_down, void* stream) {
   const int size = check_ffn(T, H, I);

@@ -116,9 +116,6 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
                "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
                : "memory");
 }
-__device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) {
-  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
-}
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }

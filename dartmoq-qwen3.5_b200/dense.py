@@ -24,13 +24,13 @@ from . import _lib
 
 _BF16, _FP16, _FP32, _INT8 = torch.bfloat16, torch.float16, torch.float32, torch.int8
 _MAX_ROWS = 1 << 30
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _call(name: str, index: int, *args) -> None:
     """One entry point on the current stream of device ``index``, which is current during the call."""
     fn = getattr(_lib.load(), name)
-    if index == torch.cuda.current_device():
+    if index == _current_device():
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -53,6 +53,14 @@ def _rows(t: torch.Tensor, cols: int) -> Tuple[torch.Tensor, int, int]:
             return t, n, pitch
         t = t.clone(memory_format=torch.contiguous_format)
     return t, n, cols
+
+
+def _matrix(w: torch.Tensor, cols: int) -> Tuple[torch.Tensor, int]:
+    """A matrix of ``cols`` columns as the kernels can read it, and its pitch."""
+    if w.is_contiguous() and not w.data_ptr() & 15:
+        return w, cols
+    w, _, pitch = _rows(w, cols)
+    return w, pitch
 
 
 def _need(cond: bool, message: str) -> None:
@@ -79,13 +87,14 @@ def _weight8(w: torch.Tensor, scale: torch.Tensor, k: int, index: int, what: str
     if w.dtype is not _INT8 or scale.dtype is not _FP32:
         raise TypeError(f"{what} must be int8 with an fp32 scale, got {w.dtype} and {scale.dtype}")
     shape = w.shape
-    if len(shape) != 2 or shape[1] != k or shape[0] < 1:
-        raise ValueError(f"{what} must have shape (outputs, {k}), got {tuple(shape)}")
+    if len(shape) != 2 or shape[1] != k or not 1 <= shape[0] <= _MAX_ROWS:
+        raise ValueError(f"{what} must have shape (outputs, {k}) with at most 2^30 outputs, got {tuple(shape)}")
     if scale.shape != shape[:1]:
         raise ValueError(f"{what} needs one scale a row: {shape[0]} rows, scales of shape {tuple(scale.shape)}")
     if w.get_device() != index or scale.get_device() != index:      # -1 on the CPU
         raise ValueError(f"{what} and its scale must be on cuda:{index}")
-    return *_rows(w, k), scale if scale.is_contiguous() else scale.contiguous()
+    w, pitch = _matrix(w, k)
+    return w, shape[0], pitch, scale if scale.is_contiguous() else scale.contiguous()
 
 
 def _bias_ptr(bias: Optional[torch.Tensor], n: int, dtype: torch.dtype, index: int):
@@ -156,7 +165,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     bias, bias_ptr = _bias_ptr(bias, n, x.dtype, index)
     rows, t, pitch = _rows(x, k)
     scratch = _int8_scratch(x, t, n, k, False)
-    out = x.new_empty(shape[:-1] + (n,))
+    out = x.new_empty((t, n) if len(shape) == 2 else shape[:-1] + (n,))
     _call("dmoq_int8_linear", index, rows.data_ptr(), x.dtype is _BF16, pitch, w.data_ptr(), w_pitch, ws.data_ptr(), bias_ptr, t, n, k,
           _ptr(scratch), out.data_ptr())
     return out
@@ -181,7 +190,7 @@ def int8_gated_linear(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.T
         raise ValueError(f"w_gate and w_up must have one shape, got {tuple(w_gate.shape)} and {tuple(w_up.shape)}")
     rows, t, pitch = _rows(x, k)
     scratch = _int8_scratch(x, t, n, k, True)
-    out = x.new_empty(shape[:-1] + (n,))
+    out = x.new_empty((t, n) if len(shape) == 2 else shape[:-1] + (n,))
     _call("dmoq_int8_gated_linear", index, rows.data_ptr(), x.dtype is _BF16, pitch, wg.data_ptr(), gate_pitch, sg.data_ptr(),
           wu.data_ptr(), up_pitch, su.data_ptr(), t, n, k, _ptr(scratch), out.data_ptr())
     return out
@@ -190,9 +199,9 @@ def int8_gated_linear(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.T
 def _ffn_forward(x: torch.Tensor, t: int, pitch: int, wg: torch.Tensor, wu: torch.Tensor, wd: torch.Tensor, save: bool):
     """y, and the hidden values h; with ``save`` also what the gradients need of them."""
     hidden, inter = wd.shape
-    wg, _, gate_pitch = _rows(wg, hidden)
-    wu, _, up_pitch = _rows(wu, hidden)
-    wd, _, down_pitch = _rows(wd, inter)
+    wg, gate_pitch = _matrix(wg, hidden)
+    wu, up_pitch = _matrix(wu, hidden)
+    wd, down_pitch = _matrix(wd, inter)
     h = x.new_empty((t, (inter + 63) & -64))       # rows on whole 128-byte lines
     saved = x.new_empty((3, t, inter), dtype=torch.int16) if save else None
     y = x.new_empty((t, hidden))
@@ -228,12 +237,12 @@ def _ffn_backward(ctx, dy):
     dy, t, dy_pitch = _rows(dy, hidden)
     # saved-tensor hooks may have laid them out anew
     x, _, x_pitch = _rows(x, hidden)
-    wg, _, gate_pitch = _rows(wg, hidden)
-    wu, _, up_pitch = _rows(wu, hidden)
-    wd, _, down_pitch = _rows(wd, inter)
+    wg, gate_pitch = _matrix(wg, hidden)
+    wu, up_pitch = _matrix(wu, hidden)
+    wd, down_pitch = _matrix(wd, inter)
     h_pitch = 0
     if h is not None:
-        h, _, h_pitch = _rows(h, h.shape[1])
+        h, h_pitch = _matrix(h, h.shape[1])
     if saved is not None:
         saved = saved.contiguous()
     d_pitch = (2 * inter + 63) & -64
@@ -266,8 +275,8 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     if w_gate.shape != (inter, hidden) or w_up.shape != (inter, hidden) or w_down.shape != (hidden, inter):
         raise ValueError(f"for x of {hidden} columns the weights must be (I, {hidden}) twice and ({hidden}, I), got {tuple(w_gate.shape)}, "
                          f"{tuple(w_up.shape)}, {tuple(w_down.shape)}")
-    if hidden < 8 or inter < 8 or (hidden | inter) & 7:
-        raise ValueError(f"hidden and intermediate sizes must be multiples of 8, got {hidden} and {inter}")
+    if hidden < 8 or inter < 8 or (hidden | inter) & 7 or hidden | inter >= 1 << 30:
+        raise ValueError(f"hidden and intermediate sizes must be multiples of 8 below 2^30, got {hidden} and {inter}")
     if w_gate.get_device() != index or w_up.get_device() != index or w_down.get_device() != index:
         raise ValueError(f"all weights must be on cuda:{index}")
     rows = x if x.dim() == 2 else x.reshape(-1, hidden)
