@@ -291,6 +291,25 @@ def test_weights_that_are_parts_of_larger_matrices(t):
     R.close(y, R.ffn(x, *flat)[3], ROUNDINGS["y"], "y")
 
 
+def test_ffn_gradients_of_shared_and_broadcast_arguments():
+    """One weight for both projections; a token repeated without memory of its own; a weight of repeated rows."""
+    _, wg, wu, wd, dy = ffn_inputs(50, 136, 264, torch.bfloat16, seed=13)
+    token = randn(rng(14), 1, 136, dtype=torch.bfloat16).requires_grad_(True)
+    row = randn(rng(15), 1, 136, scale=0.1, dtype=torch.bfloat16).requires_grad_(True)
+    w, wd = wg.requires_grad_(True), wd.requires_grad_(True)
+    x = token.expand(50, 136)
+    for gate, up in ((w, w), (row.expand(264, 136), w)):
+        leaves = [token, w, wd] + ([row] if gate is not w else [])
+        grads = torch.autograd.grad(dense.gated_feed_forward(x, gate, up, wd), leaves, dy)
+        want = R.ffn_grads(x, gate, up, wd, dy)
+        # sums over 50 tokens or 264 rows of gradients that were rounded once: one more rounding of the sum itself
+        R.close(grads[0], want["dx"].sum(0, keepdim=True), ROUNDINGS["dx"] + 1, "token")
+        R.close(grads[1], want["dw_gate"] + want["dw_up"] if gate is w else want["dw_up"], ROUNDINGS["dw_up"] + 1, "weight")
+        R.close(grads[2], want["dw_down"], ROUNDINGS["dw_down"], "dw_down")
+        if gate is not w:
+            R.close(grads[3], want["dw_gate"].sum(0, keepdim=True), ROUNDINGS["dw_gate"] + 1, "row")
+
+
 def test_ffn_empty_shapes_strides_and_refusals():
     x, wg, wu, wd, dy = ffn_inputs(24, 264, 136, torch.float16, seed=4)
     leaves = [v.requires_grad_(True) for v in (x[:0].detach(), wg, wu, wd)]
