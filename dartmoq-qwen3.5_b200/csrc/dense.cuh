@@ -49,8 +49,21 @@ struct Args {
 
 // The arithmetic of the epilogues, with its roundings spelled out (no contraction left to the compiler), so that an 8-bit result
 // does not depend on the kernel that a batch's size selects.
-__device__ __forceinline__ float scaled(uint32_t sum, float token_scale, float row_scale) {
+//
+// sum * token_scale * row_scale: the scales are multiplied first.  With either outside 2^-60 .. 2^48 their product may leave the
+// normal 32-bit numbers although the result does not (a subnormal factor of 1e-45 times a sum of 1e8, infinity times a sum of
+// zero), and neither other order of two products holds everywhere; there the three are multiplied in 64 bits, whose range holds
+// any of them.  The rule looks at the element's own scales alone: its result is the same in every batch and every kernel.
+__device__ __forceinline__ bool plain_scale(float s) {
+  const uint32_t magnitude = __float_as_uint(s) & 0x7fffffffu;
+  return magnitude - (67u << 23) < (108u << 23) || magnitude == 0u;
+}
+__device__ __forceinline__ float scaled_plain(uint32_t sum, float token_scale, float row_scale) {
   return __fmul_rn((float)(int)sum, __fmul_rn(token_scale, row_scale));
+}
+__device__ __forceinline__ float scaled(uint32_t sum, float token_scale, float row_scale) {
+  if (plain_scale(token_scale) && plain_scale(row_scale)) return scaled_plain(sum, token_scale, row_scale);
+  return __double2float_rn(__dmul_rn(__dmul_rn((double)(int)sum, (double)token_scale), (double)row_scale));
 }
 __device__ __forceinline__ float gated(float g, float u) { return __fmul_rn(__fmul_rn(g, sigmoid(g)), u); }
 // silu'(g) = s (1 + g (1 - s)) = s + silu(g) (1 - s), s = sigmoid(g)

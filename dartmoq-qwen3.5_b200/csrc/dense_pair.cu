@@ -297,6 +297,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) dense_p
             asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
           }
         }
+        if (KIND == KIND_I8) {                             // sums -> values; one look at all of the block's scales (see scaled)
+          auto values = [&](auto&& scale) {
+#pragma unroll
+            for (int q = 0; q < 32; ++q) {
+              v[q] = __float_as_uint(scale(v[q], sa, __shfl_sync(0xffffffffu, sc0, q)));
+              if (kDual) w[q] = __float_as_uint(scale(w[q], sa, __shfl_sync(0xffffffffu, sc1, q)));
+            }
+          };
+          if (__all_sync(0xffffffffu, plain_scale(sa) && plain_scale(sc0) && plain_scale(sc1)))
+            values([](uint32_t sum, float s, float r) { return scaled_plain(sum, s, r); });
+          else
+            values([](uint32_t sum, float s, float r) { return scaled(sum, s, r); });
+        }
         uint32_t o[outputs_of(EPI)][16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
@@ -304,14 +317,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) dense_p
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int q = 2 * j + h;
-            if (KIND == KIND_I8) {
-              x[h] = scaled(v[q], sa, __shfl_sync(0xffffffffu, sc0, q));
-              if (kDual) y[h] = scaled(w[q], sa, __shfl_sync(0xffffffffu, sc1, q));
-              if (EPI == EPI_SCALE && a.bias) x[h] = __fadd_rn(x[h], __shfl_sync(0xffffffffu, bias, q));
-            } else {
-              x[h] = __uint_as_float(v[q]);
-              if (kDual) y[h] = __uint_as_float(w[q]);
-            }
+            x[h] = __uint_as_float(v[q]);
+            if (kDual) y[h] = __uint_as_float(w[q]);
+            if (EPI == EPI_SCALE && a.bias) x[h] = __fadd_rn(x[h], __shfl_sync(0xffffffffu, bias, q));
           }
           if (EPI == EPI_OUT || EPI == EPI_SCALE) {
             o[0][j] = pack16(x[0], x[1], a.bf16);

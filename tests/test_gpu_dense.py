@@ -136,6 +136,37 @@ def test_int8_sums_are_exact_at_the_largest_inner_size():
         dense.int8_matmul(wide, torch.ones(1, device=DEV), wide, one[:1])
 
 
+@pytest.mark.parametrize("t", (1, 12, 40, 200, 2500))
+def test_int8_scales_whose_product_leaves_the_32_bit_range(t):
+    """Token and row scales far apart: their product alone underflows or overflows, the result does not."""
+    g = rng(90 + t)
+    n, k = 300, 528
+    codes = torch.randint(-127, 128, (t, k), generator=g).to(torch.int8).to(DEV)
+    w = torch.randint(-127, 128, (n, k), generator=g).to(torch.int8).to(DEV)
+    w[5] = 0                                                        # sums of zero
+    scale = torch.tensor([7.9e-33, 2.0 ** -61, 2e36, 1.0, 0.0, 3e-41, 1e20])[torch.arange(t) % 7].to(DEV)
+    row = torch.tensor([1e-12, 1e3, 2.0 ** 48, 0.01, 1e-38, 3e24, 2.0 ** -75, 0.0])[torch.arange(n) % 8].to(DEV)
+    y = dense.int8_matmul(codes, scale, w, row)
+    sums = codes.double() @ w.double().t()
+    want = (sums * scale.double()[:, None] * row.double()).cpu()
+    got, fi = y.double().cpu(), torch.finfo(torch.bfloat16)
+    finite = want.abs() < fi.max + 2.0 ** 119                       # half a step beyond the largest number rounds to it
+    # one rounding to 16 bits, four to 32 (the sum, two products, the result); below the normal numbers a step is not relative
+    tol = want.abs() * (2.0 ** -8 + 4 * 2.0 ** -24) + fi.smallest_normal * fi.eps
+    assert ((got - want).abs() <= tol)[finite].all()
+    assert torch.equal(got[~finite], torch.sign(want[~finite]) * float("inf"))
+    assert torch.equal(y[:, 3::8][3::7], dense.int8_matmul(codes[3::7], scale[3::7], w[3::8], row[3::8]))   # whatever the neighbours are
+    # gates: tokens 2^-100 times as large and row scales 2^100 times as large leave the 64-bit values as they are
+    x, (wg, sg), (wu, su) = acts(g, t, k, torch.bfloat16), weight8(g, n, k), weight8(g, n, k)
+    h = dense.int8_gated_linear(x * 2.0 ** -100, wg, sg * 2.0 ** 100, wu, su * 2.0 ** 100)
+    q, s = R.quantize(x)
+    gate, up = ((q @ m.double().cpu().t()) * s[:, None] * sm.double().cpu() for m, sm in ((wg, sg), (wu, su)))
+    want = R.silu(gate) * up
+    e32 = 2.0 ** -24 * (4 * (1 + gate.abs()) + 4 + 2 * (2 + gate.abs()) + 5)     # as for int8_gated_linear
+    assert ((h.double().cpu() - want).abs() <= want.abs() * (2.0 ** -8 * (1 + e32) + e32) + fi.smallest_normal * fi.eps).all()
+    healthy()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("t,n,k", SIZES8)
 def test_int8_gated_linear(t, n, k, dtype):
