@@ -210,8 +210,13 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16) {
 __device__ __forceinline__ float unpack16(uint32_t bits16, bool bf16) {
   return bf16 ? __uint_as_float(bits16 << 16) : __half2float(__ushort_as_half((unsigned short)bits16));
 }
-// sigmoid in fp32: 2 special-function instructions; the relative error of a few 2^-22 is far below the 16-bit rounding
-// of what is made of it
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+// sigmoid in fp32: 2 special-function instructions.  The exponential is off by at most 2 + 1.173 |x| units of 2^-23 (2^-19 of
+// the value at x = -12, 2^-16 at -90): below the 16-bit rounding of what is made of it.  Far below zero the quotient is the
+// exponential itself; there 1 + e^-x passes 2^126, where the fast division returns 0.
+__device__ __forceinline__ float sigmoid(float x) {
+  const bool low = x < -64.f;                // e^-64 is below half a unit of 1 + e^64
+  const float e = __expf(low ? x : -x);
+  return low ? e : __fdividef(1.f, 1.f + e);
+}
 
 }  // namespace dense

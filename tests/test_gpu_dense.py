@@ -187,6 +187,25 @@ def test_int8_gated_linear(t, n, k, dtype):
     healthy()
 
 
+@pytest.mark.parametrize("t", (1, 12, 40, 200, 2500))
+def test_gates_far_below_zero(t):
+    """silu(g) down to g = -95, where the sigmoid is a subnormal 32-bit number; an up value of 1e6 brings it back."""
+    n = 400
+    x = torch.zeros(t, 16, dtype=torch.bfloat16, device=DEV)
+    x[:, 0] = 127.0                                                  # code 127, scale 1
+    w = torch.zeros(n, 16, dtype=torch.int8, device=DEV)
+    w[:, 0] = 127
+    gate_scale = (-torch.linspace(0.0, 95.0, n) / 127 ** 2).to(DEV)
+    h = dense.int8_gated_linear(x, w, gate_scale, w, torch.full((n,), 1e6 / 127 ** 2, device=DEV))
+    gate, up = gate_scale.double().cpu() * 127 ** 2, float(torch.tensor(1e6 / 127 ** 2)) * 127 ** 2
+    want = R.silu(gate) * up
+    # relative: g carries two roundings, with silu's condition 1 + |g|, u two, the exponential 2 + 1.173 |g| units of 2^-23, five
+    # more; absolute: the sigmoid and g times it are held to a unit of 2^-149
+    e32 = 2.0 ** -24 * (2 * (1 + gate.abs()) + 2 + 2 * (2 + 1.173 * gate.abs()) + 5)
+    tol = want.abs() * (2.0 ** -8 * (1 + e32) + e32) + up * (2 * gate.abs() + 1) * 2.0 ** -149
+    assert ((h.double().cpu() - want).abs() <= tol).all()
+
+
 def test_int8_shapes_strides_and_refusals():
     g = rng(11)
     x = randn(g, 4, 6, 512, dtype=torch.bfloat16)
