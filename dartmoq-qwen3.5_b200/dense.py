@@ -80,6 +80,8 @@ def _check_input(x: torch.Tensor) -> None:
 def _check_k8(k: int) -> None:
     if k < 16 or k & 15:
         raise ValueError(f"8-bit products need an inner size that is a multiple of 16, got {k}")
+    if k > _MAX_ROWS:        # sizes travel as 32-bit numbers: a larger one would arrive as another
+        raise ValueError(f"at most 2^30 columns, got {k}")
 
 
 def _weight8(w: torch.Tensor, scale: torch.Tensor, k: int, index: int, what: str) -> Tuple[torch.Tensor, int, int, torch.Tensor]:

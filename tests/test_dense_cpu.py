@@ -89,6 +89,12 @@ def test_functions_refuse_cpu_tensors():
             call()
 
 
+@pytest.mark.parametrize("k", ((1 << 32) + 16, (1 << 31), (1 << 30) + 16))
+def test_inner_sizes_past_32_bits_are_refused(k):
+    with pytest.raises(ValueError, match="2\\^30"):
+        dense._check_k8(k)
+
+
 def test_w8a8_linear_plumbing():
     lin = D.W8A8Linear.from_metadata({"out_features": 33, "in_features": 64, "bias_shape": [33], "orig_dtype": "torch.float16"})
     assert set(lin.state_dict()) == {"weight", "weight_scale", "bias"}

@@ -136,6 +136,17 @@ def test_int8_sums_are_exact_at_the_largest_inner_size():
         dense.int8_matmul(wide, torch.ones(1, device=DEV), wide, one[:1])
 
 
+def test_inner_sizes_past_32_bits_are_refused():
+    """2^32 + 16 columns are not 16 (the tensors hold one element each)."""
+    k = (1 << 32) + 16
+    x = torch.ones(1, dtype=torch.bfloat16, device=DEV).expand(1, k)
+    w, one = torch.ones(1, dtype=torch.int8, device=DEV).expand(1, k), torch.ones(1, device=DEV)
+    for call in (lambda: dense.quantize_int8_tokens(x), lambda: dense.int8_linear(x, w, one), lambda: dense.int8_matmul(w, one, w, one),
+                 lambda: dense.int8_gated_linear(x, w, one, w, one)):
+        with pytest.raises(ValueError):
+            call()
+
+
 @pytest.mark.parametrize("t", (1, 12, 40, 200, 2500))
 def test_int8_scales_whose_product_leaves_the_32_bit_range(t):
     """Token and row scales far apart: their product alone underflows or overflows, the result does not."""
