@@ -18,8 +18,6 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
-
 from . import _lib
 
 _BF16, _FP16, _FP32, _INT8 = torch.bfloat16, torch.float16, torch.float32, torch.int8
@@ -228,8 +226,27 @@ class _GatedFeedForward(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        # grad mode is on only where a graph of the backward pass is asked for, which this has none of
-        return _ffn_backward_once(ctx, dy) if torch.is_grad_enabled() else _ffn_backward(ctx, dy)
+        if not torch.is_grad_enabled():
+            return _ffn_backward(ctx, dy)
+        # grad mode is on only where a graph of the backward pass is asked for, which this has none of.  The gradients depend on
+        # x and the weights whether or not dy requires one, so they always require one that raises.
+        with torch.no_grad():
+            grads = _ffn_backward(ctx, dy)
+        anchor = torch.empty(0, requires_grad=True)
+        marked = iter(_DifferentiableOnce.apply(anchor, *(g for g in grads if g is not None)))
+        return tuple(None if g is None else next(marked) for g in grads)
+
+
+class _DifferentiableOnce(torch.autograd.Function):
+    """Gradients as they are; asking for theirs raises."""
+
+    @staticmethod
+    def forward(ctx, anchor, *grads):
+        return tuple(g.detach() for g in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("gated_feed_forward is differentiable once: it has no second derivatives")
 
 
 def _ffn_backward(ctx, dy):
@@ -258,9 +275,6 @@ def _ffn_backward(ctx, dy):
     _call("dmoq_gated_ffn_backward", x.get_device(), dy.data_ptr(), dy_pitch, x.data_ptr(), x.dtype is _BF16, x_pitch, wg.data_ptr(),
           gate_pitch, wu.data_ptr(), up_pitch, wd.data_ptr(), down_pitch, t, hidden, inter, _ptr(h), h_pitch, _ptr(saved), _ptr(dgu), d_pitch, _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd))
     return dx, dwg, dwu, dwd
-
-
-_ffn_backward_once = once_differentiable(_ffn_backward)
 
 
 def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor) -> torch.Tensor:

@@ -404,6 +404,30 @@ def test_ffn_empty_shapes_strides_and_refusals():
         double.sum().backward()                                      # once differentiable
 
 
+def test_ffn_second_derivatives_raise_whatever_the_loss_is():
+    """A gradient of a gradient must never be left out in silence, also where the upstream gradient is a constant."""
+    x, wg, wu, wd, dy = ffn_inputs(24, 264, 136, torch.bfloat16, seed=16)
+    leaves = [v.requires_grad_(True) for v in (x, wg, wu, wd)]
+    want = torch.autograd.grad(dense.gated_feed_forward(*leaves), leaves, dy)
+    for loss in (lambda y: y.sum(), lambda y: (y * dy).sum(), lambda y: y.float().square().sum()):
+        y = dense.gated_feed_forward(*leaves)
+        g = torch.autograd.grad(loss(y), leaves, create_graph=True)
+        assert all(v.requires_grad for v in g)
+        for v in g:
+            with pytest.raises(RuntimeError, match="differentiable once"):
+                (loss(dense.gated_feed_forward(*leaves)) + v.float().square().sum()).backward()
+        for v in leaves:
+            v.grad = None
+    # the gradients themselves are what they are without a graph of them
+    g = torch.autograd.grad(dense.gated_feed_forward(*leaves), leaves, dy, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(g, want))
+    # only some arguments
+    frozen = [x.detach(), wg, wu.detach(), wd.detach()]
+    g, = torch.autograd.grad(dense.gated_feed_forward(*frozen).sum(), wg, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        g.float().sum().backward()
+
+
 def test_ffn_with_saved_tensors_moved_and_from_other_threads():
     """What is saved may come back from a hook laid out anew; calls may come from several threads and streams at once."""
     import threading
