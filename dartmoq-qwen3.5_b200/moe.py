@@ -310,7 +310,8 @@ class _Engine:
         self.E_v = self.E * self.mult
         self.k_v = self.top_k * self.mult
 
-        self.shared_expert = m.shared_expert      # another one assigned later makes a new engine
+        # modules this engine and the graphs captured from it were made with; _get_engine looks for others in their place
+        self.gate, self.shared_expert, self.shared_gate = m.gate, m.shared_expert, m.shared_expert_gate
         shared_packs = m._shared_packs()
         self.has_shared = shared_packs is not None
         self.shared_torch = (m.shared_expert is not None and m.shared_expert_gate is not None
@@ -860,10 +861,19 @@ class WxA16BitPartitionedGroupMoE(nn.Module):
 
     def _get_engine(self, device) -> _Engine:
         eng = self._engine
-        if eng is None or eng.device != device or eng.shared_expert is not self.shared_expert:
-            eng = _Engine(self, device)
-            self._engine = eng
-            self._graphs = None
+        if eng is not None:
+            shared, gate = self.shared_expert, self.shared_expert_gate
+            if eng.shared_expert is not shared or (eng.shared_gate is None) != (gate is None):
+                if eng.has_shared or self._shared_packs() is not None:
+                    eng = None                        # packed weights that the engine holds, or would
+                else:
+                    eng.shared_expert, eng.shared_torch = shared, shared is not None and gate is not None
+            if eng is not None and (eng.shared_gate is not gate or eng.gate is not self.gate):
+                eng.shared_gate, eng.gate = gate, self.gate
+                self._graphs = None                   # captured with the old gate's weights
+        if eng is None or eng.device != device:
+            eng = self._engine = self._graphs = None  # what they hold is given back before as much is taken again
+            eng = self._engine = _Engine(self, device)
         return eng
 
     def _body(self, eng, x, prof=None, partials=None):

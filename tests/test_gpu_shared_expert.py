@@ -1,0 +1,102 @@
+"""A layer's shared expert, its gate and its router assigned, replaced and removed between calls: eager, captured and replayed
+calls always compute what the module holds now."""
+import pytest
+import torch
+
+import dartmoq_b200 as D
+from dartmoq_b200 import synth
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+HIDDEN = 256
+
+
+def layer(seed=5, **kw):
+    return synth.build_layer(hidden=HIDDEN, n_experts=8, top_k=2, inter=128, bit_mix={2: 0.5, 4: 0.5}, seed=seed, **kw).to(DEV)
+
+
+def block(seed):
+    torch.manual_seed(seed)
+    return D.GatedFeedForward(HIDDEN, 384, device=DEV)
+
+
+def linear_gate(seed):
+    torch.manual_seed(seed)
+    return torch.nn.Linear(HIDDEN, 1, bias=False, dtype=torch.bfloat16, device=DEV)
+
+
+def tokens(n=40):
+    return synth.make_activations(n, HIDDEN, seed=3).to(DEV).unsqueeze(0)
+
+
+def calls(moe, x, want):
+    for _ in range(3):                              # eager, captured, replayed
+        assert torch.equal(moe(x), want)
+
+
+@torch.no_grad()
+def with_dense(routed, x, expert, gate):
+    return (routed[0] + expert(x[0]) * torch.sigmoid(gate(x[0]))).unsqueeze(0)
+
+
+@pytest.mark.parametrize("n", (40, 700))
+def test_dense_expert_and_gate_come_and_go(n):
+    x, moe = tokens(n), layer()
+    routed = moe(x).clone()
+    calls(moe, x, routed)
+    engine, a, b, ga, gb = moe._engine, block(1), block(2), linear_gate(3), linear_gate(4)
+    moe.shared_expert = a
+    calls(moe, x, routed)                           # no gate yet: the layer has no shared expert
+    moe.shared_expert_gate = ga
+    calls(moe, x, with_dense(routed, x, a, ga))
+    moe.shared_expert_gate = gb
+    calls(moe, x, with_dense(routed, x, a, gb))
+    moe.shared_expert = b
+    calls(moe, x, with_dense(routed, x, b, gb))
+    moe.shared_expert_gate = None
+    calls(moe, x, routed)
+    moe.shared_expert, moe.shared_expert_gate = None, ga
+    calls(moe, x, routed)
+    moe.shared_expert = a
+    calls(moe, x, with_dense(routed, x, a, ga))
+    assert moe._engine is engine                    # the routed experts' weights were laid out once
+
+
+@pytest.mark.parametrize("n", (40, 700))
+def test_gates_replaced_after_a_capture(n):
+    """The packed shared expert's gate and the router are part of the captured graph."""
+    x = tokens(n)
+    moe, fresh, other = layer(shared_inter=128), layer(shared_inter=128), layer(seed=6, shared_inter=128)
+    first = moe(x).clone()
+    calls(moe, x, first)
+    gate = linear_gate(7)
+    moe.shared_expert_gate = fresh.shared_expert_gate = gate
+    want = fresh(x).clone()
+    assert not torch.equal(want, first)
+    calls(moe, x, want)
+    moe.gate = other.gate
+    fresh = layer(shared_inter=128)
+    fresh.shared_expert_gate, fresh.gate = gate, other.gate
+    again = fresh(x).clone()
+    assert not torch.equal(again, want)
+    calls(moe, x, again)
+
+
+def test_packed_and_dense_experts_replace_one_another():
+    x = tokens()
+    moe, plain, other = layer(shared_inter=128), layer(shared_inter=128), layer(seed=6, shared_inter=128)
+    plain.shared_expert = None                      # the same routed experts
+    packed, gate = moe.shared_expert, moe.shared_expert_gate
+    with_packed, routed = moe(x).clone(), plain(x).clone()
+    calls(moe, x, with_packed)
+    dense = block(1)
+    moe.shared_expert = dense
+    calls(moe, x, with_dense(routed, x, dense, gate))
+    moe.shared_expert = packed
+    calls(moe, x, with_packed)
+    moe.shared_expert = other.shared_expert
+    fresh = layer(shared_inter=128)
+    fresh.shared_expert = other.shared_expert
+    calls(moe, x, fresh(x).clone())
+    moe.shared_expert_gate = None
+    calls(moe, x, routed)
