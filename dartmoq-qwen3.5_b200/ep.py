@@ -188,7 +188,8 @@ class ExpertParallelMoE(torch.nn.Module):
         self.num_experts, self.top_k = num_experts, top_k
         self.shared_expert, self.shared_expert_gate = shared_expert, shared_expert_gate
         self.group, self.exchange = group, exchange
-        self._shared_layer: list = []         # [module or None] once resolved; a list keeps it out of the submodules
+        # [module or None, the shared expert and the local module's class it was made from]; a list keeps them out of the submodules
+        self._shared_layer: list = []
         self._side_stream: list = []
         self._codes: list = []                # the code exchange's state
         self._full_meta = [full_layer] if exchange == "codes" else []
@@ -214,13 +215,15 @@ class ExpertParallelMoE(torch.nn.Module):
         caller then applies the torch modules)."""
         if self.shared_expert is None or self.shared_expert_gate is None or not x.is_cuda or x.shape[0] == 0:
             return None
-        if not self._shared_layer:
-            lm = self.local_moe
+        lm = self.local_moe
+        made = self._shared_layer
+        if not made or made[1] is not self.shared_expert or made[2] is not type(lm):
+            made.clear()                      # the old layer's memory is given back first
             layer = type(lm)(None, 1, lm.hidden_size, lm.intermediate_size, 1, self.shared_expert,
                              self.shared_expert_gate)
             layer.enable_timing = False
-            self._shared_layer.append(layer if layer._shared_packs() is not None else None)
-        layer = self._shared_layer[0]
+            made += [layer if layer._shared_packs() is not None else None, self.shared_expert, type(lm)]
+        layer = made[0]
         if layer is None:
             return None
         T = x.shape[0]

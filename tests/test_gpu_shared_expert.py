@@ -100,3 +100,32 @@ def test_packed_and_dense_experts_replace_one_another():
     calls(moe, x, fresh(x).clone())
     moe.shared_expert_gate = None
     calls(moe, x, routed)
+
+
+def test_expert_parallel_shared_expert_replaced():
+    """The wrapper's own layer of the shared expert follows the expert it holds and the local module's activation mode."""
+    from dartmoq_b200 import ep
+    x = tokens()[0]
+    a, b = layer(shared_inter=128), layer(seed=6, shared_inter=128)
+    gate = a.shared_expert_gate
+
+    def wrap(expert, cls=None):
+        local = ep.shard_experts(a, 0, 8)
+        if cls is not None:
+            cls.from_wxa16(local)
+        return ep.ExpertParallelMoE(a.gate, local, 8, 2, expert, gate)
+
+    w = wrap(a.shared_expert)
+    first = w._shared_partial(x).clone()
+    w.shared_expert = b.shared_expert
+    want = wrap(b.shared_expert)._shared_partial(x)
+    assert not torch.equal(want, first) and torch.equal(w._shared_partial(x), want)
+    w.shared_expert = block(1)
+    assert w._shared_partial(x) is None             # not packed: the caller applies the module
+    w.shared_expert = None
+    assert w._shared_partial(x) is None
+    w.shared_expert = a.shared_expert
+    assert torch.equal(w._shared_partial(x), first)
+    D.WxA8BitPartitionedGroupMoE.from_wxa16(w.local_moe)
+    eight = wrap(a.shared_expert, D.WxA8BitPartitionedGroupMoE)._shared_partial(x)
+    assert not torch.equal(eight, first) and torch.equal(w._shared_partial(x), eight)
