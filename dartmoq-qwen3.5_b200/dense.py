@@ -18,6 +18,8 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
+
 from . import _lib
 
 _BF16, _FP16, _FP32, _INT8 = torch.bfloat16, torch.float16, torch.float32, torch.int8
@@ -277,11 +279,15 @@ def _ffn_backward(ctx, dy):
     return dx, dwg, dwu, dwd
 
 
+def _has_tangent(*tensors: torch.Tensor) -> bool:
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor) -> torch.Tensor:
     """(silu(x w_gate^T) * (x w_up^T)) w_down^T for x (..., H), w_gate and w_up (I, H), w_down (H, I), all bf16 or all fp16; H and I
     multiples of 8.  Sums in fp32; the hidden values are rounded to the 16-bit type between the two kernels (they are the second
     product's operand), so fp16 hidden values beyond 65504 become infinite.  Differentiable once in every argument; each gradient
-    that is not needed is not computed (at most 2^26 tokens then)."""
+    that is not needed is not computed (at most 2^26 tokens then).  Forward-mode derivatives are refused."""
     _check_input(x)
     dt, index = x.dtype, x.get_device()
     hidden = x.shape[-1]
@@ -295,6 +301,8 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
         raise ValueError(f"hidden and intermediate sizes must be multiples of 8 below 2^30, got {hidden} and {inter}")
     if w_gate.get_device() != index or w_up.get_device() != index or w_down.get_device() != index:
         raise ValueError(f"all weights must be on cuda:{index}")
+    if _has_tangent(x, w_gate, w_up, w_down):
+        raise NotImplementedError("gated_feed_forward has no forward-mode derivative")
     rows = x if x.dim() == 2 else x.reshape(-1, hidden)
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
         y = _GatedFeedForward.apply(rows, w_gate, w_up, w_down)

@@ -95,6 +95,18 @@ def test_inner_sizes_past_32_bits_are_refused(k):
         dense._check_k8(k)
 
 
+def test_tangents_are_seen():
+    import torch.autograd.forward_ad as fwad
+
+    x = torch.zeros(3)
+    assert not dense._has_tangent(x)
+    with fwad.dual_level():
+        dual = fwad.make_dual(x, torch.ones(3))
+        assert not dense._has_tangent(x) and dense._has_tangent(x, dual)
+        with torch.no_grad():
+            assert dense._has_tangent(dual)
+
+
 def test_w8a8_linear_plumbing():
     lin = D.W8A8Linear.from_metadata({"out_features": 33, "in_features": 64, "bias_shape": [33], "orig_dtype": "torch.float16"})
     assert set(lin.state_dict()) == {"weight", "weight_scale", "bias"}

@@ -428,6 +428,28 @@ def test_ffn_second_derivatives_raise_whatever_the_loss_is():
         g.float().sum().backward()
 
 
+@pytest.mark.parametrize("which", range(4))
+def test_ffn_forward_mode_is_refused(which):
+    """A tangent must not be dropped in silence, whether or not a gradient is asked for as well."""
+    import torch.autograd.forward_ad as fwad
+
+    args = list(ffn_inputs(24, 264, 136, torch.bfloat16, seed=17)[:4])
+    with fwad.dual_level():
+        assert not dense.gated_feed_forward(*args).requires_grad     # no tangents: as ever
+        args[which] = fwad.make_dual(args[which], torch.ones_like(args[which]))
+        for grad in (False, True):
+            plain = [v if i == which else v.detach().requires_grad_(grad) for i, v in enumerate(args)]
+            with pytest.raises(NotImplementedError):
+                dense.gated_feed_forward(*plain)
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                dense.gated_feed_forward(*plain)
+    fn = lambda v: dense.gated_feed_forward(v, *args[1:])            # noqa: E731
+    if which == 0:
+        x = ffn_inputs(24, 264, 136, torch.bfloat16, seed=17)[0]
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            torch.func.jvp(fn, (x,), (torch.ones_like(x),))
+
+
 def test_ffn_with_saved_tensors_moved_and_from_other_threads():
     """What is saved may come back from a hook laid out anew; calls may come from several threads and streams at once."""
     import threading
