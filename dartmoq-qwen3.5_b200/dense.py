@@ -68,9 +68,15 @@ def _need(cond: bool, message: str) -> None:
         raise ValueError(message)
 
 
-def _check_input(x: torch.Tensor) -> None:
-    if not x.is_cuda:
+def _check_cuda(t: torch.Tensor) -> None:
+    if torch._C._get_tracing_state() is not None:      # a trace would hold the outputs' allocation and not the call that fills them
+        raise _lib.DmoqError("libdmoq operators cannot be traced")
+    if not t.is_cuda:
         raise _lib.DmoqError("libdmoq operators take CUDA tensors only (no CPU path)")
+
+
+def _check_input(x: torch.Tensor) -> None:
+    _check_cuda(x)
     if x.dtype is not _BF16 and x.dtype is not _FP16:
         raise TypeError(f"x must be fp16 or bf16, got {x.dtype}")
     if x.dim() < 1:
@@ -133,8 +139,7 @@ def int8_matmul(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, 
     """out[t, n] = scale[t] * weight_scale[n] * sum_k codes[t, k] * weight[n, k] (+ bias[n]); exact int32 sums, scales and bias
     in fp32, one rounding to ``out_dtype``.  ``codes`` int8 (..., K), ``weight`` int8 (N, K); K a multiple of 16, at most
     131056; any N."""
-    if not codes.is_cuda:
-        raise _lib.DmoqError("libdmoq operators take CUDA tensors only (no CPU path)")
+    _check_cuda(codes)
     if codes.dtype is not torch.int8 or scale.dtype is not torch.float32:
         raise TypeError(f"codes must be int8 with an fp32 scale, got {codes.dtype} and {scale.dtype}")
     if out_dtype is not _BF16 and out_dtype is not _FP16:

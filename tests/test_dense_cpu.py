@@ -95,6 +95,17 @@ def test_inner_sizes_past_32_bits_are_refused(k):
         dense._check_k8(k)
 
 
+def test_functions_refuse_to_be_traced():
+    """A recorded call would return memory that nothing fills."""
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    w8, s8 = torch.zeros(32, 64, dtype=torch.int8), torch.zeros(32)
+    w = torch.zeros(32, 64, dtype=torch.bfloat16)
+    for call in (dense.quantize_int8_tokens, lambda v: dense.int8_linear(v, w8, s8), lambda v: dense.int8_gated_linear(v, w8, s8, w8, s8),
+                 lambda v: dense.gated_feed_forward(v, w, w, w.t()), lambda v: dense.int8_matmul(v.to(torch.int8), s8[:4], w8, s8)):
+        with pytest.raises(_lib.DmoqError, match="traced"):
+            torch.jit.trace(call, (x,))
+
+
 def test_tangents_are_seen():
     import torch.autograd.forward_ad as fwad
 

@@ -687,6 +687,16 @@ def test_int8_results_do_not_depend_on_the_batch():
         assert torch.equal(dense.int8_linear(x[:t], w[:500], ws[:500]), dense.int8_linear(x, w[:500], ws[:500])[:t]), t
 
 
+@pytest.mark.filterwarnings("ignore")
+def test_modules_refuse_to_be_traced():
+    block = D.GatedFeedForward(144, 80, device=DEV)
+    x = randn(rng(60), 5, 144, dtype=torch.bfloat16)
+    for module in (block, D.W8A8GatedFeedForward.from_mlp(block), D.W8A8Linear.from_linear(block.gate_proj)):
+        with pytest.raises(_lib.DmoqError, match="traced"):
+            torch.jit.trace(module, (x,))
+        assert torch.isfinite(module(x)).all()                       # and run as ever afterwards
+
+
 FIRST_USE = """
 import sys
 sys.path.insert(0, %r)
