@@ -16,12 +16,36 @@ from . import dense
 from .linear import W8A8Linear
 
 
+def _is_silu(act) -> bool:
+    """Whether an activation (a name, a function or a module) is SiLU: by what it computes."""
+    if isinstance(act, str):
+        return act.lower() in ("silu", "swish")
+    z = torch.linspace(-8.0, 8.0, 65, device="cpu")
+    try:
+        with torch.no_grad():
+            out = act(z.clone())
+    except Exception:
+        return False
+    return torch.is_tensor(out) and out.shape == z.shape and torch.allclose(out.float().cpu(), nn.functional.silu(z), rtol=1e-4, atol=1e-6)
+
+
 def _projections(mlp):
+    """The three projections of a block that computes down(silu(gate(x)) * up(x)) with plain linears.  What can be told from the
+    block is checked (its activation, hooks and forward methods of the linears); its own ``forward`` is taken to be that."""
     parts = [getattr(mlp, name, None) for name in ("gate_proj", "up_proj", "down_proj")]
     if any(not isinstance(p, nn.Linear) for p in parts):
         raise TypeError("expected a block with gate_proj, up_proj and down_proj of type nn.Linear")
     if any(p.bias is not None for p in parts):
         raise ValueError("the gated feed-forward block has no biases")
+    for p in parts:
+        if type(p).forward is not nn.Linear.forward or "forward" in vars(p):
+            raise ValueError(f"{type(p).__name__} computes more than nn.Linear: only its weight would be taken over")
+        if p._forward_hooks or p._forward_pre_hooks or p._backward_hooks or p._backward_pre_hooks:
+            raise ValueError("hooks of the projections would no longer run: remove them first")
+    for name in ("act_fn", "activation_fn", "act", "activation", "hidden_act"):
+        act = getattr(mlp, name, None)
+        if (isinstance(act, str) or callable(act)) and not _is_silu(act):
+            raise ValueError(f"the gated feed-forward block computes SiLU, the block's {name} is {act!r}")
     return parts
 
 

@@ -160,3 +160,55 @@ def test_feed_forward_plumbing():
         D.W8A8GatedFeedForward(lin(32, 64), lin(48, 64), lin(64, 32))
     with pytest.raises(ValueError):
         D.W8A8GatedFeedForward(lin(32, 64), lin(32, 64), lin(64, 48))
+
+
+class Mlp(torch.nn.Module):
+    def __init__(self, **attributes):
+        super().__init__()
+        self.gate_proj, self.up_proj = torch.nn.Linear(64, 32, bias=False), torch.nn.Linear(64, 32, bias=False)
+        self.down_proj = torch.nn.Linear(32, 64, bias=False)
+        for name, value in attributes.items():
+            setattr(self, name, value)
+
+
+class Doubled(torch.nn.Linear):
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+def test_from_mlp_takes_silu_blocks():
+    F = torch.nn.functional
+    for act in (torch.nn.SiLU(), F.silu, lambda z: z * torch.sigmoid(z), "silu", "Swish"):
+        for name in ("act_fn", "hidden_act"):
+            assert D.GatedFeedForward.from_mlp(Mlp(**{name: act})).hidden_size == 64
+    assert D.GatedFeedForward.from_mlp(Mlp(act=None, activation=0.5)).intermediate_size == 32     # not an activation
+
+
+def test_from_mlp_refuses_what_it_would_compute_otherwise():
+    F = torch.nn.functional
+    for act in (torch.nn.GELU(), F.relu, "gelu", "gelu_pytorch_tanh", torch.nn.PReLU(), torch.nn.GLU(), lambda z: z, lambda a, b: a):
+        for name in ("act_fn", "activation_fn", "act", "activation", "hidden_act"):
+            for cls in (D.GatedFeedForward, D.W8A8GatedFeedForward):
+                with pytest.raises(ValueError, match=name):
+                    cls.from_mlp(Mlp(**{name: act}))
+    for part in ("gate_proj", "up_proj", "down_proj"):
+        mlp = Mlp(act_fn=torch.nn.SiLU())
+        n, k = getattr(mlp, part).weight.shape
+        setattr(mlp, part, Doubled(k, n, bias=False))
+        with pytest.raises(ValueError, match="Doubled"):
+            D.GatedFeedForward.from_mlp(mlp)
+        for register in ("register_forward_hook", "register_forward_pre_hook", "register_full_backward_hook", "register_full_backward_pre_hook"):
+            mlp = Mlp()
+            handle = getattr(getattr(mlp, part), register)(lambda *a: None)
+            with pytest.raises(ValueError, match="hooks"):
+                D.GatedFeedForward.from_mlp(mlp)
+            handle.remove()
+            D.GatedFeedForward.from_mlp(mlp)
+        mlp = Mlp()
+        getattr(mlp, part).forward = lambda x: x                     # as wrappers of a module's forward do
+        with pytest.raises(ValueError):
+            D.GatedFeedForward.from_mlp(mlp)
+    mlp = Mlp()
+    torch.nn.utils.parametrizations.weight_norm(mlp.up_proj)         # a computed weight is read as it is computed
+    block = D.GatedFeedForward.from_mlp(mlp)
+    assert block.up_proj.weight.grad_fn is not None
