@@ -24,6 +24,8 @@ from . import _lib
 
 _BF16, _FP16, _FP32, _INT8 = torch.bfloat16, torch.float16, torch.float32, torch.int8
 _MAX_ROWS = 1 << 30
+_MAX_SIDE = 1 << 29          # of a feed-forward block
+_MAX_GRAD_TOKENS = 1 << 26
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
@@ -302,14 +304,16 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     if w_gate.shape != (inter, hidden) or w_up.shape != (inter, hidden) or w_down.shape != (hidden, inter):
         raise ValueError(f"for x of {hidden} columns the weights must be (I, {hidden}) twice and ({hidden}, I), got {tuple(w_gate.shape)}, "
                          f"{tuple(w_up.shape)}, {tuple(w_down.shape)}")
-    if hidden < 8 or inter < 8 or (hidden | inter) & 7 or hidden | inter >= 1 << 30:
-        raise ValueError(f"hidden and intermediate sizes must be multiples of 8 below 2^30, got {hidden} and {inter}")
+    if hidden < 8 or inter < 8 or (hidden | inter) & 7 or hidden > _MAX_SIDE or inter > _MAX_SIDE:
+        raise ValueError(f"hidden and intermediate sizes must be multiples of 8 up to 2^29, got {hidden} and {inter}")
     if w_gate.get_device() != index or w_up.get_device() != index or w_down.get_device() != index:
         raise ValueError(f"all weights must be on cuda:{index}")
     if _has_tangent(x, w_gate, w_up, w_down):
         raise NotImplementedError("gated_feed_forward has no forward-mode derivative")
     rows = x if x.dim() == 2 else x.reshape(-1, hidden)
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad):
+        if rows.shape[0] > _MAX_GRAD_TOKENS:
+            raise ValueError(f"at most 2^26 tokens where gradients are needed, got {rows.shape[0]}")
         y = _GatedFeedForward.apply(rows, w_gate, w_up, w_down)
     else:
         rows, t, pitch = _rows(rows, hidden)

@@ -404,6 +404,21 @@ def test_ffn_empty_shapes_strides_and_refusals():
         double.sum().backward()                                      # once differentiable
 
 
+def test_ffn_sizes_beyond_the_limits_are_refused_before_any_work():
+    """One token or one element each in memory: the sizes are those of views."""
+    w = torch.zeros(8, 8, dtype=torch.bfloat16, device=DEV)
+    x = torch.zeros(1, 8, dtype=torch.bfloat16, device=DEV)
+    for leaf in (x, w):
+        leaf.requires_grad_(True)
+        with pytest.raises(ValueError, match="2\\^26"):
+            dense.gated_feed_forward(x.expand((1 << 26) + 1, 8), w, w, w)
+        leaf.requires_grad_(False)
+    one = torch.zeros(1, dtype=torch.bfloat16, device=DEV)
+    for h, i in (((1 << 29) + 8, 8), (8, (1 << 29) + 8)):
+        with pytest.raises(ValueError, match="2\\^29"):
+            dense.gated_feed_forward(one.expand(1, h), one.expand(i, h), one.expand(i, h), one.expand(h, i))
+
+
 def test_ffn_second_derivatives_raise_whatever_the_loss_is():
     """A gradient of a gradient must never be left out in silence, also where the upstream gradient is a constant."""
     x, wg, wu, wd, dy = ffn_inputs(24, 264, 136, torch.bfloat16, seed=16)
