@@ -11,6 +11,9 @@ loads here unchanged and the other way round.
     restore_quant_metadata   :348                        load_quantized_state_dict :612
     convert_model_to_wxa8 / wxfp8 / wxfp4   :416 / :452 / :503
 
+The dense modules beside the packed ones (``W8A8Linear`` and the gated feed-forward blocks) travel the same way, under types of
+their own in ``meta.json``; a checkpoint without them has the reference's files.
+
 Only the parts that touch the quantized modules are here; building the skeleton model (a transformers
 class on the meta device) stays with the caller.
 """
@@ -24,7 +27,8 @@ from typing import Callable, Dict, Optional, Tuple, Union
 import torch
 
 from . import format as fmt
-from .linear import WxA16Linear, WxA8Linear, WxFP8Linear
+from .ffn import GatedFeedForward, W8A8GatedFeedForward, require_silu
+from .linear import W8A8Linear, WxA16Linear, WxA8Linear, WxFP8Linear
 from .moe import (WxA16BitPartitionedGroupMoE, WxA8BitPartitionedGroupMoE, WxFP4BitPartitionedGroupMoE,
                   WxFP8BitPartitionedGroupMoE)
 
@@ -44,6 +48,14 @@ def _linear_entry(lin: WxA16Linear) -> dict:
         "bias_shape": None if lin.bias is None else list(lin.bias.shape),
         "codebook_type": getattr(lin, "codebook_type", "lloydmax"),
     }
+
+
+def _w8a8_entry(lin: W8A8Linear) -> dict:
+    out = {"type": "w8a8_linear", "in_features": lin.in_features, "out_features": lin.out_features,
+           "bias_shape": None if lin.bias is None else list(lin.bias.shape)}
+    if lin.bias is not None:
+        out["orig_dtype"] = str(lin.bias.dtype)
+    return out
 
 
 def _side_entry(packed: dict) -> dict:
@@ -79,6 +91,12 @@ def collect_quant_metadata(model, quant_args: Optional[dict] = None, model_id: O
             continue
         if isinstance(mod, WxA16Linear):
             meta["modules"][path] = _linear_entry(mod)
+        elif isinstance(mod, W8A8Linear):
+            meta["modules"][path] = _w8a8_entry(mod)
+        elif isinstance(mod, W8A8GatedFeedForward):
+            meta["modules"][path] = {"type": "w8a8_gated_ffn"}
+        elif isinstance(mod, GatedFeedForward):
+            meta["modules"][path] = {"type": "gated_ffn"}
         elif isinstance(mod, WxA16BitPartitionedGroupMoE):
             meta["layers"][path] = _moe_entry(mod)
     return meta
@@ -179,18 +197,30 @@ def _parent_of(root, path: str):
 def restore_quant_metadata(model, meta: dict, state_dict: Optional[dict] = None, key_prefix_map: PrefixMap = None):
     """Swap the skeleton model's dense modules for packed ones described by ``meta`` and fill them.
 
-    Order matters: packed Linears first (the shared expert's projections still sit in the original mlp), then each
-    mlp is replaced by a ``WxA16BitPartitionedGroupMoE`` that takes over the old mlp's ``gate``, ``shared_expert``
-    and ``shared_expert_gate``, then ``load_state_dict(strict=True, assign=True)``: every key must match.
+    Order matters: Linears first (the shared expert's projections still sit in the original mlp), then the gated feed-forward
+    blocks around such projections, then each mlp is replaced by a ``WxA16BitPartitionedGroupMoE`` that takes over the old mlp's
+    ``gate``, ``shared_expert`` and ``shared_expert_gate``, then ``load_state_dict(strict=True, assign=True)``: every key must
+    match.
     ``key_prefix_map`` renames paths and keys (a ``(old, new)`` prefix pair or a callable), for skeletons whose
     module tree is rooted differently from the checkpoint's.
     """
     rename = _mapper(key_prefix_map)
     for path, m in meta.get("modules", {}).items():
-        if m.get("type") != "wxa16_linear":
+        cls = {"wxa16_linear": WxA16Linear, "w8a8_linear": W8A8Linear}.get(m.get("type"))
+        if cls is not None:
+            parent, attr = _parent_of(model, rename(path))
+            setattr(parent, attr, cls.from_metadata(m))
+    for path, m in meta.get("modules", {}).items():
+        if m.get("type") not in ("w8a8_gated_ffn", "gated_ffn"):
             continue
         parent, attr = _parent_of(model, rename(path))
-        setattr(parent, attr, WxA16Linear.from_metadata(m))
+        old = getattr(parent, attr)
+        if m["type"] == "gated_ffn":
+            block = GatedFeedForward.from_mlp(old)
+        else:
+            require_silu(old)
+            block = W8A8GatedFeedForward(old.gate_proj, old.up_proj, old.down_proj)
+        setattr(parent, attr, block)
     for path, m in meta.get("layers", {}).items():
         parent, attr = _parent_of(model, rename(path))
         old = getattr(parent, attr)

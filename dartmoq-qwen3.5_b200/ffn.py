@@ -29,6 +29,14 @@ def _is_silu(act) -> bool:
     return torch.is_tensor(out) and out.shape == z.shape and torch.allclose(out.float().cpu(), nn.functional.silu(z), rtol=1e-4, atol=1e-6)
 
 
+def require_silu(mlp) -> None:
+    """ValueError where a block names another activation."""
+    for name in ("act_fn", "activation_fn", "act", "activation", "hidden_act"):
+        act = getattr(mlp, name, None)
+        if (isinstance(act, str) or callable(act)) and not _is_silu(act):
+            raise ValueError(f"the gated feed-forward block computes SiLU, the block's {name} is {act!r}")
+
+
 def _projections(mlp):
     """The three projections of a block that computes down(silu(gate(x)) * up(x)) with plain linears.  What can be told from the
     block is checked (its activation, hooks and forward methods of the linears); its own ``forward`` is taken to be that."""
@@ -42,10 +50,7 @@ def _projections(mlp):
             raise ValueError(f"{type(p).__name__} computes more than nn.Linear: only its weight would be taken over")
         if p._forward_hooks or p._forward_pre_hooks or p._backward_hooks or p._backward_pre_hooks:
             raise ValueError("hooks of the projections would no longer run: remove them first")
-    for name in ("act_fn", "activation_fn", "act", "activation", "hidden_act"):
-        act = getattr(mlp, name, None)
-        if (isinstance(act, str) or callable(act)) and not _is_silu(act):
-            raise ValueError(f"the gated feed-forward block computes SiLU, the block's {name} is {act!r}")
+    require_silu(mlp)
     return parts
 
 
