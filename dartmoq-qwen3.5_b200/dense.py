@@ -4,6 +4,7 @@
   int8_matmul            codes x 8-bit weight, one scale a token and one a weight row (+ bias)
   int8_linear            both of the above in one call
   int8_gated_linear      silu(x Wg^T) * (x Wu^T) with 8-bit operands: the first half of a feed-forward block
+  int8_gated_matmul      the same of codes that are there already
   gated_feed_forward     (silu(x Wg^T) * (x Wu^T)) Wd^T in 16 bits, with its gradients
 
 The modules over them are ``linear.W8A8Linear`` and ``ffn.GatedFeedForward`` / ``ffn.W8A8GatedFeedForward``; the latter two
@@ -141,8 +142,31 @@ def int8_matmul(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, 
     """out[t, n] = scale[t] * weight_scale[n] * sum_k codes[t, k] * weight[n, k] (+ bias[n]); exact int32 sums, scales and bias
     in fp32, one rounding to ``out_dtype``.  ``codes`` int8 (..., K), ``weight`` int8 (N, K); K a multiple of 16, at most
     131056; any N."""
+    codes, t, k, scale, index = _token_codes(codes, scale, out_dtype)
+    w, n, w_pitch, ws = _weight8(weight, weight_scale, k, index, "weight")
+    bias, bias_ptr = _bias_ptr(bias, n, out_dtype, index)
+    out = torch.empty(scale.shape + (n,), dtype=out_dtype, device=codes.device)
+    _call("dmoq_int8_gemm", index, codes.data_ptr(), scale.data_ptr(), w.data_ptr(), w_pitch, ws.data_ptr(), bias_ptr, out_dtype is _BF16,
+          t, n, k, out.data_ptr())
+    return out
+
+
+def int8_gated_matmul(codes: torch.Tensor, scale: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.Tensor, w_up: torch.Tensor,
+                      up_scale: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """silu(g) * u of given codes, g and u as ``int8_matmul`` has them (see ``int8_gated_linear``): for tokens whose codes are
+    there already, because another product of theirs needed them."""
+    codes, t, k, scale, index = _token_codes(codes, scale, out_dtype)
+    wg, n, gate_pitch, sg, wu, up_pitch, su = _gated_weights(w_gate, gate_scale, w_up, up_scale, k, index)
+    out = torch.empty(scale.shape + (n,), dtype=out_dtype, device=codes.device)
+    _call("dmoq_int8_gated_gemm", index, codes.data_ptr(), scale.data_ptr(), wg.data_ptr(), gate_pitch, sg.data_ptr(), wu.data_ptr(), up_pitch,
+          su.data_ptr(), out_dtype is _BF16, t, n, k, out.data_ptr())
+    return out
+
+
+def _token_codes(codes: torch.Tensor, scale: torch.Tensor, out_dtype: torch.dtype):
+    """Codes (without a pitch: the entry points take none) and scales as the kernels take them, their sizes and device."""
     _check_cuda(codes)
-    if codes.dtype is not torch.int8 or scale.dtype is not torch.float32:
+    if codes.dtype is not _INT8 or scale.dtype is not _FP32:
         raise TypeError(f"codes must be int8 with an fp32 scale, got {codes.dtype} and {scale.dtype}")
     if out_dtype is not _BF16 and out_dtype is not _FP16:
         raise TypeError(f"out_dtype must be fp16 or bf16, got {out_dtype}")
@@ -151,16 +175,16 @@ def int8_matmul(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, 
     _check_k8(k)
     _need(scale.shape == codes.shape[:-1] and scale.is_cuda and scale.get_device() == index,
           f"one scale a token on cuda:{index}: got {tuple(scale.shape)}")
-    w, n, w_pitch, ws = _weight8(weight, weight_scale, k, index, "weight")
-    bias, bias_ptr = _bias_ptr(bias, n, out_dtype, index)
-    a, t, pitch = _rows(codes, k)
-    if pitch != k:
-        a = a.contiguous()
-    scale = scale.contiguous()
-    out = torch.empty(codes.shape[:-1] + (n,), dtype=out_dtype, device=codes.device)
-    _call("dmoq_int8_gemm", index, a.data_ptr(), scale.data_ptr(), w.data_ptr(), w_pitch, ws.data_ptr(), bias_ptr, out_dtype is _BF16, t, n, k,
-          out.data_ptr())
-    return out
+    rows, t, pitch = _rows(codes, k)
+    return rows if pitch == k else rows.contiguous(), t, k, scale.contiguous(), index
+
+
+def _gated_weights(w_gate, gate_scale, w_up, up_scale, k: int, index: int):
+    wg, n, gate_pitch, sg = _weight8(w_gate, gate_scale, k, index, "w_gate")
+    wu, n_up, up_pitch, su = _weight8(w_up, up_scale, k, index, "w_up")
+    if n_up != n:
+        raise ValueError(f"w_gate and w_up must have one shape, got {tuple(w_gate.shape)} and {tuple(w_up.shape)}")
+    return wg, n, gate_pitch, sg, wu, up_pitch, su
 
 
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
@@ -193,10 +217,7 @@ def int8_gated_linear(x: torch.Tensor, w_gate: torch.Tensor, gate_scale: torch.T
     shape, index = x.shape, x.get_device()
     k = shape[-1]
     _check_k8(k)
-    wg, n, gate_pitch, sg = _weight8(w_gate, gate_scale, k, index, "w_gate")
-    wu, n_up, up_pitch, su = _weight8(w_up, up_scale, k, index, "w_up")
-    if n_up != n:
-        raise ValueError(f"w_gate and w_up must have one shape, got {tuple(w_gate.shape)} and {tuple(w_up.shape)}")
+    wg, n, gate_pitch, sg, wu, up_pitch, su = _gated_weights(w_gate, gate_scale, w_up, up_scale, k, index)
     rows, t, pitch = _rows(x, k)
     scratch = _int8_scratch(x, t, n, k, True)
     out = x.new_empty((t, n) if len(shape) == 2 else shape[:-1] + (n,))

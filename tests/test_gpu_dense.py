@@ -198,6 +198,43 @@ def test_int8_gated_linear(t, n, k, dtype):
     healthy()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,n,k", SIZES8)
+def test_int8_gated_matmul(t, n, k, dtype):
+    """Of the tokens' own codes: bit for bit what the quantiser in front of the same products gives."""
+    g = rng(t * n + k + 1)
+    x, (wg, sg), (wu, su) = acts(g, t, k, dtype), weight8(g, n, k), weight8(g, n, k)
+    codes, scale = dense.quantize_int8_tokens(x)
+    h = dense.int8_gated_matmul(codes, scale, wg, sg, wu, su, out_dtype=dtype)
+    assert h.shape == (t, n) and h.dtype == dtype
+    assert torch.equal(h, dense.int8_gated_linear(x, wg, sg, wu, su))
+    healthy()
+
+
+def test_int8_gated_matmul_shapes_strides_and_refusals():
+    g = rng(63)
+    codes = torch.randint(-128, 128, (4, 6, 512), generator=g).to(torch.int8).to(DEV)
+    scale = (torch.rand(4, 6, generator=g) * 1e-3).to(DEV)
+    (wg, sg), (wu, su) = weight8(g, 57, 512), weight8(g, 57, 512)
+    want = dense.int8_gated_matmul(codes[:, ::2, 16:272].contiguous(), scale[:, ::2].contiguous(), wg[:, :256].contiguous(), sg,
+                                   wu[:, 64:320].contiguous(), su)
+    assert want.shape == (4, 3, 57) and want.dtype == torch.bfloat16
+    assert torch.equal(dense.int8_gated_matmul(codes[:, ::2, 16:272], scale[:, ::2], wg[:, :256], sg, wu[:, 64:320], su), want)
+    one = dense.int8_gated_matmul(codes[0, 0], scale[0, 0], wg, sg, wu, su, out_dtype=torch.float16)
+    assert one.shape == (57,) and torch.equal(one, dense.int8_gated_matmul(codes[0], scale[0], wg, sg, wu, su, torch.float16)[0])
+    assert dense.int8_gated_matmul(codes[:0], scale[:0], wg, sg, wu, su).shape == (0, 6, 57)
+    for bad in ((codes.float(), scale, wg, sg, wu, su), (codes, scale.half(), wg, sg, wu, su), (codes, scale, wg.float(), sg, wu, su),
+                (codes, scale, wg, sg, wu, su, torch.float32)):
+        with pytest.raises(TypeError):
+            dense.int8_gated_matmul(*bad)
+    for bad in ((codes, scale[:1], wg, sg, wu, su), (codes, scale.cpu(), wg, sg, wu, su), (codes, scale, wg[:-1], sg[:-1], wu, su),
+                (codes, scale, wg, sg[:-1], wu, su), (codes[..., :256], scale, wg, sg, wu, su), (codes[..., :100], scale, wg, sg, wu, su)):
+        with pytest.raises(ValueError):
+            dense.int8_gated_matmul(*bad)
+    with pytest.raises(_lib.DmoqError):
+        dense.int8_gated_matmul(codes.cpu(), scale.cpu(), wg, sg, wu, su)
+
+
 @pytest.mark.parametrize("t", (1, 12, 40, 200, 2500))
 def test_gates_far_below_zero(t):
     """silu(g) down to g = -95, where the sigmoid is a subnormal 32-bit number; an up value of 1e6 brings it back."""
