@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/dmoq.h"
 
 #define DMOQ_CHECK_ARG(cond) \
@@ -22,10 +24,11 @@ static inline int dmoq_ceil_div(int a, int b) { return (a + b - 1) / b; }
 // Number of SMs of the current device, cached per process (read-only query).
 int dmoq_sm_count();
 
-// One-time kernel set-up (cudaFuncSetAttribute) is per DEVICE: a launcher keeps one flag per device ordinal.
+// One-time kernel set-up (cudaFuncSetAttribute) is per DEVICE: a launcher keeps one flag per device ordinal.  Several host
+// threads may do it at once, to the same effect.
 struct DmoqOncePerDevice {
-  bool done[64] = {};
-  bool* slot() {
+  std::atomic<bool> done[64] = {};
+  std::atomic<bool>* slot() {
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
     return &done[dev];

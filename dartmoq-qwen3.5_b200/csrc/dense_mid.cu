@@ -147,7 +147,7 @@ template <int KIND, int EPI, int BN>
 int launch(const Maps& maps, const Args& a, int splits, cudaStream_t s) {
   using C = MidCfg<BN>;
   static DmoqOncePerDevice once;
-  bool* configured = once.slot();
+  std::atomic<bool>* configured = once.slot();
   if (configured == nullptr) return DMOQ_EDEVICE;
   auto* kernel = dense_mid_kernel<KIND, EPI, BN>;
   if (!*configured) {

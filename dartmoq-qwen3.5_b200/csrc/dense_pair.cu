@@ -389,7 +389,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) dense_p
 template <int KIND, bool AMN, bool BMN, int EPI, int NP>
 int launch(Work<NP>& work, cudaStream_t s) {
   static DmoqOncePerDevice once;
-  bool* configured = once.slot();
+  std::atomic<bool>* configured = once.slot();
   if (configured == nullptr) return DMOQ_EDEVICE;
   auto* kernel = dense_pair_kernel<KIND, AMN, BMN, EPI, NP>;
   if (!*configured) {

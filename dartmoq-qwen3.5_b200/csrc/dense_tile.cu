@@ -169,12 +169,12 @@ __global__ void __launch_bounds__(256, 2) dense_tile_kernel(const __grid_constan
 // Blocks of this kernel that run at once in clusters of `splits` (a power of two up to 8), an SM each: clusters do not fill
 // every processing cluster of the device, so this is less than there are SMs.  With three stages twice as many fit.
 int tile_blocks_at_once(int splits) {
-  static int known[64][4] = {};
+  static std::atomic<int> known[64][4] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return dmoq_sm_count();
   int log = 0;
   while ((1 << log) < splits) ++log;
-  int& n = known[dev][log];
+  int n = known[dev][log];
   if (n == 0) {
     auto* kernel = dense_tile_kernel<KIND_16, false, false, EPI_OUT>;
     cudaLaunchConfig_t cfg = {};
@@ -194,7 +194,7 @@ int tile_blocks_at_once(int splits) {
       (void)cudaGetLastError();
       clusters = dmoq_sm_count() / splits;
     }
-    n = clusters * splits;
+    known[dev][log] = n = clusters * splits;
   }
   return n;
 }
@@ -204,7 +204,7 @@ namespace {
 template <int KIND, bool AMN, bool BMN, int EPI>
 int launch(const Maps& maps, const Args& a, int splits, cudaStream_t s) {
   static DmoqOncePerDevice once;
-  bool* configured = once.slot();
+  std::atomic<bool>* configured = once.slot();
   if (configured == nullptr) return DMOQ_EDEVICE;
   auto* kernel = dense_tile_kernel<KIND, AMN, BMN, EPI>;
   if (!*configured) {

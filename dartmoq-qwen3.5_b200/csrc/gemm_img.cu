@@ -911,13 +911,14 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 EncodeTiledFn encode_tiled_fn() {
-  static EncodeTiledFn fn = nullptr;
+  static std::atomic<EncodeTiledFn> known{nullptr};
+  EncodeTiledFn fn = known;
   if (fn == nullptr) {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
       return nullptr;
-    fn = reinterpret_cast<EncodeTiledFn>(p);
+    known = fn = reinterpret_cast<EncodeTiledFn>(p);
   }
   return fn;
 }
@@ -940,7 +941,7 @@ int make_image_map(CUtensorMap* map, const void* image, size_t rows, size_t row_
 template <int MODE, int EPI, int BN>
 int launch(const ImgMaps& maps, const ImgArgs& a, int work_cap, cudaStream_t s) {
   static DmoqOncePerDevice once;
-  bool* configured = once.slot();
+  std::atomic<bool>* configured = once.slot();
   if (configured == nullptr) return DMOQ_EDEVICE;
   const int bytes = (int)sizeof(Smem<BN>) + 1024;
   if (!*configured) {

@@ -821,7 +821,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(TcArgs a) {
 template <int MODE, int BIT, int EPI>
 int launch(const TcArgs& a, int work_cap, cudaStream_t s) {
   static DmoqOncePerDevice once;
-  bool* configured = once.slot();
+  std::atomic<bool>* configured = once.slot();
   if (configured == nullptr) return DMOQ_EDEVICE;
   const int bytes = (int)sizeof(Smem) + 1024;
   if (!*configured) {

@@ -489,7 +489,7 @@ constexpr size_t smem_bytes(int bit) {
 template <int MODE, int BIT, int EPI, int BM>
 int launch(const GemmArgs& a, int work_cap, cudaStream_t s) {
   static DmoqOncePerDevice once;
-  bool* configured = once.slot();
+  std::atomic<bool>* configured = once.slot();
   if (configured == nullptr) return DMOQ_EDEVICE;
   const size_t bytes = smem_bytes<MODE, BM>(BIT);
   if (!*configured) {
@@ -548,12 +548,11 @@ int dmoq_grouped_gemm_img_pools(const dmoq_route_t* route, const dmoq_pool_t* po
 // DMOQ_GEMM=mma forces the warp-level MMA kernel for every pool (A/B comparisons); default picks the
 // tcgen05 kernel wherever it applies.
 static bool use_tc_path() {
-  static int cached = -1;
-  if (cached < 0) {
+  static const bool use = [] {
     const char* v = getenv("DMOQ_GEMM");
-    cached = (v && v[0] == 'm') ? 0 : 1;
-  }
-  return cached == 1;
+    return !(v && v[0] == 'm');
+  }();
+  return use;
 }
 
 extern "C" int dmoq_grouped_gemm(const dmoq_route_t* route, const dmoq_pool_t* pools_host, int32_t pool_index,

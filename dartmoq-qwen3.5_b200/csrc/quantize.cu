@@ -84,7 +84,7 @@ extern "C" int dmoq_quantize_packed(const void* w, int32_t w_kind, int32_t N, in
   DMOQ_CHECK_ARG(w_kind >= 0 && w_kind <= 2 && N > 0 && K > 0 && K % kG == 0);
   DMOQ_CHECK_ARG(bit == 1 || bit == 2 || bit == 4 || bit == 8);
   static DmoqOncePerDevice once;
-  bool* configured = once.slot();
+  std::atomic<bool>* configured = once.slot();
   if (configured == nullptr) return DMOQ_EDEVICE;
   const size_t smem = (size_t)(kG * kG + kRows * kG + 256) * sizeof(float) + kRows * kG;
   if (!*configured) {

@@ -227,7 +227,7 @@ constexpr size_t kSmemBytes = (size_t)(kG * kPPitch + kG * kXPitch) * sizeof(flo
 template <int MODE>
 int launch_rows(const RotArgs& a, cudaStream_t s) {
   static DmoqOncePerDevice once;
-  bool* configured = once.slot();
+  std::atomic<bool>* configured = once.slot();
   if (configured == nullptr) return DMOQ_EDEVICE;
   if (!*configured) {
     if (cudaFuncSetAttribute(rotq_rows_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes) != cudaSuccess)
@@ -248,7 +248,7 @@ int launch_rows(const RotArgs& a, cudaStream_t s) {
 template <int MODE>
 int launch_tiles(const RotArgs& a, int tile_cap, cudaStream_t s) {
   static DmoqOncePerDevice once;
-  bool* configured = once.slot();
+  std::atomic<bool>* configured = once.slot();
   if (configured == nullptr) return DMOQ_EDEVICE;
   if (!*configured) {
     if (cudaFuncSetAttribute(rotq_tiles_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes) != cudaSuccess)
@@ -268,18 +268,17 @@ int launch_tiles(const RotArgs& a, int tile_cap, cudaStream_t s) {
 // The tensor-core kernel with exact fix-up is the default; DMOQ_ROTQ=chain computes every value on the CUDA-core
 // FMA chain instead (same codes, for A/B runs).  The unquantised fp16 rotation always uses the tensor cores.
 bool use_mma_rotation() {
-  static int cached = -1;
-  if (cached < 0) {
+  static const bool use = [] {
     const char* v = getenv("DMOQ_ROTQ");
-    cached = (v && v[0] == 'c') ? 0 : 1;
-  }
-  return cached == 1;
+    return !(v && v[0] == 'c');
+  }();
+  return use;
 }
 
 }  // namespace
 
 int dmoq_sm_count() {
-  static int cached[64] = {0};
+  static std::atomic<int> cached[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
   if (cached[dev] == 0) {

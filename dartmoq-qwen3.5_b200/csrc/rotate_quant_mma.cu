@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 2) rotq_mma_tiles_kernel(RotArgs a) 
 template <int MODE>
 int launch_rows(const RotArgs& a, cudaStream_t s) {
   static DmoqOncePerDevice once;
-  bool* configured = once.slot();
+  std::atomic<bool>* configured = once.slot();
   if (configured == nullptr) return DMOQ_EDEVICE;
   if (!*configured) {
     if (cudaFuncSetAttribute(rotq_mma_rows_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess)
@@ -522,7 +522,7 @@ int launch_rows(const RotArgs& a, cudaStream_t s) {
 template <int MODE>
 int launch_tiles(const RotArgs& a, int tile_cap, cudaStream_t s) {
   static DmoqOncePerDevice once;
-  bool* configured = once.slot();
+  std::atomic<bool>* configured = once.slot();
   if (configured == nullptr) return DMOQ_EDEVICE;
   if (!*configured) {
     if (cudaFuncSetAttribute(rotq_mma_tiles_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess)

@@ -316,7 +316,7 @@ int launch_route(const RouteArgs& a, bool fused, cudaStream_t s) {
   const size_t place_bytes = place_smem_bytes(r.E) + 16;
   const size_t fused_bytes = place_bytes + e_bytes + 16;
   static DmoqOncePerDevice once;
-  bool* configured = once.slot();
+  std::atomic<bool>* configured = once.slot();
   if (configured == nullptr) return DMOQ_EDEVICE;
   if (!*configured) {  // up to 4096 experts: the placement tables can exceed the default 48 KiB
     if (cudaFuncSetAttribute(route_fused_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024) != cudaSuccess ||

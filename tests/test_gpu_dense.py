@@ -780,3 +780,44 @@ def test_first_use_inside_a_capture():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", FIRST_USE % root], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.strip() == "same", r.stderr[-2000:]
+
+
+FIRST_USE_BY_THREADS = """
+import sys, threading
+sys.path.insert(0, %r)
+import torch
+from dartmoq_b200 import dense
+torch.manual_seed(0)
+w, s = torch.randint(-100, 100, (640, 512), device="cuda", dtype=torch.int8), torch.rand(640, device="cuda")
+f = [torch.randn(640, 512, device="cuda").bfloat16() * 0.05 for _ in range(2)] + [torch.randn(512, 640, device="cuda").bfloat16() * 0.05]
+xs = [torch.randn(t, 512, device="cuda").bfloat16() for t in (4, 40, 300, 3000)]
+work = lambda x: (dense.int8_linear(x, w, s), dense.int8_gated_linear(x, w, s, w, s), dense.gated_feed_forward(x, *f))
+torch.cuda.synchronize()
+start, got = threading.Barrier(8), [None] * 8
+
+def first(i):
+    with torch.cuda.stream(torch.cuda.Stream()):
+        start.wait()
+        got[i] = [work(x) for x in xs]
+        torch.cuda.current_stream().synchronize()
+
+threads = [threading.Thread(target=first, args=(i,)) for i in range(8)]
+for t in threads:
+    t.start()
+for t in threads:
+    t.join()
+for g in got:
+    assert all(torch.equal(a, b) for x, o in zip(xs, g) for a, b in zip(work(x), o))
+print("same")
+"""
+
+
+def test_first_use_by_several_threads_at_once():
+    """A fresh process in which eight threads make the first call of every kernel together."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_USE_BY_THREADS % root], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "same", r.stderr[-2000:]
