@@ -27,6 +27,7 @@ _BF16, _FP16, _FP32, _INT8 = torch.bfloat16, torch.float16, torch.float32, torch
 _MAX_ROWS = 1 << 30
 _MAX_SIDE = 1 << 29          # of a feed-forward block
 _MAX_GRAD_TOKENS = 1 << 26
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
@@ -72,7 +73,8 @@ def _need(cond: bool, message: str) -> None:
 
 
 def _check_cuda(t: torch.Tensor) -> None:
-    if torch._C._get_tracing_state() is not None:      # a trace would hold the outputs' allocation and not the call that fills them
+    # a trace (torch.jit or torch.fx) would hold the outputs' allocation and not the call that fills them
+    if torch._C._get_tracing_state() is not None or (torch._C._len_torch_dispatch_stack() and torch._C._get_dispatch_mode(_PROXY) is not None):
         raise _lib.DmoqError("libdmoq operators cannot be traced")
     if not t.is_cuda:
         raise _lib.DmoqError("libdmoq operators take CUDA tensors only (no CPU path)")

@@ -97,6 +97,8 @@ def test_inner_sizes_past_32_bits_are_refused(k):
 
 def test_functions_refuse_to_be_traced():
     """A recorded call would return memory that nothing fills."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
     x = torch.zeros(4, 64, dtype=torch.bfloat16)
     w8, s8 = torch.zeros(32, 64, dtype=torch.int8), torch.zeros(32)
     w = torch.zeros(32, 64, dtype=torch.bfloat16)
@@ -104,6 +106,8 @@ def test_functions_refuse_to_be_traced():
                  lambda v: dense.gated_feed_forward(v, w, w, w.t()), lambda v: dense.int8_matmul(v.to(torch.int8), s8[:4], w8, s8)):
         with pytest.raises(_lib.DmoqError, match="traced"):
             torch.jit.trace(call, (x,))
+        with pytest.raises(_lib.DmoqError, match="traced"):
+            make_fx(call)(x)
 
 
 def test_tangents_are_seen():
