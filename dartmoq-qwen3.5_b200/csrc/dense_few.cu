@@ -86,23 +86,31 @@ __global__ void __launch_bounds__(32 * kWarps) dense_few_kernel(const __grid_con
   }
   overlap_point();
   load_weights(warp * 128);
+  // the scales of this thread's output, long before they are needed
+  const int r = tid % kRows, token = tid / kRows, col = n0 + r;
+  float sa = 1.f, weight_scale[2] = {1.f, 1.f};
+  if (kKind == KIND_I8 && token < a.M && col < a.N) {
+    if (!FUSE) sa = a.a_scale[token];
+    weight_scale[0] = a.b_scale[0][col];
+    if (kDual) weight_scale[1] = a.b_scale[1][col];
+  }
 
   if (FUSE) {
     if (tid < 8) top[tid] = 0u;
     __syncthreads();
     const int per = 32 * kWarps / (a.M <= 1 ? 1 : a.M <= 2 ? 2 : a.M <= 4 ? 4 : 8);   // threads of a token
-    const int token = tid / per, j0 = tid % per, n8 = a.K / 8;
-    const uint4* src = reinterpret_cast<const uint4*>(f.x + token * f.x_pitch);
-    if (token < a.M) {
+    const int of = tid / per, j0 = tid % per, n8 = a.K / 8;
+    const uint4* src = reinterpret_cast<const uint4*>(f.x + of * f.x_pitch);
+    if (of < a.M) {
       uint32_t top2 = 0u;
       for (int i = j0; i < n8; i += per) top2 = magnitude_max(top2, src[i]);
-      atomicMax(&top[token], magnitude_join(top2));        // a maximum: the order does not matter
+      atomicMax(&top[of], magnitude_join(top2));           // a maximum: the order does not matter
     }
     __syncthreads();
-    if (token < a.M) {
-      const RowScale s = row_scale(top[token], a.bf16);
-      if (j0 == 0) token_scale[token] = s.scale;
-      for (int i = j0; i < n8; i += per) *reinterpret_cast<uint2*>(codes + token * code_pitch(a.K) + 8 * i) = codes8(src[i], s, a.bf16);
+    if (of < a.M) {
+      const RowScale s = row_scale(top[of], a.bf16);
+      if (j0 == 0) token_scale[of] = s.scale;
+      for (int i = j0; i < n8; i += per) *reinterpret_cast<uint2*>(codes + of * code_pitch(a.K) + 8 * i) = codes8(src[i], s, a.bf16);
     }
     __syncthreads();
   }
@@ -144,22 +152,23 @@ __global__ void __launch_bounds__(32 * kWarps) dense_few_kernel(const __grid_con
     for (int e = 0; e < 4; ++e) part[warp][g + 8 * (e >> 1)][8 * n + 2 * t + (e & 1)] = acc[n][e];
   __syncthreads();
 
-  for (int i = tid; i < kRows * a.M; i += 32 * kWarps) {
-    const int r = i % kRows, token = i / kRows, col = n0 + r;
-    if (col >= a.N) continue;
-    uint32_t v[2] = {0u, 0u};
+  if (tid >= kRows * a.M || col >= a.N) return;            // an output a thread: at most 16 rows by 16 tokens
+  uint32_t v[2] = {0u, 0u};
 #pragma unroll
-    for (int d = 0; d < (kDual ? 2 : 1); ++d)
+  for (int d = 0; d < (kDual ? 2 : 1); ++d)
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const uint32_t p = part[w][r + 8 * d][token];
-        v[d] = kKind == KIND_I8 ? v[d] + p : __float_as_uint(__uint_as_float(v[d]) + __uint_as_float(p));
-      }
-    const float sa = kKind == KIND_16 ? 1.f : FUSE ? token_scale[token] : a.a_scale[token];
-    float o[3];
-    finish<kKind, EPI>(a, token, col, v[0], v[1], sa, o);
-    a.out[0][token * a.ld_out + col] = (uint16_t)(pack16(o[0], 0.f, a.bf16) & 0xffffu);
+    for (int w = 0; w < kWarps; ++w) {
+      const uint32_t p = part[w][r + 8 * d][token];
+      v[d] = kKind == KIND_I8 ? v[d] + p : __float_as_uint(__uint_as_float(v[d]) + __uint_as_float(p));
+    }
+  if (kKind == KIND_I8) {
+    if (FUSE) sa = token_scale[token];
+#pragma unroll
+    for (int d = 0; d < (kDual ? 2 : 1); ++d) v[d] = __float_as_uint(scaled(v[d], sa, weight_scale[d]));
   }
+  float o[3];
+  finish<EPI>(a, col, __uint_as_float(v[0]), __uint_as_float(v[1]), o);
+  a.out[0][token * a.ld_out + col] = (uint16_t)(pack16(o[0], 0.f, a.bf16) & 0xffffu);
 }
 
 template <int TYPE, int EPI, bool FUSE>

@@ -69,6 +69,7 @@ __global__ void __launch_bounds__(256, MidCfg<BN>::kBlocks) dense_mid_kernel(con
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
   overlap_point();
 
+  bool mine_plain = true;
   if (warp == 0) {
     if (lane == 0) {
       int done = 0;
@@ -113,7 +114,9 @@ __global__ void __launch_bounds__(256, MidCfg<BN>::kBlocks) dense_mid_kernel(con
       }
       asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_acc) : "memory");
     }
-  } else if (warp >= 4) {
+  } else if (warp < 4) {
+    if (KIND == KIND_I8) mine_plain = plain_tile(a, 0, a.M, n0, kRows, kDual, tid - 64, 64);
+  } else {
     mbar_wait(bar_acc, 0, abort_flag, status);
     if (flag_get(abort_flag)) mbar_wait_quiet(bar_acc, 0);
     tc_fence_after();
@@ -130,7 +133,7 @@ __global__ void __launch_bounds__(256, MidCfg<BN>::kBlocks) dense_mid_kernel(con
     tc_fence_before();
   }
   __syncwarp();
-  __syncthreads();
+  const bool plain = __syncthreads_and(mine_plain);
   if (warp == 2) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(BN));
@@ -139,7 +142,7 @@ __global__ void __launch_bounds__(256, MidCfg<BN>::kBlocks) dense_mid_kernel(con
 
   // join and finish: this block's share of the tokens
   finish_rows<KIND, EPI, kRows>(a, sb, C::kPitch, (int)((long long)a.M * rank / splits), (int)((long long)a.M * (rank + 1) / splits), 0, n0,
-                                splits, tid);
+                                splits, tid, plain);
   if (splits > 1) cluster_sync();   // a block's shared memory lives until the others have read it
 }
 

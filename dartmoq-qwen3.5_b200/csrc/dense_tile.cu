@@ -73,6 +73,7 @@ __global__ void __launch_bounds__(256, 2) dense_tile_kernel(const __grid_constan
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
   overlap_point();
 
+  bool mine_plain = true;
   if (warp == 0) {
     if (lane == 0) {
       int done = 0;
@@ -135,7 +136,9 @@ __global__ void __launch_bounds__(256, 2) dense_tile_kernel(const __grid_constan
       }
       asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_acc) : "memory");
     }
-  } else if (warp >= 4) {
+  } else if (warp < 4) {
+    if (KIND == KIND_I8) mine_plain = plain_tile(a, m0, 128, n0, kCols, kDual, tid - 64, 64);
+  } else {
     mbar_wait(bar_acc, 0, abort_flag, &g_dmoq_dense_status);
     if (flag_get(abort_flag)) mbar_wait_quiet(bar_acc, 0);
     tc_fence_after();
@@ -152,7 +155,7 @@ __global__ void __launch_bounds__(256, 2) dense_tile_kernel(const __grid_constan
     tc_fence_before();
   }
   __syncwarp();
-  __syncthreads();
+  const bool plain = __syncthreads_and(mine_plain);
   if (warp == 2) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(BN));
@@ -160,7 +163,7 @@ __global__ void __launch_bounds__(256, 2) dense_tile_kernel(const __grid_constan
   if (splits > 1) cluster_sync();
 
   // join and finish: this block's rows of the tile
-  finish_rows<KIND, EPI, kCols>(a, sb, kPitch, 128 * rank / splits, 128 * (rank + 1) / splits, m0, n0, splits, tid);
+  finish_rows<KIND, EPI, kCols>(a, sb, kPitch, 128 * rank / splits, 128 * (rank + 1) / splits, m0, n0, splits, tid, plain);
   if (splits > 1) cluster_sync();   // a block's shared memory lives until the others have read it
 }
 
