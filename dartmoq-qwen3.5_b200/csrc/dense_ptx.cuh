@@ -210,13 +210,15 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16) {
 __device__ __forceinline__ float unpack16(uint32_t bits16, bool bf16) {
   return bf16 ? __uint_as_float(bits16 << 16) : __half2float(__ushort_as_half((unsigned short)bits16));
 }
-// sigmoid in fp32: 2 special-function instructions.  The exponential is off by at most 2 + 1.173 |x| units of 2^-23 (2^-19 of
-// the value at x = -12, 2^-16 at -90): below the 16-bit rounding of what is made of it.  Far below zero the quotient is the
-// exponential itself; there 1 + e^-x passes 2^126, where the fast division returns 0.
+// sigmoid in fp32, of the exponential of -|x|, which does not overflow: far below zero the result is that exponential (as
+// 1 / (1 + e^-x) the fast division returns 0 once 1 + e^-x passes 2^126, at -87).  The exponential is off by at most
+// 2 + 1.173 |x| units of 2^-23: for x < 0 so is the result (2^-19 of it at -12, 2^-16 at -90), below the 16-bit rounding of what
+// is made of it; for x > 0 that is divided by e^x.
 __device__ __forceinline__ float sigmoid(float x) {
-  const bool low = x < -64.f;                // e^-64 is below half a unit of 1 + e^64
-  const float e = __expf(low ? x : -x);
-  return low ? e : __fdividef(1.f, 1.f + e);
+  const float e = __expf(-fabsf(x));
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.f, e)));   // of 1 to 2: nothing to flush
+  return __fmul_rn(x < 0.f ? e : 1.f, r);
 }
 
 }  // namespace dense
