@@ -26,7 +26,8 @@ struct Maps {
 // silu(g) and u silu'(g) are kept to the upper 24 bits of their 32-bit floats, whatever the tensors' 16-bit type: planes 1 and 2
 // hold the upper 16 bits of either, plane 3 the next eight of both.  Rounded to 16 bits they would add a third rounding of the
 // type to dg and du, which are themselves rounded as operands of the next products; this costs half as much traffic
-// again and leaves 2^-16.  The lower bits are cut off, not rounded, so that a NaN stays one.
+// again and leaves less than 2^-15, always toward zero (2^-16 on average; a rounding of the types is up to 2^-9 or 2^-12).
+// The lower bits are cut off, not rounded, so that a NaN stays one.
 __device__ __forceinline__ uint32_t saved_low(float silu, float slope) {
   return ((__float_as_uint(silu) >> 8) & 0xffu) | (__float_as_uint(slope) & 0xff00u);
 }

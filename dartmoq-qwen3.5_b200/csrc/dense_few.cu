@@ -6,8 +6,8 @@
 // operands, which leaves the sums as they are.  The eight warps split K in steps of 128 bytes; their partial sums are joined
 // in a fixed order.  8-bit: with FUSE the block makes the codes of up to 8 tokens itself, in shared memory, while its first
 // weights are on their way (few_can_fuse), which saves a launch.
-// One token through 14336 x 4096 twice and back, 16 bits: 56 us for both launches = 6.3 TB/s (97 % of the measured bandwidth); 512 x
-// 2048 twice and back: 4.5 us, of which the weights account for 1.0.
+// One token through 14336 x 4096 twice and back, 16 bits: 68 us for both launches = 5.2 TB/s (80 % of the measured bandwidth: each
+// launch pays for its start and its join); 512 x 2048 twice and back: 5.0 us, of which the weights account for 1.0.
 #include "token_codes.cuh"
 
 namespace dense {

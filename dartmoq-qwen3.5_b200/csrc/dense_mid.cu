@@ -6,8 +6,8 @@
 // finishes.  Where
 // there are few tiles the K axis is split over a cluster's blocks, whose sums are joined through distributed shared memory
 // in rank order.  The accumulator (a lane an output, a column a token) passes through shared memory, a row a token.
-// 64 tokens: 13824 x 5120 twice 50 us = 5.7 TB/s of weights (88 % of the measured bandwidth), 5120 x 13824 in 4 parts 31 us = 4.6 TB/s
-// (40 tiles: their start, join and end show).
+// 64 tokens, 16 bits: 13824 x 5120 twice 51 us = 5.6 TB/s of weights (86 % of the measured bandwidth), and with 5120 x 13824 in 4
+// parts behind it 78 us (40 tiles of that: their start, join and end show).  8 bits: 13824 x 5120 13 us.
 #include "dense.cuh"
 
 __device__ int g_dmoq_dense_mid_status = 0;

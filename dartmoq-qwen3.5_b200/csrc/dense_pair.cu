@@ -11,9 +11,10 @@
 //   warps 4-11  take the sums out of TMEM, finish them, and write 32 x 32 blocks out through shared memory (plain
 //               stores of 64-byte rows: a TMA store costs each warp a proxy fence of about 500 cycles a block, which made the
 //               epilogue the longer half of tiles with a short K)
-// Bound by the tensor cores at the clock that the power limit leaves: 16384 x 4096 by K = 4096 in 8 bits 161 us = 3.4 Pop/s (tensor pipe
-// 89 % active at 1.58 GHz), 8192 x 14336 twice by K = 4096 in bf16 with the saved planes 1.29 ms = 1.49 PFLOP/s.  A product of one
-// round of tiles shows its epilogue: 8192 x 512 twice by K = 2048 with the saved planes takes 32 us, 10 of them for 34 MB of outputs.
+// Bound by the tensor cores at the clock that the power limit leaves: 16384 x 4096 by K = 4096 in 8 bits 170 us = 3.2 Pop/s in a
+// burst and 195 us = 2.8 Pop/s held for seconds (tensor pipe 89 % active), 8192 x 14336 twice by K = 4096 in bf16 with the saved
+// planes 1.34 ms = 1.44 PFLOP/s in a burst.  A product of one round of tiles shows its epilogue: 8192 x 512 twice by K = 2048 with
+// the saved planes takes 33 us, 10 of them for 34 MB of outputs.
 // Pairs rather than single blocks: each SM reads half as much of B from shared memory and L2.
 #include "dense.cuh"
 

@@ -11,8 +11,9 @@ The modules over them are ``linear.W8A8Linear`` and ``ffn.GatedFeedForward`` / `
 serve as ``shared_expert`` of the MoE modules.
 
 All work goes to the current stream of the tensors' device, whichever device is current; nothing synchronises and every
-buffer comes from torch's allocator.  The 8-bit operators have no gradients: their results never require one.  Errors follow
-``kernels``: ``DmoqError`` for tensors that are not on a CUDA device, ``TypeError`` for a wrong dtype, ``ValueError`` for shapes.
+buffer comes from torch's allocator.  The 8-bit operators have no gradients: their results never require one and carry no
+tangent.  Errors follow ``kernels``: ``DmoqError`` for tensors that are not on a CUDA device, for calls inside a trace and for
+inner sizes above 131056 of an 8-bit product, ``TypeError`` for a wrong dtype, ``ValueError`` for all other shapes.
 """
 from __future__ import annotations
 
@@ -128,7 +129,7 @@ def _ptr(t: Optional[torch.Tensor]):
 def quantize_int8_tokens(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """Symmetric 8-bit codes of each row of ``x`` (..., K): scale = max|x| / 127 in fp32, code = rint(127 x / max|x|) with ties
     to even, correctly rounded.  A row of zeros has scale 0; a row with an infinity or a NaN has codes 0 and scale NaN, so
-    that what is computed from it is NaN.  Returns (int8 (..., K), fp32 (...)).  K is a multiple of 16."""
+    that what is computed from it is NaN.  Returns (int8 (..., K), fp32 (...)).  K is a multiple of 16, at most 2^30."""
     _check_input(x)
     k = x.shape[-1]
     _check_k8(k)
@@ -143,7 +144,7 @@ def int8_matmul(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, 
                 bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """out[t, n] = scale[t] * weight_scale[n] * sum_k codes[t, k] * weight[n, k] (+ bias[n]); exact int32 sums, scales and bias
     in fp32, one rounding to ``out_dtype``.  ``codes`` int8 (..., K), ``weight`` int8 (N, K); K a multiple of 16, at most
-    131056; any N."""
+    131056; any N.  Codes whose rows do not follow one another are copied first."""
     codes, t, k, scale, index = _token_codes(codes, scale, out_dtype)
     w, n, w_pitch, ws = _weight8(weight, weight_scale, k, index, "weight")
     bias, bias_ptr = _bias_ptr(bias, n, out_dtype, index)
@@ -243,10 +244,10 @@ def _ffn_forward(x: torch.Tensor, t: int, pitch: int, wg: torch.Tensor, wu: torc
 
 
 class _GatedFeedForward(torch.autograd.Function):
-    """What the gradients need of the hidden values is kept as silu(g) and u silu'(g) to 24 bits each, not as g and u in 16: dg =
-    dh * (u silu'(g)) and du = dh * silu(g) are then rounded to 16 bits (they are operands of the next products) from values
-    that carry no other rounding of that type, and backward computes no exponentials.  With h that is 8 bytes a hidden
-    value, as much as g, u, silu(g) and h in 16 bits."""
+    """What the gradients need of the hidden values is kept as silu(g) and u silu'(g) in the upper 24 bits of their floats, not as
+    g and u in 16: dg = dh * (u silu'(g)) and du = dh * silu(g) are then rounded to 16 bits (they are operands of the next
+    products) from values that carry no other rounding of that type, and backward computes no exponentials.  With h that is
+    8 bytes a hidden value, as much as g, u, silu(g) and h in 16 bits."""
 
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down):
@@ -304,8 +305,9 @@ def _ffn_backward(ctx, dy):
     dwg = dw[0] if need_g else None
     dwu = dw[-1] if need_u else None
     dwd = x.new_empty((hidden, inter)) if need_d else None
-    _call("dmoq_gated_ffn_backward", x.get_device(), dy.data_ptr(), dy_pitch, x.data_ptr(), x.dtype is _BF16, x_pitch, wg.data_ptr(),
-          gate_pitch, wu.data_ptr(), up_pitch, wd.data_ptr(), down_pitch, t, hidden, inter, _ptr(h), h_pitch, _ptr(saved), _ptr(dgu), d_pitch, _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd))
+    _call("dmoq_gated_ffn_backward", x.get_device(), dy.data_ptr(), dy_pitch, x.data_ptr(), x.dtype is _BF16, x_pitch,
+          wg.data_ptr(), gate_pitch, wu.data_ptr(), up_pitch, wd.data_ptr(), down_pitch, t, hidden, inter, _ptr(h), h_pitch,
+          _ptr(saved), _ptr(dgu), d_pitch, _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(dwd))
     return dx, dwg, dwu, dwd
 
 
@@ -315,9 +317,11 @@ def _has_tangent(*tensors: torch.Tensor) -> bool:
 
 def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor) -> torch.Tensor:
     """(silu(x w_gate^T) * (x w_up^T)) w_down^T for x (..., H), w_gate and w_up (I, H), w_down (H, I), all bf16 or all fp16; H and I
-    multiples of 8.  Sums in fp32; the hidden values are rounded to the 16-bit type between the two kernels (they are the second
-    product's operand), so fp16 hidden values beyond 65504 become infinite.  Differentiable once in every argument; each gradient
-    that is not needed is not computed (at most 2^26 tokens then).  Forward-mode derivatives are refused."""
+    multiples of 8, at most 2^29.  Sums in fp32; the hidden values are rounded to the 16-bit type between the two kernels (they are
+    the second product's operand), and so are their gradients in the backward pass: beyond 65504 fp16 ones become infinite.
+    Differentiable once in every argument (a second derivative raises, forward-mode ones are refused) for at most 2^26 tokens;
+    each gradient that is not needed is not computed.  Those of w_gate and w_up are halves of one buffer: memory is given back
+    when neither is held."""
     _check_input(x)
     dt, index = x.dtype, x.get_device()
     hidden = x.shape[-1]

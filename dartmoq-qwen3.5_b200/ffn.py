@@ -4,7 +4,7 @@ Both classes hold ``gate_proj`` / ``up_proj`` / ``down_proj`` as the shared expe
 (quantization/wxa16/bit_partitioned_moe.py:1101-1106), so a state dict of such a block loads unchanged, and either serves as
 ``shared_expert`` of the MoE modules.
 
-``GatedFeedForward``       16-bit weights, differentiable
+``GatedFeedForward``       16-bit weights, differentiable when it is called by itself (the MoE modules run without gradients)
 ``W8A8GatedFeedForward``   8-bit weights and activations (one scale a weight row, one a token), inference only
 """
 from __future__ import annotations
@@ -55,7 +55,9 @@ def _projections(mlp):
 
 
 class GatedFeedForward(nn.Module):
-    """The block in bf16 or fp16; trains like the three ``nn.Linear`` it holds."""
+    """The block in bf16 or fp16; trains like the three ``nn.Linear`` it holds.  It reads their weights: hooks that are put on
+    the linears later do not run.  As ``shared_expert`` of a MoE module it is served only: those compute without gradients, so
+    it is trained by itself (against the outputs of the dense model, say) before or between."""
 
     def __init__(self, hidden_size: int, intermediate_size: int, dtype: torch.dtype = torch.bfloat16, device=None):
         super().__init__()

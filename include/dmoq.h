@@ -364,10 +364,12 @@ int dmoq_quantize_packed(const void* w, int32_t w_kind, int32_t N, int32_t K, in
  * 8-bit products: K a multiple of 16, at most 131056 (the int32 sums are exact); any number of outputs.
  *   token_quant: scales[t] = max|x[t]| / 127, codes[t][k] = rint(127 x[t][k] / max|x[t]|), ties to even, correctly rounded; a row
  *                of zeros has scale 0, a row with an infinity or NaN has codes 0 and scale NaN
- *   int8_gemm:   out[t][n] = scales[t] w_scale[n] sum_k codes[t][k] w[n][k] (+ bias[n]), rounded once to 16 bits
+ *   int8_gemm:   out[t][n] = scales[t] w_scale[n] sum_k codes[t][k] w[n][k] (+ bias[n]), rounded once to 16 bits; any scales,
+ *                also where their product is no normal 32-bit number
  *   int8_gated_gemm: out = silu(g) u, g and u the products with w_gate and w_up, rounded once
  *   int8_linear, int8_gated_linear: the same with token_quant in front; scratch (16-byte aligned, for the codes and scales) has
- *                int8_scratch_bytes(T, N or I, K, 0 or 1) bytes, which is 0 where the tokens are few enough for the product to make their codes
+ *                int8_scratch_bytes(T, N or I, K, 0 or 1) bytes, which is 0 where the tokens are few enough for the product to
+ *                make their codes
  */
 int dmoq_token_quant(const void* x, int32_t is_bf16, int32_t T, int32_t K, int64_t x_pitch, int8_t* codes, float* scales,
                      void* stream);
@@ -376,27 +378,31 @@ int dmoq_int8_gemm(const int8_t* codes, const float* scales, const int8_t* w, in
 int dmoq_int8_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w, int64_t w_pitch, const float* w_scale,
                      const void* bias, int32_t T, int32_t N, int32_t K, void* scratch, void* out, void* stream);
 int dmoq_int8_gated_gemm(const int8_t* codes, const float* scales, const int8_t* w_gate, int64_t gate_pitch,
-                         const float* gate_scale, const int8_t* w_up, int64_t up_pitch, const float* up_scale, int32_t is_bf16, int32_t T, int32_t I, int32_t K, void* out,
-                         void* stream);
+                         const float* gate_scale, const int8_t* w_up, int64_t up_pitch, const float* up_scale, int32_t is_bf16,
+                         int32_t T, int32_t I, int32_t K, void* out, void* stream);
 int dmoq_int8_gated_linear(const void* x, int32_t is_bf16, int64_t x_pitch, const int8_t* w_gate, int64_t gate_pitch,
-                           const float* gate_scale, const int8_t* w_up, int64_t up_pitch, const float* up_scale, int32_t T, int32_t I, int32_t K, void* scratch,
-                           void* out, void* stream);
+                           const float* gate_scale, const int8_t* w_up, int64_t up_pitch, const float* up_scale, int32_t T,
+                           int32_t I, int32_t K, void* scratch, void* out, void* stream);
 size_t dmoq_int8_scratch_bytes(int32_t T, int32_t N, int32_t K, int32_t gated);
 
 /*
- * Gated feed-forward block: h = silu(x w_gate^T) * (x w_up^T), y = h w_down^T; x, y (T, H), w_gate and w_up (I, H), w_down (H, I),
- * h (T, I); H and I multiples of 8.  saved (optional), three planes (T, I) of 16 bits, receives what the gradients need: the upper
- * 24 bits of the 32-bit silu(g) and u silu'(g) (upper halves in planes 0 and 1, the next eight bits of both in plane 2).
- * backward (at most 2^26 tokens): dh = dy w_down, dg = dh * u silu'(g), du = dh * silu(g); d_gate_up (T, 2 I) scratch = [dg | du].  Pitches of h and
- * d_gate_up that are multiples of 64 keep their rows on whole 128-byte lines;
+ * Gated feed-forward block: h = silu(x w_gate^T) * (x w_up^T), y = h w_down^T; x, y (T, H), w_gate and w_up (I, H),
+ * w_down (H, I), h (T, I); H and I multiples of 8, at most 2^29.  saved (optional), three planes (T, I) of 16 bits, receives what
+ * the gradients need: the upper 24 bits of the 32-bit silu(g) and u silu'(g) (upper halves in planes 0 and 1, the next eight
+ * bits of both in plane 2).
+ * backward (at most 2^26 tokens): dh = dy w_down, dg = dh * u silu'(g), du = dh * silu(g); d_gate_up (T, 2 I) scratch =
+ * [dg | du].  Pitches of h and d_gate_up that are multiples of 64 keep their rows on whole 128-byte lines;
  *   dx = dg w_gate + du w_up, dw_gate = dg^T x, dw_up = du^T x, dw_down = dy^T h.  Outputs that are NULL are not computed, and
  *   what only they need may be NULL too.  dw_up = dw_gate + H * I elements lets one product compute both.
  */
 int dmoq_gated_ffn(const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate, int64_t gate_pitch, const void* w_up,
-                   int64_t up_pitch, const void* w_down, int64_t down_pitch, int32_t T, int32_t H, int32_t I, void* h, int64_t h_pitch, void* saved, void* y, void* stream);
-int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const void* x, int32_t is_bf16, int64_t x_pitch, const void* w_gate,
-                            int64_t gate_pitch, const void* w_up, int64_t up_pitch, const void* w_down, int64_t down_pitch, int32_t T, int32_t H, int32_t I, const void* h, int64_t h_pitch,
-                            const void* saved, void* d_gate_up, int64_t d_pitch, void* dx, void* dw_gate, void* dw_up, void* dw_down, void* stream);
+                   int64_t up_pitch, const void* w_down, int64_t down_pitch, int32_t T, int32_t H, int32_t I, void* h,
+                   int64_t h_pitch, void* saved, void* y, void* stream);
+int dmoq_gated_ffn_backward(const void* dy, int64_t dy_pitch, const void* x, int32_t is_bf16, int64_t x_pitch,
+                            const void* w_gate, int64_t gate_pitch, const void* w_up, int64_t up_pitch, const void* w_down,
+                            int64_t down_pitch, int32_t T, int32_t H, int32_t I, const void* h, int64_t h_pitch,
+                            const void* saved, void* d_gate_up, int64_t d_pitch, void* dx, void* dw_gate, void* dw_up,
+                            void* dw_down, void* stream);
 
 #ifdef __cplusplus
 }
