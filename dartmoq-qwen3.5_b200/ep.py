@@ -188,7 +188,8 @@ class ExpertParallelMoE(torch.nn.Module):
         self.num_experts, self.top_k = num_experts, top_k
         self.shared_expert, self.shared_expert_gate = shared_expert, shared_expert_gate
         self.group, self.exchange = group, exchange
-        # [module or None, the shared expert and the local module's class it was made from]; a list keeps them out of the submodules
+        # [module or None, what it was made from: the shared expert, its projections, the local module's class]; a list keeps them
+        # out of the submodules
         self._shared_layer: list = []
         self._side_stream: list = []
         self._codes: list = []                # the code exchange's state
@@ -215,14 +216,17 @@ class ExpertParallelMoE(torch.nn.Module):
         caller then applies the torch modules)."""
         if self.shared_expert is None or self.shared_expert_gate is None or not x.is_cuda or x.shape[0] == 0:
             return None
+        from .moe import _shared_parts
+
         lm = self.local_moe
         made = self._shared_layer
-        if not made or made[1] is not self.shared_expert or made[2] is not type(lm):
+        source = (self.shared_expert, _shared_parts(self.shared_expert), type(lm))
+        if not made or made[1] != source:
             made.clear()                      # the old layer's memory is given back first
             layer = type(lm)(None, 1, lm.hidden_size, lm.intermediate_size, 1, self.shared_expert,
                              self.shared_expert_gate)
             layer.enable_timing = False
-            made += [layer if layer._shared_packs() is not None else None, self.shared_expert, type(lm)]
+            made += [layer if layer._shared_packs() is not None else None, source]
         layer = made[0]
         if layer is None:
             return None

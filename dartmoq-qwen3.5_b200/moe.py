@@ -312,6 +312,7 @@ class _Engine:
 
         # modules this engine and the graphs captured from it were made with; _get_engine looks for others in their place
         self.gate, self.shared_expert, self.shared_gate = m.gate, m.shared_expert, m.shared_expert_gate
+        self.shared_parts = _shared_parts(m.shared_expert)
         shared_packs = m._shared_packs()
         self.has_shared = shared_packs is not None
         self.shared_torch = (m.shared_expert is not None and m.shared_expert_gate is not None
@@ -711,6 +712,12 @@ class _EventProfiler:
 
 # =========================================================================== modules
 
+def _shared_parts(expert) -> tuple:
+    """A shared expert's gate, up and down projection; None for one that it lacks.  (Modules compare by identity.)"""
+    held = getattr(expert, "_modules", None) or {}
+    return tuple(held[n] if n in held else getattr(expert, n, None) for n in ("gate_proj", "up_proj", "down_proj"))
+
+
 class WxA16BitPartitionedGroupMoE(nn.Module):
     """Bit-partitioned MoE over packed weights, fp16 activations."""
 
@@ -842,7 +849,7 @@ class WxA16BitPartitionedGroupMoE(nn.Module):
         se = self.shared_expert
         if se is None or self.shared_expert_gate is None:
             return None
-        parts = [getattr(se, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
+        parts = _shared_parts(se)
         if any(p is None or not hasattr(p, "packed_indices") for p in parts):
             return None
         g, u, d = parts
@@ -863,7 +870,8 @@ class WxA16BitPartitionedGroupMoE(nn.Module):
         eng = self._engine
         if eng is not None:
             shared, gate = self.shared_expert, self.shared_expert_gate
-            if eng.shared_expert is not shared or (eng.shared_gate is None) != (gate is None):
+            if (eng.shared_expert is not shared or (eng.shared_gate is None) != (gate is None)
+                    or eng.has_shared and eng.shared_parts != _shared_parts(shared)):
                 if eng.has_shared or self._shared_packs() is not None:
                     eng = None                        # packed weights that the engine holds, or would
                 else:

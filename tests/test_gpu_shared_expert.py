@@ -129,3 +129,28 @@ def test_expert_parallel_shared_expert_replaced():
     D.WxA8BitPartitionedGroupMoE.from_wxa16(w.local_moe)
     eight = wrap(a.shared_expert, D.WxA8BitPartitionedGroupMoE)._shared_partial(x)
     assert not torch.equal(eight, first) and torch.equal(w._shared_partial(x), eight)
+
+
+def test_projections_of_a_packed_expert_replaced():
+    """One of the packed expert's projections put in another's place, or a dense one: never the old weights."""
+    from dartmoq_b200 import ep
+    x = tokens()
+    moe, fresh, other = layer(shared_inter=128), layer(shared_inter=128), layer(seed=6, shared_inter=128)
+    wrap = ep.ExpertParallelMoE(moe.gate, ep.shard_experts(moe, 0, 8), 8, 2, moe.shared_expert, moe.shared_expert_gate)
+    first, alone = moe(x).clone(), wrap._shared_partial(x[0]).clone()
+    calls(moe, x, first)
+    moe.shared_expert.down_proj = fresh.shared_expert.down_proj = other.shared_expert.down_proj
+    want = fresh(x).clone()
+    assert not torch.equal(want, first)
+    calls(moe, x, want)
+    again = ep.ExpertParallelMoE(moe.gate, ep.shard_experts(moe, 0, 8), 8, 2, moe.shared_expert, moe.shared_expert_gate)
+    assert not torch.equal(again._shared_partial(x[0]), alone)
+    assert torch.equal(wrap._shared_partial(x[0]), again._shared_partial(x[0]))
+    torch.manual_seed(9)
+    dense = D.W8A8Linear.from_linear(torch.nn.Linear(128, HIDDEN, bias=False, dtype=torch.bfloat16, device=DEV))
+    moe.shared_expert.down_proj = dense
+    plain = layer(shared_inter=128)
+    plain.shared_expert = None
+    routed = plain(x).clone()
+    calls(moe, x, with_dense(routed, x, moe.shared_expert, moe.shared_expert_gate))
+    assert wrap._shared_partial(x[0]) is None       # the caller applies the module
