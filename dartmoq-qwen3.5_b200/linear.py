@@ -91,6 +91,10 @@ class WxA16Linear(nn.Module):
         self._rt = None
         return ret
 
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        self._rt = None
+
     def _runtime(self, device):
         rt = self._rt
         if rt is not None and rt["device"] == device:

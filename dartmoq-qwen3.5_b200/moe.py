@@ -75,6 +75,10 @@ class WxA16Weights(nn.Module):
         self._cache = {"gate_up": None, "down": None}
         return ret
 
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        self._cache = {"gate_up": None, "down": None}
+
     def _packed(self, side: str) -> dict:
         d = self._cache[side]
         if d is None:
@@ -754,10 +758,17 @@ class WxA16BitPartitionedGroupMoE(nn.Module):
     # ------------------------------------------------------------------ construction
     def _apply(self, fn, *args, **kwargs):
         ret = super()._apply(fn, *args, **kwargs)
+        self._drop_caches()
+        return ret
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        self._drop_caches()           # the engine's weights are copies, captured graphs hold addresses
+
+    def _drop_caches(self):
         for attr in self._DEVICE_CACHE_ATTRS:
             if hasattr(self, attr):
                 setattr(self, attr, None)
-        return ret
 
     @classmethod
     @torch.no_grad()

@@ -154,3 +154,27 @@ def test_projections_of_a_packed_expert_replaced():
     routed = plain(x).clone()
     calls(moe, x, with_dense(routed, x, moe.shared_expert, moe.shared_expert_gate))
     assert wrap._shared_partial(x[0]) is None       # the caller applies the module
+
+
+@pytest.mark.parametrize("assign", (False, True))
+@pytest.mark.parametrize("n", (40, 700))
+def test_a_state_dict_loaded_after_calls_is_used(n, assign):
+    """The engine's weights are copies and captured graphs hold addresses: both are made anew after a load."""
+    x, bits = tokens(n), [2, 4, 2, 4, 4, 2, 2, 4]
+    a, b, c = layer(expert_bits=bits), layer(seed=6, expert_bits=bits), layer(expert_bits=bits)
+    first = a(x).clone()
+    calls(a, x, first)
+    c.load_state_dict(b.state_dict())               # before its first call
+    want = c(x).clone()
+    assert not torch.equal(want, first)
+    a.load_state_dict({k: v.clone() for k, v in b.state_dict().items()}, assign=assign)
+    calls(a, x, want)
+    for bit, w in a.bit_weights.items():
+        for side in ("gate_up", "down"):
+            pk = getattr(w, side + "_packed")
+            assert pk["norms"] is getattr(w, side + "_norms")
+    lin, other = (layer(seed=s, shared_inter=128).shared_expert.gate_proj for s in (5, 6))
+    fresh = D.WxA16Linear(other.in_features, other.out_features, 8, 128, other.packed_indices, other.codebook, other.norms, lin.seed)
+    lin(x[0])
+    lin.load_state_dict({k: v.clone() for k, v in other.state_dict().items()}, assign=assign)
+    assert torch.equal(lin(x[0]), fresh(x[0]))
