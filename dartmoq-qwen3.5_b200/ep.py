@@ -206,6 +206,14 @@ class ExpertParallelMoE(torch.nn.Module):
         self.last_stage_ms = None
         self.last_launches = 0
 
+    def _apply(self, fn, *args, **kwargs):
+        self._shared_layer.clear()            # a layer's engine holds copies of the weights
+        return super()._apply(fn, *args, **kwargs)
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        self._shared_layer.clear()
+        super()._load_from_state_dict(*args, **kwargs)
+
     def _local_partial(self, x_all, w_all, local_idx):
         eng = self.local_moe._get_engine(x_all.device)
         return eng.run(x_all, w_all, local_idx, None)

@@ -178,3 +178,21 @@ def test_a_state_dict_loaded_after_calls_is_used(n, assign):
     lin(x[0])
     lin.load_state_dict({k: v.clone() for k, v in other.state_dict().items()}, assign=assign)
     assert torch.equal(lin(x[0]), fresh(x[0]))
+
+
+@pytest.mark.parametrize("assign", (False, True))
+def test_expert_parallel_weights_loaded_after_calls(assign):
+    from dartmoq_b200 import ep
+    x, bits = tokens()[0], [2, 4, 2, 4, 4, 2, 2, 4]
+    a, b = layer(shared_inter=128, expert_bits=bits), layer(shared_inter=128, seed=6, expert_bits=bits)
+    for u, v in zip(a.shared_expert.children(), b.shared_expert.children()):
+        v.seed = u.seed                             # rotations are not part of a state dict
+
+    def wrap(m):
+        return ep.ExpertParallelMoE(m.gate, ep.shard_experts(m, 0, 8), 8, 2, m.shared_expert, m.shared_expert_gate)
+
+    w, other = wrap(a), wrap(b)
+    first, want = w._shared_partial(x).clone(), other._shared_partial(x).clone()
+    assert not torch.equal(first, want)
+    w.load_state_dict({k: v.clone() for k, v in other.state_dict().items()}, assign=assign)
+    assert torch.equal(w._shared_partial(x), want)
