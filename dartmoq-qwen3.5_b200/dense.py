@@ -28,13 +28,22 @@ _BF16, _FP16, _FP32, _INT8 = torch.bfloat16, torch.float16, torch.float32, torch
 _MAX_ROWS = 1 << 30
 _MAX_SIDE = 1 << 29          # of a feed-forward block
 _MAX_GRAD_TOKENS = 1 << 26
-_PROXY = torch._C._TorchDispatchModeKey.PROXY
+_tracing, _modes, _mode, _PROXY = (torch._C._get_tracing_state, torch._C._len_torch_dispatch_stack, torch._C._get_dispatch_mode,
+                                   torch._C._TorchDispatchModeKey.PROXY)
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
+_entries: dict = {}
+
+
+def _entry(name: str):
+    fn = _entries[name] = getattr(_lib.load(), name)
+    return fn
 
 
 def _call(name: str, index: int, *args) -> None:
     """One entry point on the current stream of device ``index``, which is current during the call."""
-    fn = getattr(_lib.load(), name)
+    fn = _entries.get(name) or _entry(name)
     if index == _current_device():
         rc = fn(*args, _raw_stream(index))
     else:
@@ -75,7 +84,7 @@ def _need(cond: bool, message: str) -> None:
 
 def _check_cuda(t: torch.Tensor) -> None:
     # a trace (torch.jit or torch.fx) would hold the outputs' allocation and not the call that fills them
-    if torch._C._get_tracing_state() is not None or (torch._C._len_torch_dispatch_stack() and torch._C._get_dispatch_mode(_PROXY) is not None):
+    if _tracing() is not None or (_modes() and _mode(_PROXY) is not None):
         raise _lib.DmoqError("libdmoq operators cannot be traced")
     if not t.is_cuda:
         raise _lib.DmoqError("libdmoq operators take CUDA tensors only (no CPU path)")
@@ -208,7 +217,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
 
 
 def _int8_scratch(x: torch.Tensor, t: int, n: int, k: int, gated: bool) -> Optional[torch.Tensor]:
-    need = _lib.load().dmoq_int8_scratch_bytes(t, n, k, gated)
+    need = (_entries.get("dmoq_int8_scratch_bytes") or _entry("dmoq_int8_scratch_bytes"))(t, n, k, gated)
     return x.new_empty((need,), dtype=torch.uint8) if need else None
 
 
